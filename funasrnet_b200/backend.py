@@ -57,6 +57,7 @@ class CudaFloatBackend:
         h = C.c_void_p()
         check(lib().fa_backend_create(device, C.byref(h)))
         self._h = h
+        self.device = device
         self._lock = threading.Lock()
         self._resident: "weakref.WeakKeyDictionary[Weight, C.c_void_p]" = weakref.WeakKeyDictionary()
         self._disposed = False

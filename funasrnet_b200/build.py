@@ -26,7 +26,8 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # path as unreachable and drops it.
 NVCC_FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-fmad=false", "-Xcompiler", "-fPIC,-O3,-ffp-contract=off",
                      "-Xptxas", "-v", "-diag-error", "20011,20012,20013,20014,20015"]
-SOURCES = ["decoder_kernels.cu", "mega.cu", "batch.cu", "f32_stream.cu", "runtime.cu", "host_util.cpp"]
+SOURCES = ["decoder_kernels.cu", "mega.cu", "batch.cu", "f32_stream.cu", "dev_attention.cu", "dev_logits.cu",
+           "runtime.cu", "host_util.cpp"]
 
 
 def nvcc() -> str:

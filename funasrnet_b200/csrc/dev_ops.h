@@ -1,0 +1,36 @@
+// The device-pointer operators behind fa_dev_* (dev_attention.cu, dev_logits.cu).
+// Argument structs are the C ABI's; the launchers expect them checked.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include "../../include/funasr_cuda.h"
+#include "fa_common.h"
+
+namespace fa {
+
+// The structs as hosts in other languages lay them out: no padding.
+static_assert(sizeof(fa_attention_packed_args) == 184 && sizeof(fa_attention_shared_args) == 232 &&
+                  sizeof(fa_logits_args) == 168,
+              "argument struct layout");
+
+// kHandled, or kDeclined for sizes and alignments outside the kernels; throws
+// on inconsistent arguments.  Host checks only: no device is needed.
+int check_attention_packed(const fa_attention_packed_args* a);
+int check_attention_shared(const fa_attention_shared_args* a);
+int check_logits(const fa_logits_args* a);
+
+int64_t attention_packed_workspace(int64_t total_q, int64_t total_k, int sequences, int heads, int kv_heads,
+                                   int head_size);
+int64_t attention_shared_workspace(int64_t prefix_len, int64_t suffix_capacity, int sequences, int heads, int kv_heads,
+                                   int head_size);
+
+void launch_attention_packed(const fa_attention_packed_args& a, cudaStream_t stream);
+void launch_attention_shared(const fa_attention_shared_args& a, cudaStream_t stream);
+void launch_adjust_logits(const fa_logits_args& a, cudaStream_t stream);
+
+// Waits for the device, then the error word of its current context's kernels
+// (0: no bounded wait gave up), cleared by the read.
+int take_device_error();
+
+}  // namespace fa

@@ -19,6 +19,7 @@
 
 #include "../../include/funasr_cuda.h"
 #include "batch.h"
+#include "dev_ops.h"
 #include "fa_common.h"
 #include "gguf.h"
 #include "kernels.h"
@@ -709,6 +710,60 @@ int fa_lm_head_argmax_noalloc(fa_backend* b, const fa_weight* w, const float* x,
     launch_gemv(a, st);
     return (int)kHandled;
   });
+}
+
+// ------------------------------------------------ device-pointer operators ----
+
+}  // extern "C"
+
+// The arguments are checked before the backend, so that a refusal needs no device.
+template <typename Args>
+static int enqueue_dev(fa_backend* b, const Args* args, void* stream, int (*check)(const Args*),
+                       void (*launch)(const Args&, cudaStream_t)) {
+  return guarded([&] {
+    const int rc = check(args);
+    if (rc != kHandled) return rc;
+    check_backend(b);
+    std::lock_guard<std::mutex> lk(b->mu);
+    if (b->disposed) throw Error(kErrDisposed, "backend disposed");
+    DeviceGuard g(b->device);
+    launch(*args, stream != nullptr ? static_cast<cudaStream_t>(stream) : b->stream);
+    return (int)kHandled;
+  });
+}
+
+extern "C" {
+
+int fa_dev_status(fa_backend* b) {
+  return guarded([&] {
+    check_backend(b);
+    DeviceGuard g(b->device);
+    const int code = take_device_error();
+    if (code != 0) throw Error(kErrTimeout, "a bounded device wait gave up (code " + std::to_string(code) + ")");
+    return (int)kHandled;
+  });
+}
+
+int fa_dev_attention_packed(fa_backend* b, const fa_attention_packed_args* args, void* stream) {
+  return enqueue_dev(b, args, stream, check_attention_packed, launch_attention_packed);
+}
+
+int64_t fa_dev_attention_packed_workspace(int64_t total_q, int64_t total_k, int sequences, int heads, int kv_heads,
+                                          int head_size) {
+  return attention_packed_workspace(total_q, total_k, sequences, heads, kv_heads, head_size);
+}
+
+int fa_dev_attention_shared(fa_backend* b, const fa_attention_shared_args* args, void* stream) {
+  return enqueue_dev(b, args, stream, check_attention_shared, launch_attention_shared);
+}
+
+int64_t fa_dev_attention_shared_workspace(int64_t prefix_len, int64_t suffix_capacity, int sequences, int heads,
+                                          int kv_heads, int head_size) {
+  return attention_shared_workspace(prefix_len, suffix_capacity, sequences, heads, kv_heads, head_size);
+}
+
+int fa_dev_adjust_logits(fa_backend* b, const fa_logits_args* args, void* stream) {
+  return enqueue_dev(b, args, stream, check_logits, launch_adjust_logits);
 }
 
 int fa_synth_write_gguf(const char* path, uint64_t seed, int layers, int vocab, int width, int ffn, int quantized) {

@@ -312,6 +312,148 @@ int fa_batch_last_ms(const fa_batch* batch, float* ms);
 int fa_lm_head_argmax_noalloc(fa_backend* backend, const fa_weight* weight, const float* x, const float* gamma,
                               float eps, float* logits, int32_t* token, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Device-pointer operators.  They have no counterpart in the reference, whose
+ * decoder handles one context at a time and picks its tokens greedily; a server
+ * that decodes many FunAsr contexts on one GPU needs them around that step:
+ * attention over several prompts at once, attention of a batch that shares its
+ * prompt prefix (FunAsr.cs:134-138 caches one), and the changes to the logits
+ * that hot words, grammars and penalties ask for before the greedy pick.
+ *
+ * Conventions of this group
+ *  - Every pointer inside the argument structs is a device pointer on the
+ *    backend's device; the struct itself is host memory, read during the call.
+ *  - A call enqueues its kernels on `stream` (a cudaStream_t; NULL selects the
+ *    backend's own stream, as fa_lm_head_argmax_noalloc does; cudaStreamLegacy
+ *    names the default stream) and returns; the caller synchronises.
+ *  - Nothing is allocated, so calls can be captured into a CUDA graph.  A call
+ *    that needs scratch memory takes it from `workspace`, whose contents need no
+ *    preparation and mean nothing afterwards; calls that may overlap in time
+ *    (on two streams, in two graphs) need a workspace each.
+ *  - Strides count elements.  The innermost dimension is contiguous.
+ *  - FA_DECLINED, with the outputs untouched, for shapes and alignments outside
+ *    the limits given at each call; FA_ERR_ARGUMENT for inconsistent arguments.
+ *  - Offsets and lengths are read on the device and clamped to the extents that
+ *    the struct gives: wrong ones give unspecified results, never an access
+ *    outside the arrays.
+ *  - A device wait that gave up (a fault of this library) is reported by
+ *    fa_dev_status.
+ * ------------------------------------------------------------------------ */
+#define FA_DTYPE_F32 0
+#define FA_DTYPE_F16 1
+#define FA_DTYPE_BF16 2
+
+/* Waits for the device, then FA_OK, or FA_ERR_TIMEOUT when a bounded wait of one
+ * of the operators below gave up since the last call (its outputs are invalid). */
+int fa_dev_status(fa_backend* backend);
+
+/* Attention of several packed sequences.  Sequence b has the queries
+ * q_offsets[b] .. q_offsets[b+1] and the keys k_offsets[b] .. k_offsets[b+1];
+ * with L queries and K keys, query i of it sees
+ *     all K keys (causal == 0), or its first i + K - L + 1 (causal != 0):
+ * the queries are the last L positions of the sequence, so a whole prompt has
+ * L == K and a later chunk of it has K > L.
+ *     out = sum_j softmax_j(scale * q . k_j) v_j,  lse = log sum_j exp(scale * q . k_j)
+ * A query that sees no key gets out = 0 and lse = -inf.  Query head h reads KV
+ * head h / (heads / kv_heads).  Scores, softmax statistics and sums are 32-bit;
+ * the probabilities are rounded to the type of v for their product with it.
+ * Rows of out and lse outside q_offsets[0] .. q_offsets[sequences] stay as they were.
+ * Limits (else FA_DECLINED): FA_DTYPE_F16 or FA_DTYPE_BF16; head_size a multiple
+ * of 8 up to 128; heads / kv_heads up to 64; every base address and stride a
+ * multiple of 16 bytes (the stride of a dimension of length one counts too); total_q * heads and total_k below 2^31. */
+typedef struct fa_attention_packed_args {
+  const void* q;            /* [total_q x heads x head_size] */
+  const void* k;            /* [total_k x kv_heads x head_size] */
+  const void* v;
+  void* out;                /* [total_q x heads x head_size] */
+  float* lse;               /* [total_q x heads], contiguous, or NULL */
+  const int32_t* q_offsets; /* [sequences + 1], not decreasing */
+  const int32_t* k_offsets;
+  void* workspace;          /* fa_dev_attention_packed_workspace bytes, 16-byte aligned */
+  int64_t workspace_bytes;
+  int64_t q_stride[2];      /* token, head */
+  int64_t k_stride[2];
+  int64_t v_stride[2];
+  int64_t out_stride[2];
+  int64_t total_q, total_k;
+  int32_t dtype, sequences, heads, kv_heads, head_size, causal;
+  float scale;
+  int32_t reserved;         /* 0 */
+} fa_attention_packed_args;
+int fa_dev_attention_packed(fa_backend* backend, const fa_attention_packed_args* args, void* stream);
+/* Bytes of workspace a call of these sizes needs (0: none). */
+int64_t fa_dev_attention_packed_workspace(int64_t total_q, int64_t total_k, int sequences, int heads, int kv_heads,
+                                          int head_size);
+
+/* Attention of one query token per sequence over a prefix that all sequences
+ * share followed by the sequence's own keys: what decoding sessions of one
+ * prompt computes (fa_session_share_prefix), with the prefix stored and read once
+ * for the whole batch.  Sequence b sees the prefix_len prefix keys and the first
+ * suffix_lens[b] of its suffix_capacity own ones (what lies behind is not used).
+ * Formula, precision, empty rows and limits as fa_dev_attention_packed. */
+typedef struct fa_attention_shared_args {
+  const void* q;               /* [sequences x heads x head_size] */
+  const void* prefix_k;        /* [prefix_len x kv_heads x head_size] */
+  const void* prefix_v;
+  const void* suffix_k;        /* [sequences x suffix_capacity x kv_heads x head_size] */
+  const void* suffix_v;
+  void* out;                   /* [sequences x heads x head_size] */
+  float* lse;                  /* [sequences x heads], contiguous, or NULL */
+  const int32_t* suffix_lens;  /* [sequences] */
+  void* workspace;             /* fa_dev_attention_shared_workspace bytes, 16-byte aligned */
+  int64_t workspace_bytes;
+  int64_t q_stride[2];         /* sequence, head */
+  int64_t prefix_k_stride[2];  /* position, head */
+  int64_t prefix_v_stride[2];
+  int64_t suffix_k_stride[3];  /* sequence, position, head */
+  int64_t suffix_v_stride[3];
+  int64_t out_stride[2];       /* sequence, head */
+  int64_t prefix_len, suffix_capacity;
+  int32_t dtype, sequences, heads, kv_heads, head_size;
+  float scale;
+} fa_attention_shared_args;
+int fa_dev_attention_shared(fa_backend* backend, const fa_attention_shared_args* args, void* stream);
+int64_t fa_dev_attention_shared_workspace(int64_t prefix_len, int64_t suffix_capacity, int sequences, int heads,
+                                          int kv_heads, int head_size);
+
+/* What changes the logits between the lm_head and the greedy pick
+ * (QwenDecoder.cs:262-268, 278-326), and that pick.  For every row, in 32 bits
+ * and in this order:
+ *     x > 0 ? x / repetition : x * repetition   tokens anywhere in the row's history
+ *     x - (frequency * n + presence)            tokens that its generated part holds n > 0 times
+ *     x + bias                                  tokens of its bias list (the last entry of a token counts)
+ *     -inf                                      tokens whose bit in its mask is 0
+ * out gets the result in the type of the logits (it may be the logits themselves);
+ * tokens gets the lowest index of the row's largest 32-bit value, -1 when no
+ * value is above -inf (NaN is above nothing).  A row's history is history_offsets[r] ..
+ * history_offsets[r+1]; its first prompt_lens[r] tokens are the prompt, the rest
+ * was generated.  Ids outside the vocabulary are ignored.  Bit t % 32 of word
+ * t / 32 of mask row mask_rows[r] allows token t; a negative or too large
+ * mask_rows[r] allows every token.
+ * Limits (else FA_DECLINED): vocab up to FA_LOGITS_MAX_VOCAB. */
+#define FA_LOGITS_MAX_VOCAB 16777216
+typedef struct fa_logits_args {
+  const void* logits;               /* [rows x vocab] */
+  void* out;                        /* [rows x vocab] */
+  int32_t* tokens;                  /* [rows], or NULL */
+  const int32_t* history;           /* [history_total], or NULL: no history */
+  const int32_t* history_offsets;   /* [rows + 1], not decreasing */
+  const int32_t* prompt_lens;       /* [rows], or NULL: all generated */
+  const float* repetition;          /* [rows], or NULL: 1 */
+  const float* presence;            /* [rows], or NULL: 0 */
+  const float* frequency;           /* [rows], or NULL: 0 */
+  const int32_t* bias_tokens;       /* [bias_total], or NULL: no biases */
+  const float* bias_values;         /* [bias_total] */
+  const int32_t* bias_offsets;      /* [rows + 1], not decreasing */
+  const uint32_t* mask;             /* [mask_count x mask_stride], or NULL: every token allowed */
+  const int32_t* mask_rows;         /* [rows], or NULL: row r has mask row r */
+  int64_t logits_stride, out_stride;/* elements between rows */
+  int64_t mask_stride;              /* words between mask rows */
+  int64_t history_total, bias_total;
+  int32_t dtype, rows, vocab, mask_count;
+} fa_logits_args;
+int fa_dev_adjust_logits(fa_backend* backend, const fa_logits_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
