@@ -1144,10 +1144,10 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 }
 
 void encode_tensor_map(CUtensorMap* m, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims,
-                       const cuuint64_t* strides, const cuuint32_t* box) {
-  const cuuint32_t estr[3] = {1, 1, 1};
+                       const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   const CUresult r = encode_fn()(m, type, rank, const_cast<void*>(base), dims, strides, box, estr,
-                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) throw Error(kErrCuda, "cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
 }
