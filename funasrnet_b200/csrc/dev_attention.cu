@@ -52,60 +52,6 @@ bool heads_supported(int dtype, int heads, int kv_heads, int head_size) {
 
 // ------------------------------------------------------------ kernels ----
 
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, float* v) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  const T* t = reinterpret_cast<const T*>(&u);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = (float)t[i];
-}
-
-struct KvRun {
-  const void *k, *v;
-  long long k_row, v_row;  // element strides between keys
-  int n;                   // keys
-};
-
-// One warp: one query head over up to two runs of keys, lane l holding the
-// channels 4l .. 4l + 3.
-template <typename T>
-__device__ __forceinline__ void attend_row(const T* q, const KvRun* runs, int n_runs, int head_size, float scale, T* out,
-                                           float* lse) {
-  const int lane = threadIdx.x & 31, c = lane * 4;
-  const bool on = c < head_size;
-  float qv[4] = {}, o[4] = {};
-  if (on) load4(q + c, qv);
-  float m = -INFINITY, l = 0.0f;
-  for (int r = 0; r < n_runs; ++r) {
-    for (int j = 0; j < runs[r].n; ++j) {
-      float kv[4] = {}, vv[4] = {};
-      if (on) {
-        load4(static_cast<const T*>(runs[r].k) + j * runs[r].k_row + c, kv);
-        load4(static_cast<const T*>(runs[r].v) + j * runs[r].v_row + c, vv);
-      }
-      float s = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s = fmaf(qv[i], kv[i], s);
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-      s *= scale;
-      const float top = fmaxf(m, s), base = top == -INFINITY ? 0.0f : top;
-      const float f = expf(m - base), p = expf(s - base);
-      m = top;
-      l = l * f + p;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = o[i] * f + p * vv[i];
-    }
-  }
-  if (on) {
-    T t[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) t[i] = (T)(l == 0.0f ? 0.0f : o[i] / l);
-    *reinterpret_cast<uint2*>(out + c) = *reinterpret_cast<const uint2*>(t);
-  }
-  if (lse && lane == 0) *lse = (m == -INFINITY ? 0.0f : m) + logf(l);
-}
-
 __device__ __forceinline__ int clamp_to(int x, long long hi) { return (int)min((long long)max(x, 0), hi); }
 
 // -------------------------------------------------- tensor-core attention ----
@@ -130,7 +76,7 @@ struct TcArgs {
   void* out = nullptr;
   long long out_token = 0, out_head = 0;
   float* lse = nullptr;
-  float* part_o = nullptr;     // splits > 1: [splits x total_q x heads x head_size], and the rows' lse
+  float* part_o = nullptr;     // with part_o: [splits x total_q x heads x head_size], and the rows' lse
   float* part_lse = nullptr;
   int* err = nullptr;
 };
@@ -470,7 +416,7 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
 #pragma unroll
         for (int e = 0; e < 32; e += 8) {
           if (!live || k + e >= a.head_size) continue;
-          if (a.splits > 1) {
+          if (a.part_o) {
             *reinterpret_cast<float4*>(part + k + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
             *reinterpret_cast<float4*>(part + k + e + 4) = make_float4(v[e + 4], v[e + 5], v[e + 6], v[e + 7]);
           } else {
@@ -481,8 +427,8 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
         }
       }
       const float lse = (m == -INFINITY ? 0.0f : m * a.scale) + logf(l);
-      if (live && a.splits > 1) a.part_lse[split * a.total_q * a.heads + row] = lse;
-      if (live && a.splits == 1 && a.lse) a.lse[row] = lse;
+      if (live && a.part_o) a.part_lse[split * a.total_q * a.heads + row] = lse;
+      if (live && !a.part_o && a.lse) a.lse[row] = lse;
     }
   }
   ptx::tc_fence_before();
@@ -493,11 +439,265 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
   }
 }
 
+// ------------------------------------------------------ one query a sequence ----
+
+constexpr int kRowWarps = 4;   // warps of a CTA, each with its own keys and softmax state
+constexpr int kChunk = 16;     // keys per step of a warp: the MMA's M
+constexpr int kRowHeads = 8;   // query heads of a CTA: the MMA's N
+
+struct Run {  // keys and values of one KV head: row i at k + i * k_row
+  const void *k = nullptr, *v = nullptr;
+  long long k_row = 0, v_row = 0, k_head = 0, v_head = 0, k_seq = 0, v_seq = 0;
+};
+
+struct RowsArgs {
+  const void* q = nullptr;
+  long long q_seq = 0, q_head = 0;
+  Run prefix, suffix;
+  int prefix_len = 0;             // keys of the prefix that this kernel reads (0: attention_tc_kernel does)
+  const int* suffix_lens = nullptr;
+  int capacity = 0;
+  int sequences = 0, heads = 0, kv_heads = 0, group = 0, head_size = 0;
+  int blocks = 1;                 // blocks of kRowHeads heads of a group
+  int splits = 1;
+  float scale = 0.0f, scale_log2 = 0.0f;
+  void* out = nullptr;            // the result (part_o == nullptr), or parts:
+  long long out_seq = 0, out_head = 0;
+  float* lse = nullptr;
+  float* part_o = nullptr;        // [splits x sequences x heads x head_size]
+  float* part_lse = nullptr;      // [splits x sequences x heads]
+  int wait = 0;                   // the launch before this one must be over when this one is
+};
+
+// D (m16n8) += A (m16k16) x B (k16n8), f32 accumulator.
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float* d, unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
+                                         unsigned b1) {
+  if (BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 8 x 8 matrix of 16-bit values, lane (g, t) holding row g, columns 2t and 2t + 1: transposed.
+__device__ __forceinline__ unsigned transpose8(unsigned x) {
+  unsigned y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint4 load16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+// One query token of one sequence, up to 8 of the heads that share a KV head.
+// The keys stream from global memory straight into MMA operands: a warp takes
+// 16 keys a step and lane (g = lane / 4, t = lane % 4) loads
+//   K rows g and g + 8, channels 32b + 8t .. + 7   (16 bytes each),
+//   V rows 2t, 2t + 1, 2t + 8, 2t + 9, channels 64h + 8g .. + 7.
+// S^T = K Q^T sums over channels, whose order is free as long as Q has the same:
+// the four words of a 16-byte load serve as the k index of two MMAs.  O^T = V^T P^T
+// needs pairs of keys in a word: two rows' words interleaved by prmt, so that
+// the MMA of word r has channels 64h + 8g + 2r and + 2r + 1 as its rows g and g + 8.
+// P^T goes from S^T's layout to the operand's through movmatrix.  No shared
+// memory until the warps' sums are joined at the end.  Bound: the bytes of K
+// and V; the heads share them, so N = 8 serves groups up to 8 in one pass.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(32 * kRowWarps, 4) attention_rows_kernel(const RowsArgs a) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  constexpr int KB = D / 32, VB = D / 64, NO = D / 16;
+  __shared__ float sm_o[kRowWarps][kRowHeads][D + 4];
+  __shared__ float sm_m[kRowWarps][kRowHeads], sm_l[kRowWarps][kRowHeads];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  unsigned id = blockIdx.x;
+  const int kvh = id % a.kv_heads;
+  id /= a.kv_heads;
+  const int block = id % a.blocks;
+  id /= a.blocks;
+  const int split = id % a.splits;
+  const int seq = id / a.splits;
+  const int head0 = kvh * a.group + block * kRowHeads, n_heads = min(kRowHeads, a.group - block * kRowHeads);
+  const int own = a.suffix_lens ? clamp_to(a.suffix_lens[seq], a.capacity) : 0;
+  ptx::griddep_launch();
+
+  // Chunks of 16 keys: the prefix's, then the sequence's own.
+  const int pc = (a.prefix_len + kChunk - 1) / kChunk, chunks = pc + (own + kChunk - 1) / kChunk;
+  const int c0 = (int)((long long)chunks * split / a.splits), c1 = (int)((long long)chunks * (split + 1) / a.splits);
+  const T* pk = static_cast<const T*>(a.prefix.k) + kvh * a.prefix.k_head;
+  const T* pv = static_cast<const T*>(a.prefix.v) + kvh * a.prefix.v_head;
+  const T* sk = static_cast<const T*>(a.suffix.k) + seq * a.suffix.k_seq + kvh * a.suffix.k_head;
+  const T* sv = static_cast<const T*>(a.suffix.v) + seq * a.suffix.v_seq + kvh * a.suffix.v_head;
+
+  unsigned q[KB][4];  // the B operand of S^T: head g, channels 32b + 8t .. + 7
+#pragma unroll
+  for (int b = 0; b < KB; ++b) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (g < n_heads && 32 * b + 8 * t < a.head_size)
+      v = load16(static_cast<const T*>(a.q) + seq * a.q_seq + (head0 + g) * a.q_head + 32 * b + 8 * t);
+    q[b][0] = v.x;
+    q[b][1] = v.y;
+    q[b][2] = v.z;
+    q[b][3] = v.w;
+  }
+  float o[NO][4];
+#pragma unroll
+  for (int i = 0; i < NO; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};  // heads 2t, 2t + 1
+  const float c = a.scale_log2;
+
+  uint4 kx[2][KB];
+  auto load_k = [&](int ch) {
+    const bool own_keys = ch >= pc;
+    const int key0 = (own_keys ? ch - pc : ch) * kChunk, n = own_keys ? own : a.prefix_len;
+    const T* base = own_keys ? sk : pk;
+    const long long row = own_keys ? a.suffix.k_row : a.prefix.k_row;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int key = key0 + g + 8 * i;
+#pragma unroll
+      for (int b = 0; b < KB; ++b)
+        kx[i][b] = key < n && 32 * b + 8 * t < a.head_size ? load16(base + key * row + 32 * b + 8 * t)
+                                                           : make_uint4(0, 0, 0, 0);
+    }
+  };
+  int ch = c0 + warp;
+  if (ch < c1) load_k(ch);
+  for (; ch < c1; ch += kRowWarps) {
+    const bool own_keys = ch >= pc;
+    const int key0 = (own_keys ? ch - pc : ch) * kChunk, n = own_keys ? own : a.prefix_len;
+    uint4 vx[4][VB];
+    {
+      const T* base = own_keys ? sv : pv;
+      const long long row = own_keys ? a.suffix.v_row : a.prefix.v_row;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = key0 + 2 * t + (i & 1) + 8 * (i >> 1);
+#pragma unroll
+        for (int h = 0; h < VB; ++h)
+          vx[i][h] = key < n && 64 * h + 8 * g < a.head_size ? load16(base + key * row + 64 * h + 8 * g)
+                                                             : make_uint4(0, 0, 0, 0);
+      }
+    }
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // key g: heads 2t, 2t + 1; key g + 8: the same heads
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+      mma16816<BF16>(s, kx[0][b].x, kx[1][b].x, kx[0][b].y, kx[1][b].y, q[b][0], q[b][1]);
+      mma16816<BF16>(s, kx[0][b].z, kx[1][b].z, kx[0][b].w, kx[1][b].w, q[b][2], q[b][3]);
+    }
+    if (ch + kRowWarps < c1) load_k(ch + kRowWarps);
+    if (key0 + g >= n) s[0] = s[1] = -INFINITY;
+    if (key0 + g + 8 >= n) s[2] = s[3] = -INFINITY;
+    // The maximum moves only when a score is 2^kSlack above it.
+    const float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
+    if (__any_sync(0xffffffffu, x0 * c > m[0] * c + kSlack || x1 * c > m[1] * c + kSlack)) {
+      float x[2] = {x0, x1};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) x[i] = fmaxf(x[i], __shfl_xor_sync(0xffffffffu, x[i], d));
+        const float top = fmaxf(m[i], x[i]);
+        const float f = top == m[i] ? 1.0f : ptx::ex2((m[i] - top) * c);  // 0 while the sums are empty
+        m[i] = top;
+        l[i] *= f;
+#pragma unroll
+        for (int k = 0; k < NO; ++k) {
+          o[k][i] *= f;
+          o[k][2 + i] *= f;
+        }
+      }
+    }
+    const float base0 = m[0] == -INFINITY ? 0.0f : m[0] * c, base1 = m[1] == -INFINITY ? 0.0f : m[1] * c;
+    const float p0 = ptx::ex2(fmaf(s[0], c, -base0)), p1 = ptx::ex2(fmaf(s[1], c, -base1));
+    const float p2 = ptx::ex2(fmaf(s[2], c, -base0)), p3 = ptx::ex2(fmaf(s[3], c, -base1));
+    l[0] += p0 + p2;
+    l[1] += p1 + p3;
+    const unsigned b0 = transpose8(ptx::pack16<BF16>(p0, p1)), b1 = transpose8(ptx::pack16<BF16>(p2, p3));
+#pragma unroll
+    for (int h = 0; h < VB; ++h) {
+      const unsigned* v0 = reinterpret_cast<const unsigned*>(&vx[0][h]);
+      const unsigned* v1 = reinterpret_cast<const unsigned*>(&vx[1][h]);
+      const unsigned* v2 = reinterpret_cast<const unsigned*>(&vx[2][h]);
+      const unsigned* v3 = reinterpret_cast<const unsigned*>(&vx[3][h]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        mma16816<BF16>(o[4 * h + r], __byte_perm(v0[r], v1[r], 0x5410), __byte_perm(v0[r], v1[r], 0x7632),
+                       __byte_perm(v2[r], v3[r], 0x5410), __byte_perm(v2[r], v3[r], 0x7632), b0, b1);
+    }
+  }
+
+  // ---- join the warps ----
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
+    if (g == 0) {
+      sm_m[warp][2 * t + i] = m[i];
+      sm_l[warp][2 * t + i] = l[i];
+    }
+#pragma unroll
+    for (int h = 0; h < VB; ++h)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *reinterpret_cast<float2*>(&sm_o[warp][2 * t + i][64 * h + 8 * g + 2 * r]) =
+            make_float2(o[4 * h + r][i], o[4 * h + r][2 + i]);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < n_heads * (D / 4); e += 32 * kRowWarps) {
+    const int h = e / (D / 4), ch0 = (e % (D / 4)) * 4;
+    float top = -INFINITY, sum = 0.0f, v[4] = {};
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, sm_m[w][h]);
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) {
+      const float f = ptx::ex2((sm_m[w][h] - base) * c);
+      sum = fmaf(f, sm_l[w][h], sum);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = fmaf(f, sm_o[w][h][ch0 + i], v[i]);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = sum == 0.0f ? 0.0f : v[i] * inv;
+    const long long row = ((long long)split * a.sequences + seq) * a.heads + head0 + h;
+    if (ch0 < a.head_size) {
+      if (a.part_o)
+        *reinterpret_cast<float4*>(a.part_o + row * a.head_size + ch0) = make_float4(v[0], v[1], v[2], v[3]);
+      else
+        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + seq * a.out_seq + (head0 + h) * a.out_head + ch0) =
+            make_uint2(ptx::pack16<BF16>(v[0], v[1]), ptx::pack16<BF16>(v[2], v[3]));
+    }
+    if (ch0 == 0) {
+      const float lse = base * a.scale + logf(sum);
+      if (a.part_lse) a.part_lse[row] = lse;
+      else if (a.lse) a.lse[row] = lse;
+    }
+  }
+  if (a.wait && blockIdx.x == gridDim.x - 1) ptx::griddep_wait();
+}
+
 // Joins the parts of a row: lse = log sum_s e^lse_s, out = sum_s e^(lse_s - lse) o_s,
-// in the order of the splits.  One warp per row.
+// in the order of the parts.  One warp per row.
+struct JoinArgs {
+  const int* q_off = nullptr;  // rows of [q_off[0], q_off[sequences]) only (null: all)
+  int sequences = 0;
+  long long tokens = 0;
+  int heads = 0, head_size = 0, parts = 0;
+  const float* part_o = nullptr;
+  const float* part_lse = nullptr;
+  void* out = nullptr;
+  long long out_token = 0, out_head = 0;
+  float* lse = nullptr;
+};
+
 template <typename T>
-__global__ void __launch_bounds__(128) join_kernel(const TcArgs a) {
-  const long long rows = a.total_q * a.heads, row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+__global__ void __launch_bounds__(128) join_kernel(const JoinArgs a) {
+  const long long rows = a.tokens * a.heads, row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   ptx::griddep_wait();
   if (row >= rows) return;
@@ -505,11 +705,14 @@ __global__ void __launch_bounds__(128) join_kernel(const TcArgs a) {
   const int h = (int)(row - t * a.heads);
   if (a.q_off && (t < a.q_off[0] || t >= a.q_off[a.sequences])) return;
   float top = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_lse[s * rows + row]);
+  for (int s = lane; s < a.parts; s += 32) top = fmaxf(top, a.part_lse[s * rows + row]);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
   const float base = top == -INFINITY ? 0.0f : top;
   float sum = 0.0f, o[4] = {};
   const int c = lane * 4;
-  for (int s = 0; s < a.splits; ++s) {
+#pragma unroll 4
+  for (int s = 0; s < a.parts; ++s) {
     const float f = expf(a.part_lse[s * rows + row] - base);
     sum += f;
     if (c < a.head_size) {
@@ -547,13 +750,40 @@ void encode_kv(CUtensorMap* m, int dtype, const void* base, int head_size, int k
   encode_tensor_map(m, map_type(dtype), 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// Launches behind a kernel of this file that signals its dependents early.
+template <typename... P, typename... A>
+void launch_after(void (*kernel)(P...), unsigned grid, unsigned block, cudaStream_t stream, A&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  FA_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...));
+}
+
 template <int D, bool BF16>
-void launch_tc(const TcArgs& t, const TcMaps& maps, cudaStream_t stream) {
+void launch_tc_as(const TcArgs& t, const TcMaps& maps, cudaStream_t stream) {
   FA_CUDA(cudaFuncSetAttribute(attention_tc_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                TcLayout<D>::kTotal));
   const unsigned grid = (unsigned)t.tiles * t.kv_heads * t.splits;
   attention_tc_kernel<D, BF16><<<grid, 320, TcLayout<D>::kTotal, stream>>>(t, maps);
   FA_CUDA(cudaGetLastError());
+}
+void launch_tc(const TcArgs& t, const TcMaps& maps, int dtype, cudaStream_t stream) {
+  const bool bf16 = dtype == FA_DTYPE_BF16;
+  if (t.head_size <= 64)
+    bf16 ? launch_tc_as<64, true>(t, maps, stream) : launch_tc_as<64, false>(t, maps, stream);
+  else
+    bf16 ? launch_tc_as<128, true>(t, maps, stream) : launch_tc_as<128, false>(t, maps, stream);
+}
+
+void launch_join(const JoinArgs& j, int dtype, cudaStream_t stream) {
+  const unsigned grid = (unsigned)((j.tokens * j.heads + 3) / 4);
+  launch_after(dtype == FA_DTYPE_BF16 ? join_kernel<__nv_bfloat16> : join_kernel<__half>, grid, 128, stream, j);
 }
 
 int* error_word() {
@@ -562,30 +792,23 @@ int* error_word() {
   return static_cast<int*>(p);
 }
 
+// Query rows as (channel, head of the group, KV head, token).
+void encode_q(CUtensorMap* m, int dtype, const void* base, int head_size, int group, int kv_heads, int64_t tokens,
+              const int64_t* stride, int tile_tokens) {
+  const cuuint64_t dims[4] = {(cuuint64_t)head_size, (cuuint64_t)group, (cuuint64_t)kv_heads, (cuuint64_t)tokens};
+  const cuuint64_t strides[3] = {map_stride(group, stride[1]), map_stride(kv_heads, stride[1] * group),
+                                 map_stride(tokens, stride[0])};
+  const cuuint32_t box[4] = {64, (cuuint32_t)group, 1, (cuuint32_t)tile_tokens};
+  encode_tensor_map(m, map_type(dtype), 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+constexpr int kSms = 148;
+
+// Bytes of `parts` partial results of `rows` rows.
+int64_t part_bytes(int64_t parts, int64_t rows, int head_size) { return parts * rows * (head_size + 4) * 4; }
+
 // Tile pairs of a packed call, an upper bound (tile_sequence).
 int64_t tile_pairs(int64_t total_q, int sequences, int group) { return total_q / (2 * (kRows / group)) + sequences; }
-
-template <typename T>
-__global__ void __launch_bounds__(128) shared_rows_kernel(const fa_attention_shared_args a) {
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const long long b = row / a.heads;
-  const int h = (int)(row - b * a.heads);
-  if (b >= a.sequences) return;
-  const int kh = h / (a.heads / a.kv_heads);
-  KvRun run[2];
-  run[0].k = static_cast<const T*>(a.prefix_k) + kh * a.prefix_k_stride[1];
-  run[0].v = static_cast<const T*>(a.prefix_v) + kh * a.prefix_v_stride[1];
-  run[0].k_row = a.prefix_k_stride[0];
-  run[0].v_row = a.prefix_v_stride[0];
-  run[0].n = (int)a.prefix_len;
-  run[1].k = static_cast<const T*>(a.suffix_k) + b * a.suffix_k_stride[0] + kh * a.suffix_k_stride[2];
-  run[1].v = static_cast<const T*>(a.suffix_v) + b * a.suffix_v_stride[0] + kh * a.suffix_v_stride[2];
-  run[1].k_row = a.suffix_k_stride[1];
-  run[1].v_row = a.suffix_v_stride[1];
-  run[1].n = a.suffix_lens ? clamp_to(a.suffix_lens[b], a.suffix_capacity) : 0;
-  attend_row<T>(static_cast<const T*>(a.q) + b * a.q_stride[0] + h * a.q_stride[1], run, 2, a.head_size, a.scale,
-                static_cast<T*>(a.out) + b * a.out_stride[0] + h * a.out_stride[1], a.lse ? a.lse + row : nullptr);
-}
 
 }  // namespace
 
@@ -644,8 +867,51 @@ int check_attention_shared(const fa_attention_shared_args* a) {
   return kHandled;
 }
 
-int64_t attention_packed_workspace(int64_t, int64_t, int, int, int, int) { return 0; }
-int64_t attention_shared_workspace(int64_t, int64_t, int, int, int, int) { return 0; }
+namespace {
+
+// Key ranges that a packed call is cut into: when its tiles leave SMs idle and
+// the sequences are long enough on average that a part has at least 4 steps.
+int packed_splits(int64_t total_q, int64_t total_k, int sequences, int heads, int kv_heads) {
+  const int64_t ctas = std::max<int64_t>(1, tile_pairs(total_q, sequences, heads / kv_heads) * kv_heads);
+  const int64_t steps = sequences > 0 ? total_k / sequences / kKeys : 0;
+  return (int)std::max<int64_t>(1, std::min({kSms / ctas, steps / 4, (int64_t)64}));
+}
+
+// How a shared-prefix call is cut.
+struct SharedPlan {
+  bool tc = false;      // the prefix on the tensor cores, for all sequences at once
+  int tc_splits = 0;    // its key ranges
+  int row_splits = 1;   // key ranges of attention_rows_kernel
+  int parts() const { return tc || row_splits > 1 ? tc_splits + row_splits : 0; }
+};
+SharedPlan shared_plan(int64_t prefix_len, int64_t capacity, int sequences, int heads, int kv_heads) {
+  SharedPlan p;
+  const int group = heads / kv_heads;
+  p.tc = sequences >= 4 && prefix_len >= 256;
+  if (p.tc) {
+    const int64_t ctas = ((int64_t)sequences * group + 2 * kRows - 1) / (2 * kRows) * kv_heads;
+    p.tc_splits = (int)std::max<int64_t>(1, std::min<int64_t>(kSms / ctas, (prefix_len + kKeys - 1) / kKeys));
+  }
+  const int64_t ctas = (int64_t)sequences * kv_heads * ((group + kRowHeads - 1) / kRowHeads);
+  const int64_t chunks = ((p.tc ? 0 : prefix_len) + capacity) / kChunk;
+  p.row_splits = (int)std::max<int64_t>(1, std::min<int64_t>(4 * kSms / ctas, chunks / (4 * kRowWarps)));
+  return p;
+}
+
+}  // namespace
+
+int64_t attention_packed_workspace(int64_t total_q, int64_t total_k, int sequences, int heads, int kv_heads,
+                                   int head_size) {
+  if (total_q <= 0 || sequences <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > 64) return 0;
+  const int splits = packed_splits(total_q, total_k, sequences, heads, kv_heads);
+  return splits > 1 ? part_bytes(splits, total_q * heads, head_size) : 0;
+}
+int64_t attention_shared_workspace(int64_t prefix_len, int64_t suffix_capacity, int sequences, int heads, int kv_heads,
+                                   int head_size) {
+  if (sequences <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > 64) return 0;
+  const SharedPlan p = shared_plan(prefix_len, suffix_capacity, sequences, heads, kv_heads);
+  return part_bytes(p.parts(), (int64_t)sequences * heads, head_size);
+}
 
 void launch_attention_packed(const fa_attention_packed_args& a, cudaStream_t stream) {
   if (a.total_q == 0 || a.sequences == 0) return;
@@ -661,6 +927,7 @@ void launch_attention_packed(const fa_attention_packed_args& a, cudaStream_t str
   t.head_size = a.head_size;
   t.tokens = kRows / t.group;
   t.tiles = (int)tile_pairs(a.total_q, a.sequences, t.group);
+  t.splits = packed_splits(a.total_q, a.total_k, a.sequences, a.heads, a.kv_heads);
   t.causal = a.causal;
   t.scale = a.scale;
   t.scale_log2 = (float)(a.scale * 1.4426950408889634);
@@ -669,38 +936,130 @@ void launch_attention_packed(const fa_attention_packed_args& a, cudaStream_t str
   t.out_head = a.out_stride[1];
   t.lse = a.lse;
   t.err = error_word();
-  TcMaps maps;
-  {
-    const cuuint64_t dims[4] = {(cuuint64_t)a.head_size, (cuuint64_t)t.group, (cuuint64_t)a.kv_heads,
-                                (cuuint64_t)a.total_q};
-    const cuuint64_t strides[3] = {map_stride(t.group, a.q_stride[1]),
-                                   map_stride(a.kv_heads, a.q_stride[1] * t.group), map_stride(a.total_q, a.q_stride[0])};
-    const cuuint32_t box[4] = {64, (cuuint32_t)t.group, 1, (cuuint32_t)t.tokens};
-    encode_tensor_map(&maps.q, map_type(a.dtype), 4, a.q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (t.splits > 1) {
+    t.part_o = static_cast<float*>(a.workspace);
+    t.part_lse = t.part_o + t.splits * a.total_q * a.heads * a.head_size;
   }
+  TcMaps maps;
+  encode_q(&maps.q, a.dtype, a.q, a.head_size, t.group, a.kv_heads, a.total_q, a.q_stride, t.tokens);
   if (a.total_k > 0) {
     encode_kv(&maps.k, a.dtype, a.k, a.head_size, a.kv_heads, a.total_k, a.k_stride);
     encode_kv(&maps.v, a.dtype, a.v, a.head_size, a.kv_heads, a.total_k, a.v_stride);
   } else {
     maps.k = maps.v = maps.q;  // never used: no sequence has a key
   }
-  const bool bf16 = a.dtype == FA_DTYPE_BF16;
-  if (a.head_size <= 64)
-    bf16 ? launch_tc<64, true>(t, maps, stream) : launch_tc<64, false>(t, maps, stream);
-  else
-    bf16 ? launch_tc<128, true>(t, maps, stream) : launch_tc<128, false>(t, maps, stream);
+  launch_tc(t, maps, a.dtype, stream);
+  if (t.splits > 1) {
+    JoinArgs j;
+    j.q_off = a.q_offsets;
+    j.sequences = a.sequences;
+    j.tokens = a.total_q;
+    j.heads = a.heads;
+    j.head_size = a.head_size;
+    j.parts = t.splits;
+    j.part_o = t.part_o;
+    j.part_lse = t.part_lse;
+    j.out = a.out;
+    j.out_token = a.out_stride[0];
+    j.out_head = a.out_stride[1];
+    j.lse = a.lse;
+    launch_join(j, a.dtype, stream);
+  }
 }
 
 void launch_attention_shared(const fa_attention_shared_args& a, cudaStream_t stream) {
   if (a.sequences == 0) return;
-  const unsigned grid = (unsigned)(((int64_t)a.sequences * a.heads + 3) / 4);
-  fa_attention_shared_args s = a;
-  if (a.suffix_capacity == 0) s.suffix_lens = nullptr;
-  if (a.dtype == FA_DTYPE_F16)
-    shared_rows_kernel<__half><<<grid, 128, 0, stream>>>(s);
-  else
-    shared_rows_kernel<__nv_bfloat16><<<grid, 128, 0, stream>>>(s);
-  FA_CUDA(cudaGetLastError());
+  const SharedPlan plan = shared_plan(a.prefix_len, a.suffix_capacity, a.sequences, a.heads, a.kv_heads);
+  const int64_t rows = (int64_t)a.sequences * a.heads;
+  const int group = a.heads / a.kv_heads, parts = plan.parts();
+  float* part_o = parts ? static_cast<float*>(a.workspace) : nullptr;
+  float* part_lse = parts ? part_o + parts * rows * a.head_size : nullptr;
+  const float scale_log2 = (float)(a.scale * 1.4426950408889634);
+  if (plan.tc) {
+    TcArgs t;
+    t.total_q = a.sequences;
+    t.total_k = a.prefix_len;
+    t.heads = a.heads;
+    t.kv_heads = a.kv_heads;
+    t.group = group;
+    t.head_size = a.head_size;
+    t.tokens = kRows / group;
+    t.tiles = (a.sequences + 2 * t.tokens - 1) / (2 * t.tokens);
+    t.splits = plan.tc_splits;
+    t.scale = a.scale;
+    t.scale_log2 = scale_log2;
+    t.part_o = part_o;
+    t.part_lse = part_lse;
+    t.err = error_word();
+    TcMaps maps;
+    encode_q(&maps.q, a.dtype, a.q, a.head_size, group, a.kv_heads, a.sequences, a.q_stride, t.tokens);
+    encode_kv(&maps.k, a.dtype, a.prefix_k, a.head_size, a.kv_heads, a.prefix_len, a.prefix_k_stride);
+    encode_kv(&maps.v, a.dtype, a.prefix_v, a.head_size, a.kv_heads, a.prefix_len, a.prefix_v_stride);
+    launch_tc(t, maps, a.dtype, stream);
+  }
+  RowsArgs r;
+  r.q = a.q;
+  r.q_seq = a.q_stride[0];
+  r.q_head = a.q_stride[1];
+  r.prefix.k = a.prefix_k;
+  r.prefix.v = a.prefix_v;
+  r.prefix.k_row = a.prefix_k_stride[0];
+  r.prefix.v_row = a.prefix_v_stride[0];
+  r.prefix.k_head = a.prefix_k_stride[1];
+  r.prefix.v_head = a.prefix_v_stride[1];
+  r.suffix.k = a.suffix_k;
+  r.suffix.v = a.suffix_v;
+  r.suffix.k_seq = a.suffix_k_stride[0];
+  r.suffix.v_seq = a.suffix_v_stride[0];
+  r.suffix.k_row = a.suffix_k_stride[1];
+  r.suffix.v_row = a.suffix_v_stride[1];
+  r.suffix.k_head = a.suffix_k_stride[2];
+  r.suffix.v_head = a.suffix_v_stride[2];
+  r.prefix_len = plan.tc ? 0 : (int)a.prefix_len;
+  r.suffix_lens = a.suffix_capacity > 0 ? a.suffix_lens : nullptr;
+  r.capacity = (int)a.suffix_capacity;
+  r.sequences = a.sequences;
+  r.heads = a.heads;
+  r.kv_heads = a.kv_heads;
+  r.group = group;
+  r.head_size = a.head_size;
+  r.blocks = (group + kRowHeads - 1) / kRowHeads;
+  r.splits = plan.row_splits;
+  r.scale = a.scale;
+  r.scale_log2 = scale_log2;
+  r.out = a.out;
+  r.out_seq = a.out_stride[0];
+  r.out_head = a.out_stride[1];
+  r.lse = a.lse;
+  r.wait = plan.tc;
+  if (parts) {
+    r.part_o = part_o + plan.tc_splits * rows * a.head_size;
+    r.part_lse = part_lse + plan.tc_splits * rows;
+  }
+  const unsigned grid = (unsigned)((int64_t)a.sequences * a.kv_heads * r.blocks * r.splits);
+  const bool bf16 = a.dtype == FA_DTYPE_BF16;
+  auto kernel = a.head_size <= 64 ? (bf16 ? attention_rows_kernel<64, true> : attention_rows_kernel<64, false>)
+                                  : (bf16 ? attention_rows_kernel<128, true> : attention_rows_kernel<128, false>);
+  if (plan.tc) {
+    launch_after(kernel, grid, 32 * kRowWarps, stream, r);
+  } else {
+    kernel<<<grid, 32 * kRowWarps, 0, stream>>>(r);
+    FA_CUDA(cudaGetLastError());
+  }
+  if (parts) {
+    JoinArgs j;
+    j.tokens = a.sequences;
+    j.heads = a.heads;
+    j.head_size = a.head_size;
+    j.parts = parts;
+    j.part_o = part_o;
+    j.part_lse = part_lse;
+    j.out = a.out;
+    j.out_token = a.out_stride[0];
+    j.out_head = a.out_stride[1];
+    j.lse = a.lse;
+    launch_join(j, a.dtype, stream);
+  }
 }
 
 int take_device_error() {
