@@ -254,12 +254,12 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
     auto ring = [&](int n) { return sbase + L::kKv + (n % L::kStages) * L::kTile; };
     auto ring_wait = [&](int n) { wait(&kv_full[n % L::kStages], (n / L::kStages) & 1, kAttnWaitLoad); };
     auto scores = [&](int w, int i) {  // S_w = Q_w K_i^T
-      if (lane == 0) {
-        const unsigned q = sbase + w * L::kTile, k = ring(2 * i);
-        for (int s = 0; s < k_s; ++s) {
-          const unsigned off = (s >> 2) * L::kHalf + (s & 3) * 32;
-          ptx::tc_mma_ss(tmem + w * kKeys, ptx::smem_desc_128b(q + off, 16, 1024), ptx::smem_desc_128b(k + off, 16, 1024),
-                         id_s, s > 0);
+      const uint64_t q = ptx::smem_desc_128b(sbase + w * L::kTile, 16, 1024), k = ptx::smem_desc_128b(ring(2 * i), 16, 1024);
+      if (ptx::elect()) {
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+          const unsigned off = ((s >> 2) * L::kHalf + (s & 3) * 32) >> 4;
+          if (s < k_s) ptx::tc_mma_ss(tmem + w * kKeys, q + off, k + off, id_s, s > 0);
         }
         ptx::tc_commit(&s_full[w]);
       }
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
         wait(&q_full[w], 0, kAttnWaitLoad);
         if (ok) scores(w, 0);
       }
-    if (ok && cnt > 0 && lane == 0) ptx::tc_commit(&kv_empty[0]);
+    if (ok && cnt > 0 && ptx::elect()) ptx::tc_commit(&kv_empty[0]);
     __syncwarp();
     for (int i = 0; i < cnt && ok; ++i) {
       ring_wait(2 * i + 1);
@@ -293,30 +293,31 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
         if (i >= mine) continue;
         wait(&p_full[w], i & 1, kAttnWaitSoftmax);
         if (!ok) break;
-        if (lane == 0) {
-          const unsigned v = ring(2 * i + 1);
-          const int steps = (min(end[w] - (ja + i) * kKeys, kKeys) + 15) / 16;
-          for (int s = 0; s < steps; ++s)
-            ptx::tc_mma_ts(tmem + 256 + w * D, tmem + w * kKeys + s * 8,
-                           ptx::smem_desc_128b(v + s * 2048, L::kHalf, 1024), id_o, i > 0 || s > 0);
+        const uint64_t v = ptx::smem_desc_128b(ring(2 * i + 1), L::kHalf, 1024);
+        const int steps = (min(end[w] - (ja + i) * kKeys, kKeys) + 15) / 16;
+        if (ptx::elect()) {
+#pragma unroll
+          for (int s = 0; s < kKeys / 16; ++s)
+            if (s < steps)
+              ptx::tc_mma_ts(tmem + 256 + w * D, tmem + w * kKeys + s * 8, v + (s * 2048 >> 4), id_o, i > 0 || s > 0);
         }
         __syncwarp();
         if (i + 1 < mine) {
           if (!have_k) ring_wait(2 * i + 2);
           have_k = true;
           if (ok) scores(w, i + 1);
-        } else if (lane == 0) {
+        } else if (ptx::elect()) {
           ptx::tc_commit(&o_full[w]);
         }
         __syncwarp();
       }
-      if (ok && lane == 0) {
+      if (ok && ptx::elect()) {
         ptx::tc_commit(&kv_empty[(2 * i + 1) % L::kStages]);
         if (i + 1 < cnt) ptx::tc_commit(&kv_empty[(2 * i + 2) % L::kStages]);
       }
       __syncwarp();
     }
-    if (lane == 0 && !ok) {  // MMAs in flight finish before their memory is freed
+    if (!ok && ptx::elect()) {  // MMAs in flight finish before their memory is freed
       ptx::tc_commit(drained);
       ptx::wait_phase(drained, 0, abort_flag, a.err, kAttnWaitMma, false);
     }
@@ -339,56 +340,93 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
       ok = __all_sync(0xffffffffu, ptx::wait_phase(&s_full[w], i & 1, abort_flag, a.err, kAttnWaitMma));
       if (!ok) break;
       ptx::tc_fence_after();
-      unsigned u[128];
-      float* s = reinterpret_cast<float*>(u);
+      const int lim = sees - (ja + i) * kKeys;  // keys of this step that the row sees
+      bool done = false;
+      if (i > 0 && __all_sync(0xffffffffu, lim >= kKeys)) {
+        // Every key is seen, and the maximum so far most likely serves: the
+        // exponentials start with the first scores instead of after the last,
+        // and count only if no score is too far above the maximum.
+        const uint64_t c2 = ptx::pair(c, c);
+        const float nb = m == -INFINITY ? 0.0f : -m * c;
+        const uint64_t nb2 = ptx::pair(nb, nb);
+        unsigned p[64], u[2][32];
+        uint64_t sum[2] = {0, 0};
+        float top[2] = {-INFINITY, -INFINITY};
+        ptx::tmem_ld32(s_addr, u[0]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) ptx::tmem_ld32(s_addr + 32 * k, u + 32 * k);
-      ptx::tc_wait_ld();
-      const int lim = sees - (ja + i) * kKeys;
-      if (__any_sync(0xffffffffu, lim < kKeys)) {
+        for (int k = 0; k < 4; ++k) {
+          ptx::tc_wait_ld();
+          if (k < 3) ptx::tmem_ld32(s_addr + 32 * (k + 1), u[(k + 1) & 1]);
 #pragma unroll
-        for (int k = 0; k < kKeys; ++k)
-          if (k >= lim) s[k] = -INFINITY;
-      }
-      float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-      for (int k = 4; k < kKeys; ++k) top[k & 3] = fmaxf(top[k & 3], s[k]);
-      const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-      if (i == 0) {
-        m = mx;
-      } else {
-        const bool rise = mx * c > m * c + kSlack;
-        if (__any_sync(0xffffffffu, rise)) {
-          const float f = rise ? ptx::ex2((m - mx) * c) : 1.0f;
-          if (rise) m = mx;
-          l *= f;
-#pragma unroll 1
-          for (int k = 0; k < D; k += 32) {
-            unsigned o[32];
-            ptx::tmem_ld32(o_addr + k, o);
-            ptx::tc_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            ptx::tmem_st32(o_addr + k, o);
+          for (int e = 0; e < 16; ++e) {
+            const float s0 = __uint_as_float(u[k & 1][2 * e]), s1 = __uint_as_float(u[k & 1][2 * e + 1]);
+            top[e & 1] = ptx::max3(top[e & 1], s0, s1);
+            float x0, x1;
+            ptx::unpair(ptx::fma2(ptx::pair(s0, s1), c2, nb2), x0, x1);
+            x0 = ptx::ex2(x0);
+            x1 = ptx::ex2(x1);
+            sum[e & 1] = ptx::add2(sum[e & 1], ptx::pair(x0, x1));
+            p[16 * k + e] = ptx::pack16<BF16>(x0, x1);
           }
         }
-      }
-      const float base = m == -INFINITY ? 0.0f : m * c;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        unsigned p[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p0 = ptx::ex2(fmaf(s[32 * k + 2 * e], c, -base));
-          const float p1 = ptx::ex2(fmaf(s[32 * k + 2 * e + 1], c, -base));
-          sum[(2 * e) & 3] += p0;
-          sum[(2 * e + 1) & 3] += p1;
-          p[e] = ptx::pack16<BF16>(p0, p1);
+        done = !__any_sync(0xffffffffu, fmaxf(top[0], top[1]) * c > m * c + kSlack);
+        if (done) {
+          ptx::tmem_st32(s_addr, p);
+          ptx::tmem_st32(s_addr + 32, p + 32);
+          float a0, a1;
+          ptx::unpair(ptx::add2(sum[0], sum[1]), a0, a1);
+          l += a0 + a1;
         }
-        ptx::tmem_st16(s_addr + 16 * k, p);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      if (!done) {
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int k = 0; k < kKeys; k += 32) {
+          unsigned u[32];
+          ptx::tmem_ld32(s_addr + k, u);
+          ptx::tc_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (k + e < lim) mx = fmaxf(mx, __uint_as_float(u[e]));
+        }
+        if (i == 0) {
+          m = mx;
+        } else {
+          const bool rise = mx * c > m * c + kSlack;
+          if (__any_sync(0xffffffffu, rise)) {
+            const float f = rise ? ptx::ex2((m - mx) * c) : 1.0f;
+            if (rise) m = mx;
+            l *= f;
+#pragma unroll 1
+            for (int k = 0; k < D; k += 32) {
+              unsigned o[32];
+              ptx::tmem_ld32(o_addr + k, o);
+              ptx::tc_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              ptx::tmem_st32(o_addr + k, o);
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.0f : m * c;
+        float sum[2] = {0.0f, 0.0f};
+#pragma unroll 1
+        for (int k = 0; k < kKeys; k += 32) {
+          unsigned u[32], p[16];
+          ptx::tmem_ld32(s_addr + k, u);
+          ptx::tc_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float p0 = k + 2 * e < lim ? ptx::ex2(fmaf(__uint_as_float(u[2 * e]), c, -base)) : 0.0f;
+            const float p1 = k + 2 * e + 1 < lim ? ptx::ex2(fmaf(__uint_as_float(u[2 * e + 1]), c, -base)) : 0.0f;
+            sum[0] += p0;
+            sum[1] += p1;
+            p[e] = ptx::pack16<BF16>(p0, p1);
+          }
+          ptx::tmem_st16(s_addr + k / 2, p);
+        }
+        l += sum[0] + sum[1];
+      }
       ptx::tc_wait_st();
       ptx::tc_fence_before();
       __syncwarp();

@@ -107,6 +107,15 @@ __device__ __forceinline__ void tc_mma_ts(unsigned d, unsigned a, uint64_t b, un
       : "memory");
 }
 
+// True in one thread of a converged warp, the same at every call.  Unlike a test
+// of the lane number it tells the compiler that one thread runs the branch, so
+// that MMA operands stay in uniform registers.
+__device__ __forceinline__ bool elect() {
+  unsigned r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
+}
+
 // Shared-memory matrix descriptor of a 128-byte-swizzled operand: `lbo` bytes
 // between 64-element blocks of the contiguous dimension (where that one is not
 // the summed one), `sbo` bytes between groups of 8 rows.
@@ -156,6 +165,30 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// Pairs of floats in one register pair: two IEEE operations per instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 // Two floats rounded to 16 bits, `lo` in the lower half.
 template <bool BF16>
