@@ -57,8 +57,13 @@ __device__ __forceinline__ int clamp_to(int x, long long hi) { return (int)min((
 // -------------------------------------------------- tensor-core attention ----
 
 constexpr int kRows = 128;     // query rows of one tile (TMEM lanes): tokens x heads of a KV head's group
-constexpr int kKeys = 128;     // keys per step
+constexpr int kKeys = 128;     // keys of a K or V tile in shared memory
+constexpr int kUnit = 64;      // keys per softmax step: half a tile
 constexpr float kSlack = 8.0f; // powers of two by which a row's maximum may rise before its sums are rescaled
+
+constexpr unsigned kTmS = 0, kTmO = 256;  // TMEM columns of S and O
+
+constexpr int kTcThreads = 352;  // 8 softmax warps, 2 that issue MMAs, 1 that copies
 
 enum AttnError : int { kAttnWaitLoad = 41, kAttnWaitMma = 42, kAttnWaitSoftmax = 43, kAttnWaitFree = 44 };
 
@@ -94,7 +99,9 @@ struct TcLayout {
   static constexpr int kStages = D == 128 ? 5 : 8;  // K and V tiles in flight
   static constexpr int kKv = 2 * kTile;
   static constexpr int kBars = kKv + kStages * kTile;
-  static constexpr int kNumBars = 2 * kStages + 2 + 2 + 2 + 2 + 1;
+  // TMEM columns (all 512 are allocated, so they start at 0): tile 0's S buffers
+  // 0 and 64, tile 1's 128 and 192, O0 256, O1 256 + D.
+  static constexpr int kNumBars = 2 * kStages + 2 + 4 + 4 + 4 + 2;
   static constexpr int kMisc = kBars + 8 * kNumBars;
   static constexpr int kTotal = kMisc + 16 + 1024;  // 1024: the tiles start on a swizzle atom
   static_assert(kTotal <= 227 * 1024, "shared memory");
@@ -119,18 +126,21 @@ __device__ __forceinline__ int tile_sequence(const TcArgs& a, int tile, int span
 }
 
 // One CTA: two tiles of 128 query rows (tokens x the heads that share a KV
-// head) against the keys of their sequence, 128 keys a step:
-//   warp 9   copies Q, then K and V tiles through a ring (TMA);
-//   warp 8   issues S = Q K^T into TMEM and O += P V with P from TMEM
-//            (tcgen05.mma; tile 0's and tile 1's in turn, so that the tensor
-//            core works on one tile while the other's softmax runs);
+// head) against the keys of their sequence, 64 keys a step:
+//   warp 10  copies Q, then K and V tiles through a ring (TMA);
+//   warps 8 and 9, one per tile: issue S = Q K^T into TMEM and O += P V with P
+//            from TMEM (tcgen05.mma; one thread issues an MMA per ~62 cycles, an
+//            MMA of 64 keys lasts 32 to 48: one issuer for both tiles was the bound);
 //   warps 0-3 and 4-7, one thread per row: running maximum, p = 2^(s - m),
 //            P in 16 bits over S's columns, row sums in 32 bits.
-// The row maximum that the exponents subtract only moves when it rises by more
-// than 2^kSlack, so O (in TMEM) is rescaled rarely; S of step i + 1 is issued
-// after P V of step i, so a completed S also says that O is at rest.
+// TMEM holds two S buffers of 64 keys per tile next to the two O: while a tile's
+// softmax works on one buffer, the tensor core turns the other's P into O and
+// refills it, so neither waits for the other's whole step.  (With one buffer of
+// 128 keys a step was the sum softmax + P V + Q K^T + the hand-offs: 3490 cycles
+// against 2048 of MMA.)  The row maximum that the exponents subtract only moves
+// when it rises by more than 2^kSlack, so O (in TMEM) is rescaled rarely.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, const __grid_constant__ TcMaps maps) {
+__global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const TcArgs a, const __grid_constant__ TcMaps maps) {
   using L = TcLayout<D>;
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   extern __shared__ uint8_t sm_raw[];
@@ -139,10 +149,10 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
   uint64_t* kv_full = reinterpret_cast<uint64_t*>(sm + L::kBars);
   uint64_t* kv_empty = kv_full + L::kStages;
   uint64_t* q_full = kv_empty + L::kStages;  // [2] per tile
-  uint64_t* s_full = q_full + 2;             // [2] scores complete (and the O before them)
-  uint64_t* p_full = s_full + 2;             // [2] probabilities stored
-  uint64_t* o_full = p_full + 2;             // [2] output complete
-  uint64_t* drained = o_full + 2;
+  uint64_t* s_full = q_full + 2;             // [2 tiles x 2 buffers] scores complete
+  uint64_t* p_full = s_full + 4;             // [2 x 2] probabilities stored
+  uint64_t* pv_done = p_full + 4;            // [2 x 2] their product with V added to O
+  uint64_t* drained = pv_done + 4;           // [2]
   unsigned* tmem_slot = reinterpret_cast<unsigned*>(sm + L::kMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::kMisc + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -174,22 +184,25 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
   }
   const int steps_all = (max(end[0], end[1]) + kKeys - 1) / kKeys;
   const int ja = (int)((long long)steps_all * split / a.splits), jb = (int)((long long)steps_all * (split + 1) / a.splits);
-  const int cnt0 = max(0, min(jb, (end[0] + kKeys - 1) / kKeys) - ja);
-  const int cnt1 = max(0, min(jb, (end[1] + kKeys - 1) / kKeys) - ja);
-  const int cnt = max(cnt0, cnt1);
+  const int key0 = ja * kKeys;  // this split's first key
+  const int cnt0 = max(0, (min(jb * kKeys, end[0]) - key0 + kUnit - 1) / kUnit);  // steps of the tiles
+  const int cnt1 = max(0, (min(jb * kKeys, end[1]) - key0 + kUnit - 1) / kUnit);
+  const int cnt = max(cnt0, cnt1), kv_tiles = (cnt + 1) / 2;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::kStages; ++s) {
       ptx::mbar_init(&kv_full[s], 1);
-      ptx::mbar_init(&kv_empty[s], 1);
+      ptx::mbar_init(&kv_empty[s], 2);  // both issuers
     }
     for (int w = 0; w < 2; ++w) {
       ptx::mbar_init(&q_full[w], 1);
-      ptx::mbar_init(&s_full[w], 1);
-      ptx::mbar_init(&p_full[w], 4);
-      ptx::mbar_init(&o_full[w], 1);
+      ptx::mbar_init(&drained[w], 1);
     }
-    ptx::mbar_init(drained, 1);
+    for (int b = 0; b < 4; ++b) {
+      ptx::mbar_init(&s_full[b], 1);
+      ptx::mbar_init(&p_full[b], 4);
+      ptx::mbar_init(&pv_done[b], 1);
+    }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -201,10 +214,9 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  const unsigned tmem = *tmem_slot;  // columns: S0 0, S1 128, O0 256, O1 256 + D
 
-  if (warp == 9) {
-    // ---- copies: ring slot of K step i: 2i, of V step i: 2i + 1 ----
+  if (warp == 10) {
+    // ---- copies: ring number of K tile i: 2i, of V tile i: 2i + 1 ----
     if (lane == 0) {
       int n = 0;  // ring tiles issued
       bool ok = true;
@@ -215,7 +227,7 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
         if (!ok) return;
         ptx::mbar_expect_tx(&kv_full[st], L::kTile);
         for (int h = 0; h < L::kHalves; ++h)
-          ptx::tma_load_3d(sbase + L::kKv + st * L::kTile + h * L::kHalf, map, h * 64, kvh, k0 + (ja + i) * kKeys,
+          ptx::tma_load_3d(sbase + L::kKv + st * L::kTile + h * L::kHalf, map, h * 64, kvh, k0 + key0 + i * kKeys,
                            &kv_full[st]);
         ++n;
       };
@@ -229,9 +241,9 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
       load_q(0);
       if (cnt > 0) load_kv(&maps.k, 0);
       load_q(1);
-      for (int i = 0; i < cnt && ok; ++i) {
+      for (int i = 0; i < kv_tiles && ok; ++i) {
         load_kv(&maps.v, i);
-        if (i + 1 < cnt && ok) load_kv(&maps.k, i + 1);
+        if (i + 1 < kv_tiles && ok) load_kv(&maps.k, i + 1);
       }
       // Copies in flight land before the CTA exits.
       for (int s = max(0, n - L::kStages); s < n; ++s)
@@ -240,9 +252,11 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
       if (cnt1 > 0) ptx::wait_phase(&q_full[1], 0, abort_flag, a.err, kAttnWaitLoad, false);
     }
     __syncwarp();
-  } else if (warp == 8) {
-    // ---- MMAs ----
-    const unsigned id_s = ptx::idesc_f16(BF16, false, kRows, kKeys);
+  } else if (warp >= 8) {
+    // ---- MMAs of one tile: uniform values, constant offsets and no arithmetic
+    // between the MMAs of a step ----
+    const int w = warp - 8, mine = w ? cnt1 : cnt0;
+    const unsigned id_s = ptx::idesc_f16(BF16, false, kRows, kUnit);
     const int n_o = (a.head_size + 15) / 16 * 16;  // channels past head_size are zeros (TMA fill)
     const unsigned id_o = ptx::idesc_f16(BF16, true, kRows, n_o);
     const int k_s = n_o / 16;
@@ -251,75 +265,101 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
       ok = ok && __all_sync(0xffffffffu, ptx::wait_phase(bar, parity, abort_flag, a.err, code));
       ptx::tc_fence_after();
     };
-    auto ring = [&](int n) { return sbase + L::kKv + (n % L::kStages) * L::kTile; };
-    auto ring_wait = [&](int n) { wait(&kv_full[n % L::kStages], (n / L::kStages) & 1, kAttnWaitLoad); };
-    auto scores = [&](int w, int i) {  // S_w = Q_w K_i^T
-      const uint64_t q = ptx::smem_desc_128b(sbase + w * L::kTile, 16, 1024), k = ptx::smem_desc_128b(ring(2 * i), 16, 1024);
-      if (ptx::elect()) {
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-          const unsigned off = ((s >> 2) * L::kHalf + (s & 3) * 32) >> 4;
-          if (s < k_s) ptx::tc_mma_ss(tmem + w * kKeys, q + off, k + off, id_s, s > 0);
+    const unsigned q_low = ptx::smem_desc_low(sbase, 16), k_low = ptx::smem_desc_low(sbase + L::kKv, 16),
+                   v_low = ptx::smem_desc_low(sbase + L::kKv, L::kHalf);
+    struct Slot {  // a tile's place in the ring; K tiles have even numbers, V tiles odd ones
+      int st;
+      unsigned ph;
+      __device__ __forceinline__ void next() {
+        st += 2;
+        if (st >= L::kStages) {
+          st -= L::kStages;
+          ph ^= 1;
         }
-        ptx::tc_commit(&s_full[w]);
+      }
+    };
+    Slot ks{0, 0}, vs{1, 0};
+    auto scores = [&](int b) {  // S_w of the K tile's half b into buffer b
+      const unsigned q = q_low + w * (L::kTile >> 4);
+      const unsigned k = k_low + ks.st * (L::kTile >> 4) + b * (kUnit * 128 >> 4);
+      if (ptx::elect()) {
+        if (k_s == D / 16) {
+#pragma unroll
+          for (int s = 0; s < D / 16; ++s) {
+            const unsigned off = ((s >> 2) * L::kHalf + (s & 3) * 32) >> 4;
+            ptx::tc_mma_ss(kTmS + w * 128 + b * kUnit, q + off, k + off, id_s, s > 0);
+          }
+        } else {
+          for (int s = 0; s < k_s; ++s) {
+            const unsigned off = ((s >> 2) * L::kHalf + (s & 3) * 32) >> 4;
+            ptx::tc_mma_ss(kTmS + w * 128 + b * kUnit, q + off, k + off, id_s, s > 0);
+          }
+        }
+        ptx::tc_commit(&s_full[2 * w + b]);
       }
       __syncwarp();
     };
-    if (cnt > 0) ring_wait(0);
-    for (int w = 0; w < 2 && ok; ++w)
-      if ((w ? cnt1 : cnt0) > 0) {
-        wait(&q_full[w], 0, kAttnWaitLoad);
-        if (ok) scores(w, 0);
+    auto values = [&](int b, int steps, bool acc) {  // O_w += P_w (buffer b) x the V tile's half b
+      const unsigned v = v_low + vs.st * (L::kTile >> 4) + b * (kUnit * 128 >> 4);
+      if (ptx::elect()) {
+        if (steps == kUnit / 16) {
+#pragma unroll
+          for (int s = 0; s < kUnit / 16; ++s)
+            ptx::tc_mma_ts(kTmO + w * D, kTmS + w * 128 + b * kUnit + s * 8, v + (s * 2048 >> 4), id_o, acc || s > 0);
+        } else {
+          for (int s = 0; s < steps; ++s)
+            ptx::tc_mma_ts(kTmO + w * D, kTmS + w * 128 + b * kUnit + s * 8, v + (s * 2048 >> 4), id_o, acc || s > 0);
+        }
+        ptx::tc_commit(&pv_done[2 * w + b]);
       }
+      __syncwarp();
+    };
+    if (cnt > 0) wait(&kv_full[0], 0, kAttnWaitLoad);
+    if (mine > 0) {
+      wait(&q_full[w], 0, kAttnWaitLoad);
+      if (ok) scores(0);
+      if (ok && mine > 1) scores(1);
+    }
     if (ok && cnt > 0 && ptx::elect()) ptx::tc_commit(&kv_empty[0]);
     __syncwarp();
-    for (int i = 0; i < cnt && ok; ++i) {
-      ring_wait(2 * i + 1);
+    ks.next();
+    for (int n0 = 0; n0 < cnt && ok; n0 += 2) {  // one V tile, and the K tile after its own
+      // Waits, and releases below, also for tiles that only the other issuer uses:
+      // one that ran ahead would release a slot's next use.
+      wait(&kv_full[vs.st], vs.ph, kAttnWaitLoad);
+      if (n0 + 2 < cnt) wait(&kv_full[ks.st], ks.ph, kAttnWaitLoad);
       if (!ok) break;
       // Value rows behind the last key that a row sees are not the sequence's
       // own, or masked for every row here: 0 x what they hold must stay 0.
-      const int most = min(max(end[0], end[1]) - (ja + i) * kKeys, kKeys), padded = (most + 15) / 16 * 16;
-      if (most < padded) {
-        uint8_t* v = sm + L::kKv + ((2 * i + 1) % L::kStages) * L::kTile;
+      const int most = min(max(end[0], end[1]) - key0 - n0 * kUnit, kKeys), padded = (most + 15) / 16 * 16;
+      if (n0 < mine && most < padded) {
+        uint8_t* v = sm + L::kKv + vs.st * L::kTile;
         for (int c = lane; c < (padded - most) * 8; c += 32)
           for (int h = 0; h < L::kHalves; ++h)
             *reinterpret_cast<uint4*>(v + h * L::kHalf + (most + c / 8) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
-      bool have_k = false;
-      for (int w = 0; w < 2 && ok; ++w) {
-        const int mine = w ? cnt1 : cnt0;
-        if (i >= mine) continue;
-        wait(&p_full[w], i & 1, kAttnWaitSoftmax);
-        if (!ok) break;
-        const uint64_t v = ptx::smem_desc_128b(ring(2 * i + 1), L::kHalf, 1024);
-        const int steps = (min(end[w] - (ja + i) * kKeys, kKeys) + 15) / 16;
-        if (ptx::elect()) {
 #pragma unroll
-          for (int s = 0; s < kKeys / 16; ++s)
-            if (s < steps)
-              ptx::tc_mma_ts(tmem + 256 + w * D, tmem + w * kKeys + s * 8, v + (s * 2048 >> 4), id_o, i > 0 || s > 0);
-        }
-        __syncwarp();
-        if (i + 1 < mine) {
-          if (!have_k) ring_wait(2 * i + 2);
-          have_k = true;
-          if (ok) scores(w, i + 1);
-        } else if (ptx::elect()) {
-          ptx::tc_commit(&o_full[w]);
-        }
-        __syncwarp();
+      for (int b = 0; b < 2; ++b) {
+        const int n = n0 + b;
+        if (!ok || n >= mine) continue;
+        wait(&p_full[2 * w + b], (n0 >> 1) & 1, kAttnWaitSoftmax);
+        if (!ok) continue;
+        values(b, (min(end[w] - key0 - n * kUnit, kUnit) + 15) / 16, n > 0);
+        if (n + 2 < mine) scores(b);
       }
       if (ok && ptx::elect()) {
-        ptx::tc_commit(&kv_empty[(2 * i + 1) % L::kStages]);
-        if (i + 1 < cnt) ptx::tc_commit(&kv_empty[(2 * i + 2) % L::kStages]);
+        ptx::tc_commit(&kv_empty[vs.st]);
+        if (n0 + 2 < cnt) ptx::tc_commit(&kv_empty[ks.st]);
       }
       __syncwarp();
+      vs.next();
+      ks.next();
     }
     if (!ok && ptx::elect()) {  // MMAs in flight finish before their memory is freed
-      ptx::tc_commit(drained);
-      ptx::wait_phase(drained, 0, abort_flag, a.err, kAttnWaitMma, false);
+      ptx::tc_commit(&drained[w]);
+      ptx::wait_phase(&drained[w], 0, abort_flag, a.err, kAttnWaitMma, false);
     }
     __syncwarp();
   } else {
@@ -327,7 +367,7 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
     const int w = warp >> 2;
     const int r = threadIdx.x & 127;
     const unsigned lanes = (unsigned)(32 * (warp & 3)) << 16;
-    const unsigned s_addr = tmem + lanes + w * kKeys, o_addr = tmem + lanes + 256 + w * D;
+    const unsigned o_addr = lanes + kTmO + w * D;
     const int tok_in = r / a.group, g = r - tok_in * a.group;
     const int tok = tok0 + w * a.tokens + tok_in;
     const bool live = tok_in < a.tokens && tok < q_len;
@@ -336,30 +376,32 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
     const float c = a.scale_log2;
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
-    for (int i = 0; i < mine; ++i) {
-      ok = __all_sync(0xffffffffu, ptx::wait_phase(&s_full[w], i & 1, abort_flag, a.err, kAttnWaitMma));
+    for (int n = 0; n < mine; ++n) {
+      ok = __all_sync(0xffffffffu,
+                      ptx::wait_phase(&s_full[2 * w + (n & 1)], (n >> 1) & 1, abort_flag, a.err, kAttnWaitMma));
       if (!ok) break;
       ptx::tc_fence_after();
-      const int lim = sees - (ja + i) * kKeys;  // keys of this step that the row sees
+      const unsigned s_addr = lanes + kTmS + w * 128 + (n & 1) * kUnit;
+      const int lim = sees - key0 - n * kUnit;  // keys of this step that the row sees
       bool done = false;
-      if (i > 0 && __all_sync(0xffffffffu, lim >= kKeys)) {
+      if (n > 0 && __all_sync(0xffffffffu, lim >= kUnit)) {
         // Every key is seen, and the maximum so far most likely serves: the
         // exponentials start with the first scores instead of after the last,
         // and count only if no score is too far above the maximum.
         const uint64_t c2 = ptx::pair(c, c);
         const float nb = m == -INFINITY ? 0.0f : -m * c;
         const uint64_t nb2 = ptx::pair(nb, nb);
-        unsigned p[64], u[2][32];
+        unsigned p[32], u[2][32];
         uint64_t sum[2] = {0, 0};
         float top[2] = {-INFINITY, -INFINITY};
         ptx::tmem_ld32(s_addr, u[0]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 2; ++k) {
           ptx::tc_wait_ld();
-          if (k < 3) ptx::tmem_ld32(s_addr + 32 * (k + 1), u[(k + 1) & 1]);
+          if (k < 1) ptx::tmem_ld32(s_addr + 32, u[1]);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float s0 = __uint_as_float(u[k & 1][2 * e]), s1 = __uint_as_float(u[k & 1][2 * e + 1]);
+            const float s0 = __uint_as_float(u[k][2 * e]), s1 = __uint_as_float(u[k][2 * e + 1]);
             top[e & 1] = ptx::max3(top[e & 1], s0, s1);
             float x0, x1;
             ptx::unpair(ptx::fma2(ptx::pair(s0, s1), c2, nb2), x0, x1);
@@ -372,7 +414,6 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
         done = !__any_sync(0xffffffffu, fmaxf(top[0], top[1]) * c > m * c + kSlack);
         if (done) {
           ptx::tmem_st32(s_addr, p);
-          ptx::tmem_st32(s_addr + 32, p + 32);
           float a0, a1;
           ptx::unpair(ptx::add2(sum[0], sum[1]), a0, a1);
           l += a0 + a1;
@@ -381,7 +422,7 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
       if (!done) {
         float mx = -INFINITY;
 #pragma unroll 1
-        for (int k = 0; k < kKeys; k += 32) {
+        for (int k = 0; k < kUnit; k += 32) {
           unsigned u[32];
           ptx::tmem_ld32(s_addr + k, u);
           ptx::tc_wait_ld();
@@ -389,11 +430,17 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
           for (int e = 0; e < 32; ++e)
             if (k + e < lim) mx = fmaxf(mx, __uint_as_float(u[e]));
         }
-        if (i == 0) {
+        if (n == 0) {
           m = mx;
         } else {
           const bool rise = mx * c > m * c + kSlack;
           if (__any_sync(0xffffffffu, rise)) {
+            // O is at rest once the step before is in it.
+            ok = __all_sync(0xffffffffu,
+                            ptx::wait_phase(&pv_done[2 * w + ((n - 1) & 1)], ((n - 1) >> 1) & 1, abort_flag, a.err,
+                                            kAttnWaitMma));
+            if (!ok) break;
+            ptx::tc_fence_after();
             const float f = rise ? ptx::ex2((m - mx) * c) : 1.0f;
             if (rise) m = mx;
             l *= f;
@@ -411,7 +458,7 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
         const float base = m == -INFINITY ? 0.0f : m * c;
         float sum[2] = {0.0f, 0.0f};
 #pragma unroll 1
-        for (int k = 0; k < kKeys; k += 32) {
+        for (int k = 0; k < kUnit; k += 32) {
           unsigned u[32], p[16];
           ptx::tmem_ld32(s_addr + k, u);
           ptx::tc_wait_ld();
@@ -430,9 +477,11 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
       ptx::tc_wait_st();
       ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&p_full[w]);
+      if (lane == 0) ptx::mbar_arrive(&p_full[2 * w + (n & 1)]);
     }
-    if (ok && mine > 0) ok = __all_sync(0xffffffffu, ptx::wait_phase(&o_full[w], 0, abort_flag, a.err, kAttnWaitMma));
+    if (ok && mine > 0)
+      ok = __all_sync(0xffffffffu, ptx::wait_phase(&pv_done[2 * w + ((mine - 1) & 1)], ((mine - 1) >> 1) & 1, abort_flag,
+                                                   a.err, kAttnWaitMma));
     if (ok) {
       ptx::tc_fence_after();
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -473,7 +522,7 @@ __global__ void __launch_bounds__(320, 1) attention_tc_kernel(const TcArgs a, co
   __syncthreads();
   if (warp == 8) {
     ptx::tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(*tmem_slot) : "memory");
   }
 }
 
@@ -808,7 +857,7 @@ void launch_tc_as(const TcArgs& t, const TcMaps& maps, cudaStream_t stream) {
   FA_CUDA(cudaFuncSetAttribute(attention_tc_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                TcLayout<D>::kTotal));
   const unsigned grid = (unsigned)t.tiles * t.kv_heads * t.splits;
-  attention_tc_kernel<D, BF16><<<grid, 320, TcLayout<D>::kTotal, stream>>>(t, maps);
+  attention_tc_kernel<D, BF16><<<grid, kTcThreads, TcLayout<D>::kTotal, stream>>>(t, maps);
   FA_CUDA(cudaGetLastError());
 }
 void launch_tc(const TcArgs& t, const TcMaps& maps, int dtype, cudaStream_t stream) {
@@ -859,7 +908,7 @@ int check_attention_packed(const fa_attention_packed_args* a) {
   need_strides(a->v_stride, 2);
   need_strides(a->out_stride, 2);
   if (!heads_supported(a->dtype, a->heads, a->kv_heads, a->head_size)) return kDeclined;
-  if (a->total_q * a->heads >= (1ll << 31) || a->total_k >= (1ll << 31)) return kDeclined;
+  if (a->total_q * a->heads >= (1ll << 31) || a->total_k >= (1ll << 30)) return kDeclined;
   if (a->total_q == 0 || a->sequences == 0) return kHandled;
   need(a->q && a->out && a->q_offsets && a->k_offsets, "null q, out, q_offsets or k_offsets");
   need(a->total_k == 0 || (a->k && a->v), "null k or v");
@@ -885,7 +934,7 @@ int check_attention_shared(const fa_attention_shared_args* a) {
   need_strides(a->suffix_v_stride, 3);
   need_strides(a->out_stride, 2);
   if (!heads_supported(a->dtype, a->heads, a->kv_heads, a->head_size)) return kDeclined;
-  if ((int64_t)a->sequences * a->heads >= (1ll << 31) || a->prefix_len + a->suffix_capacity >= (1ll << 31))
+  if ((int64_t)a->sequences * a->heads >= (1ll << 31) || a->prefix_len + a->suffix_capacity >= (1ll << 30))
     return kDeclined;
   if (a->sequences == 0) return kHandled;
   need(a->q && a->out, "null q or out");

@@ -91,19 +91,29 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
                : "memory");
 }
 
-// D[tmem] (+)= A[smem] x B[smem]; D is overwritten when acc == 0.
-__device__ __forceinline__ void tc_mma_ss(unsigned d, uint64_t a, uint64_t b, unsigned idesc, unsigned acc) {
+// Shared-memory matrix descriptor of a 128-byte-swizzled operand.  Upper word:
+// 1024 bytes between groups of 8 rows (64 at bit 32), version 1 (bit 46),
+// 128-byte swizzle (2 at bit 61).  Lower word: the address and `lbo`, the bytes
+// between 64-element blocks of the contiguous dimension where that one is not
+// the summed one, both in units of 16 bytes.
+constexpr unsigned kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ unsigned smem_desc_low(unsigned addr, unsigned lbo) { return (addr >> 4) | ((lbo >> 4) << 16); }
+// D[tmem] (+)= A[smem] x B[smem]; D is overwritten when acc == 0.  Descriptors
+// as their lower words (address and the contiguous dimension's block stride)
+// and the upper word that all operands here share.
+__device__ __forceinline__ void tc_mma_ss(unsigned d, unsigned a, unsigned b, unsigned idesc, bool acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n .reg .pred p;\n .reg .b64 da, db;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n"
+      " setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((unsigned)acc), "n"(kDescHigh)
       : "memory");
 }
 // D[tmem] (+)= A[tmem] x B[smem].
-__device__ __forceinline__ void tc_mma_ts(unsigned d, unsigned a, uint64_t b, unsigned idesc, unsigned acc) {
+__device__ __forceinline__ void tc_mma_ts(unsigned d, unsigned a, unsigned b, unsigned idesc, bool acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(
-          d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n .reg .pred p;\n .reg .b64 db;\n mov.b64 db, {%2, %5};\n"
+      " setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((unsigned)acc), "n"(kDescHigh)
       : "memory");
 }
 
@@ -116,13 +126,6 @@ __device__ __forceinline__ bool elect() {
   return r != 0;
 }
 
-// Shared-memory matrix descriptor of a 128-byte-swizzled operand: `lbo` bytes
-// between 64-element blocks of the contiguous dimension (where that one is not
-// the summed one), `sbo` bytes between groups of 8 rows.
-__device__ __forceinline__ uint64_t smem_desc_128b(unsigned addr, unsigned lbo, unsigned sbo) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
-         ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46) | (2ull << 61);
-}
 // Instruction descriptor of kind::f16: f32 accumulator (bit 4), operand types
 // (bits 7 and 10: 0 f16, 1 bf16), B stored along its rows (bit 16), N >> 3, M >> 4.
 __host__ __device__ constexpr unsigned idesc_f16(bool bf16, bool b_rows, int m, int n) {

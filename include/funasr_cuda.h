@@ -360,7 +360,8 @@ int fa_dev_status(fa_backend* backend);
  * Rows of out and lse outside q_offsets[0] .. q_offsets[sequences] stay as they were.
  * Limits (else FA_DECLINED): FA_DTYPE_F16 or FA_DTYPE_BF16; head_size a multiple
  * of 8 up to 128; heads / kv_heads up to 64; every base address and stride a
- * multiple of 16 bytes (the stride of a dimension of length one counts too); total_q * heads and total_k below 2^31. */
+ * multiple of 16 bytes (the stride of a dimension of length one counts too); total_q * heads
+ * below 2^31, total_k below 2^30. */
 typedef struct fa_attention_packed_args {
   const void* q;            /* [total_q x heads x head_size] */
   const void* k;            /* [total_k x kv_heads x head_size] */
