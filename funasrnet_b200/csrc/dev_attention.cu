@@ -873,12 +873,6 @@ void launch_join(const JoinArgs& j, int dtype, cudaStream_t stream) {
   launch_after(dtype == FA_DTYPE_BF16 ? join_kernel<__nv_bfloat16> : join_kernel<__half>, grid, 128, stream, j);
 }
 
-int* error_word() {
-  void* p = nullptr;
-  FA_CUDA(cudaGetSymbolAddress(&p, g_dev_error));
-  return static_cast<int*>(p);
-}
-
 // Query rows as (channel, head of the group, KV head, token).
 void encode_q(CUtensorMap* m, int dtype, const void* base, int head_size, int group, int kv_heads, int64_t tokens,
               const int64_t* stride, int tile_tokens) {
@@ -1022,7 +1016,7 @@ void launch_attention_packed(const fa_attention_packed_args& a, cudaStream_t str
   t.out_token = a.out_stride[0];
   t.out_head = a.out_stride[1];
   t.lse = a.lse;
-  t.err = error_word();
+  t.err = device_error_word();
   if (t.splits > 1) {
     t.part_o = static_cast<float*>(a.workspace);
     t.part_lse = t.part_o + t.splits * a.total_q * a.heads * a.head_size;
@@ -1077,7 +1071,7 @@ void launch_attention_shared(const fa_attention_shared_args& a, cudaStream_t str
     t.scale_log2 = scale_log2;
     t.part_o = part_o;
     t.part_lse = part_lse;
-    t.err = error_word();
+    t.err = device_error_word();
     TcMaps maps;
     encode_q(&maps.q, a.dtype, a.q, a.head_size, group, a.kv_heads, a.sequences, a.q_stride, t.tokens);
     encode_kv(&maps.k, a.dtype, a.prefix_k, a.head_size, a.kv_heads, a.prefix_len, a.prefix_k_stride);
@@ -1147,6 +1141,12 @@ void launch_attention_shared(const fa_attention_shared_args& a, cudaStream_t str
     j.lse = a.lse;
     launch_join(j, a.dtype, stream);
   }
+}
+
+int* device_error_word() {
+  void* p = nullptr;
+  FA_CUDA(cudaGetSymbolAddress(&p, g_dev_error));
+  return static_cast<int*>(p);
 }
 
 int take_device_error() {

@@ -1,11 +1,15 @@
 // Penalties, biases and masks on logits, and the greedy pick (fa_dev_adjust_logits).
 //
-// One thread-block cluster per row.  Its CTAs share the vocabulary in windows;
-// a CTA counts the row's history over its window in shared memory (integer
-// atomics, so the order of arrival cannot change a result), then streams the
-// window's logits once: read, change, write, and keep the best (value, index).
-// The cluster's CTAs hand their best to the first one through distributed
-// shared memory.  Bound: the logits' bytes, read once and written once.
+// Almost every logit only passes through: the history and the biases touch a few
+// hundred tokens of a vocabulary.  So a CTA first marks those in a bitmap and
+// gathers (token, times generated, last bias entry) in a hash table, both in
+// shared memory and with integer atomics, so that the order of arrival cannot
+// change a result; then it streams its part of the row, copying bits, writing
+// -inf under the mask and keeping the largest unmarked value; then it computes
+// the marked tokens, one thread each.  (Counts per token in shared memory, looked
+// up for every logit, took twice as long: the tables held the stream up.)  The
+// CTAs of a row form a cluster and send their best (value, index) to the first.
+// One launch, no scratch.  Bound: the logits' bytes, read once and written once.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -13,6 +17,7 @@
 #include <algorithm>
 
 #include "dev_ops.h"
+#include "dev_ptx.cuh"
 
 namespace fa {
 
@@ -20,16 +25,16 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kCluster = 8;        // CTAs per row
-constexpr int kWindow = 8192;      // tokens per window at most (two words of shared memory each)
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kMaxCluster = 16;
+constexpr int kSlots = 2048;   // hash table; also the tokens of a pass once it overflows
+constexpr int kUnroll = 4;     // 16-byte groups per thread and iteration
+constexpr int kWanted = 148;   // CTAs from which a row is not cut further
+constexpr int kMinSpan = 2048, kMaxSpan = 1 << 20;  // tokens of a CTA
 
 void need(bool ok, const char* what) {
   if (!ok) throw Error(kErrArgument, what);
 }
-
-template <typename T>
-__device__ __forceinline__ float to_f32(T v) { return (float)v; }
 
 struct Best {
   float v;
@@ -50,29 +55,96 @@ __device__ __forceinline__ Best warp_best(Best b) {
   return b;
 }
 
-__device__ __forceinline__ long long clamp_off(int x, long long hi) { return min((long long)max(x, 0), hi); }
+__device__ __forceinline__ int clamp_off(int x, long long hi) { return (int)min((long long)max(x, 0), hi); }
+
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// Writes `b` to `slot` of the cluster's first CTA and counts its bytes on that
+// CTA's barrier.
+__device__ __forceinline__ void send_best(Best b, Best* slot, uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .b32 s, m;\n .reg .b64 v;\n mapa.shared::cluster.u32 s, %0, 0;\n mapa.shared::cluster.u32 m, %1, 0;\n"
+      " mov.b64 v, {%2, %3};\n st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [s], v, [m];\n}\n" ::"r"(
+          ptx::saddr(slot)),
+      "r"(ptx::saddr(bar)), "r"(__float_as_uint(b.v)), "r"(b.i)
+      : "memory");
+}
+
+constexpr int kLogitsWait = 51;  // error-word code of a best value that never came
+
+// f(token, index) for the entries [i0, i1) of a list, by all threads of the CTA.
+template <typename F>
+__device__ __forceinline__ void for_entries(const int* list, int i0, int i1, F&& f) {
+  for (int i = i0 + (int)threadIdx.x; i < i1; i += 4 * kThreads) {
+    int t[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) t[k] = i1 - i > k * kThreads ? list[i + k * kThreads] : -1;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f(t[k], i + k * kThreads);
+  }
+}
+
+// The bits of tokens e .. last (fewer than 32) from 32-bit words whose first stands for tokens 32 * w0 on.
+__device__ __forceinline__ unsigned bits_of(const unsigned* words, int w0, int e, int last) {
+  return __funnelshift_r(words[(e >> 5) - w0], words[(last >> 5) - w0], e & 31);
+}
 
 template <typename T>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads)
-    adjust_logits_kernel(const fa_logits_args a, int window, int windows) {
-  extern __shared__ unsigned sm_words[];
-  unsigned* seen = sm_words;                          // bit 31: in the history; below: times generated
-  int* bias_at = reinterpret_cast<int*>(sm_words + (a.history ? window : 0));  // last bias entry + 1
-  __shared__ Best part[kThreads / 32];
-  __shared__ Best mine;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int rank = (int)cluster.block_rank();
-  const int row = blockIdx.x / kCluster;
-  constexpr int VE = 16 / sizeof(T);
+__global__ void __launch_bounds__(kThreads, 2) adjust_logits_kernel(const fa_logits_args a, int span, int* err) {
+  constexpr int VE = 16 / sizeof(T), U = kUnroll, kStep = kThreads * VE;
+  constexpr unsigned kFull = (1u << VE) - 1;
+  extern __shared__ __align__(16) unsigned marks[];  // one bit per token of the part
+  __shared__ int slot_token[kSlots];      // -1: free
+  __shared__ unsigned slot_seen[kSlots];  // bit 31: in the prompt; below: times generated.  Then the new logit
+  __shared__ int slot_bias[kSlots];       // last bias entry + 1
+  __shared__ int overflow;
+  __shared__ __align__(16) Best from[kMaxCluster * kWarps];  // the first CTA: every warp's best
+  __shared__ uint64_t arrived;
+  const int rank = (int)cg::this_cluster().block_rank(), ranks = (int)cg::this_cluster().num_blocks();
+  const int row = blockIdx.x / ranks;
+  const int lo = rank * span, hi = min(lo + span, a.vocab);  // this CTA's tokens; span is a multiple of 32
 
-  const float rep = a.repetition ? a.repetition[row] : 1.0f;
-  const float pres = a.presence ? a.presence[row] : 0.0f;
-  const float freq = a.frequency ? a.frequency[row] : 0.0f;
-  long long h0 = 0, h1 = 0, made = 0, b0 = 0, b1 = 0;
+  const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
+  T* out = static_cast<T*>(a.out) + row * a.out_stride;
+  // Elements by which the row's start lies past a 16-byte boundary; vector
+  // loads start on the boundaries, vector stores where out lies alike.
+  const int skew = (int)((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T));
+  const bool alike = (reinterpret_cast<uintptr_t>(out) & 15) / sizeof(T) == (unsigned)skew;
+  const int first = (lo + skew) / VE * VE - skew + (int)threadIdx.x * VE;  // this thread's first group
+
+  auto load = [&](int e) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (e >= lo && e + VE <= hi) {
+      v = __ldcs(reinterpret_cast<const uint4*>(in + e));
+    } else if (e < hi) {  // the part's ragged ends
+      T* t = reinterpret_cast<T*>(&v);
+#pragma unroll
+      for (int i = 0; i < VE; ++i)
+        if (e + i >= lo && e + i < hi) t[i] = in[e + i];
+    }
+    return v;
+  };
+  uint4 v[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) v[u] = load(first + u * kStep);
+
+  if (ranks > 1 && a.tokens) {
+    if (threadIdx.x == 0) {
+      ptx::mbar_init(&arrived, 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      ptx::mbar_expect_tx(&arrived, (unsigned)(ranks * kWarps * sizeof(Best)));
+    }
+    cluster_arrive();
+  }
+  int h0 = 0, made = 0, h1 = 0, b0 = 0, b1 = 0;  // prompt [h0, made), generated [made, h1), biases [b0, b1)
   if (a.history) {
     h0 = clamp_off(a.history_offsets[row], a.history_total);
     h1 = clamp_off(a.history_offsets[row + 1], a.history_total);
-    made = h0 + (a.prompt_lens ? max(a.prompt_lens[row], 0) : 0);
+    if (a.prompt_lens) made = max(min(a.prompt_lens[row], h1 - h0), 0);
+    made += h0;
   }
   if (a.bias_tokens) {
     b0 = clamp_off(a.bias_offsets[row], a.bias_total);
@@ -83,105 +155,213 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads)
     const int r = a.mask_rows ? a.mask_rows[row] : row;
     if (r >= 0 && r < a.mask_count) mask = a.mask + r * a.mask_stride;
   }
-  const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
-  T* out = static_cast<T*>(a.out) + row * a.out_stride;
-  // Elements by which the row's start lies past a 16-byte boundary; vector
-  // loads start on the boundaries, vector stores where out lies alike.
-  const int skew = (int)((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T));
-  const bool alike = (reinterpret_cast<uintptr_t>(out) & 15) / sizeof(T) == (unsigned)skew;
+  const bool marked = h1 > h0 || b1 > b0;
+  const float rep = a.repetition ? a.repetition[row] : 1.0f;
+  const float pres = a.presence ? a.presence[row] : 0.0f;
+  const float freq = a.frequency ? a.frequency[row] : 0.0f;
 
+  auto clear = [&] {
+    for (int s = threadIdx.x; s < kSlots; s += kThreads) {
+      slot_token[s] = -1;
+      slot_seen[s] = 0;
+      slot_bias[s] = 0;
+    }
+  };
+  // Gathers the entries of tokens [g0, g1) into the slots: by hash, marking the
+  // tokens, or (kDirect) at token - g0.
+  auto gather = [&](auto direct, int g0, int g1) {
+    constexpr bool kDirect = decltype(direct)::value;
+    const unsigned n = g1 - g0;
+    auto slot_of = [&](int t) {
+      if (kDirect) {
+        slot_token[t - g0] = t;
+        return t - g0;
+      }
+      atomicOr(&marks[(t - lo) >> 5], 1u << (t & 31));
+      int s = (int)((unsigned)t * 2654435761u >> 21);  // multiplicative hash to 11 bits
+      for (int probe = 0; probe < 32; ++probe, s = (s + 1) & (kSlots - 1)) {
+        const int before = atomicCAS(&slot_token[s], -1, t);
+        if (before == -1 || before == t) return s;
+      }
+      overflow = 1;
+      return -1;
+    };
+    for_entries(a.history, h0, h1, [&](int t, int i) {
+      if ((unsigned)(t - g0) >= n) return;
+      const int s = slot_of(t);
+      if (s < 0) return;
+      if (i < made) atomicOr(&slot_seen[s], 0x80000000u);
+      else atomicAdd(&slot_seen[s], 1u);
+    });
+    for_entries(a.bias_tokens, b0, b1, [&](int t, int i) {
+      if ((unsigned)(t - g0) >= n) return;
+      const int s = slot_of(t);
+      if (s >= 0) atomicMax(&slot_bias[s], i - b0 + 1);
+    });
+  };
+  // The new logits of this thread's slots, in the place of what the slots counted.
+  auto compute = [&](const T* from_row) {
+    constexpr int K = kSlots / kThreads;
+    float x[K], bias[K];
+    unsigned allowed[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int s = threadIdx.x + k * kThreads, t = slot_token[s], b = slot_bias[s];
+      x[k] = t < 0 ? 0.0f : (float)from_row[t];
+      bias[k] = t < 0 || b == 0 ? 0.0f : a.bias_values[b0 + b - 1];
+      allowed[k] = t < 0 || mask == nullptr ? 1u : mask[t >> 5] >> (t & 31);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int s = threadIdx.x + k * kThreads;
+      const unsigned seen = slot_seen[s], n = seen & 0x7fffffffu;
+      float y = x[k];
+      if (seen != 0) y = y > 0.0f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
+      if (n != 0) y = __fsub_rn(y, __fadd_rn(__fmul_rn(freq, (float)n), pres));
+      if (slot_bias[s] != 0) y = __fadd_rn(y, bias[k]);
+      slot_seen[s] = __float_as_uint(allowed[k] & 1u ? y : -INFINITY);
+    }
+  };
+  if (marked) {
+    clear();
+    for (int i = threadIdx.x; i < span / 32; i += kThreads) marks[i] = 0;
+    if (threadIdx.x == 0) overflow = 0;
+    __syncthreads();
+    gather(std::false_type{}, lo, hi);
+    __syncthreads();
+    if (!overflow) compute(in);  // their logits' latency passes with the stream's first
+  }
+
+  // ---- the stream ----
   Best best{-INFINITY, -1};
-  for (int w = rank; w < windows; w += kCluster) {
-    const int lo = w * window, hi = min(lo + window, a.vocab);
-    __syncthreads();
-    if (a.history)
-      for (int i = threadIdx.x; i < window; i += kThreads) seen[i] = 0;
-    if (a.bias_tokens)
-      for (int i = threadIdx.x; i < window; i += kThreads) bias_at[i] = 0;
-    __syncthreads();
-    for (long long i = h0 + threadIdx.x; i < h1; i += kThreads) {
-      const int t = a.history[i];
-      if (t >= lo && t < hi) {
-        atomicOr(&seen[t - lo], 0x80000000u);
-        if (i >= made) atomicAdd(&seen[t - lo], 1u);
+  for (int e0 = first; e0 < hi; e0 += U * kStep) {
+    uint4 next[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) next[u] = load(e0 + (U + u) * kStep);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = e0 + u * kStep;
+      if (e >= hi) break;
+      const bool whole = e >= lo && e + VE <= hi;
+      const int from_e = max(e, lo), last = min(e + VE, hi) - 1;
+      unsigned keep = ~0u, open = ~0u;  // elements that stay as they are; that may be the largest
+      if (!whole) open = (kFull << (from_e - e)) & (kFull >> (e + VE - 1 - last));
+      if (mask) {
+        keep = bits_of(mask, 0, from_e, last) << (from_e - e);
+        open &= keep;
       }
-    }
-    for (long long i = b0 + threadIdx.x; i < b1; i += kThreads) {
-      const int t = a.bias_tokens[i];
-      if (t >= lo && t < hi) atomicMax(&bias_at[t - lo], (int)(i - b0) + 1);
-    }
-    __syncthreads();
-    const int groups = (hi - lo + skew + VE - 1 + (lo % VE)) / VE + 1;
-    const int first = (lo + skew) / VE * VE - skew;  // <= lo, on a boundary
-    for (int g = threadIdx.x; g < groups; g += kThreads) {
-      const int e0 = first + g * VE;
-      if (e0 >= hi) break;
-      const bool whole = e0 >= lo && e0 + VE <= hi;
-      T v[VE];
-      if (whole) {
-        *reinterpret_cast<uint4*>(v) = __ldcs(reinterpret_cast<const uint4*>(in + e0));
+      if (marked) {
+        const unsigned m = bits_of(marks, lo >> 5, from_e, last) << (from_e - e);
+        keep |= m;
+        open &= ~m;
+      }
+      T* t = reinterpret_cast<T*>(&v[u]);
+      float x[VE];
+#pragma unroll
+      for (int i = 0; i < VE; ++i) x[i] = (float)t[i];
+      if ((open & kFull) != kFull) {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          if (!((open >> i) & 1u)) x[i] = -INFINITY;
+          if (!((keep >> i) & 1u)) t[i] = T(-INFINITY);
+        }
+      }
+      float top = x[0];
+#pragma unroll
+      for (int i = 1; i < VE; ++i) top = fmaxf(top, x[i]);
+      if (top > best.v) {
+        best.v = top;
+#pragma unroll
+        for (int i = VE - 1; i >= 0; --i)
+          if (x[i] == top) best.i = e + i;
+      }
+      if (alike && whole) {
+        __stcs(reinterpret_cast<uint4*>(out + e), v[u]);
       } else {
 #pragma unroll
         for (int i = 0; i < VE; ++i)
-          if (e0 + i >= lo && e0 + i < hi) v[i] = in[e0 + i];
+          if (e + i >= lo && e + i < hi) out[e + i] = t[i];
       }
+    }
 #pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        const int t = e0 + i;
-        if (t < lo || t >= hi) continue;
-        float x = to_f32(v[i]);
-        if (a.history) {
-          const unsigned s = seen[t - lo];
-          if (s != 0) {
-            x = x > 0.0f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-            const unsigned n = s & 0x7fffffffu;
-            if (n != 0) x = __fsub_rn(x, __fadd_rn(__fmul_rn(freq, (float)n), pres));
-          }
-        }
-        if (a.bias_tokens) {
-          const int at = bias_at[t - lo];
-          if (at != 0) x = __fadd_rn(x, a.bias_values[b0 + at - 1]);
-        }
-        if (mask && !((mask[t >> 5] >> (t & 31)) & 1u)) x = -INFINITY;
-        if (x > best.v) best = Best{x, t};
-        v[i] = (T)x;
+    for (int u = 0; u < U; ++u) v[u] = next[u];
+  }
+
+  // ---- the marked tokens, whose logits the stream left as they were ----
+  if (marked) {
+    auto finish = [&] {
+#pragma unroll
+      for (int k = 0; k < kSlots / kThreads; ++k) {
+        const int s = threadIdx.x + k * kThreads, t = slot_token[s];
+        if (t < 0) continue;
+        const float x = __uint_as_float(slot_seen[s]);
+        if (x > best.v || (x == best.v && best.i >= 0 && t < best.i)) best = Best{x, t};
+        out[t] = (T)x;
       }
-      if (whole && alike) {
-        __stcs(reinterpret_cast<uint4*>(out + e0), *reinterpret_cast<const uint4*>(v));
-      } else {
-#pragma unroll
-        for (int i = 0; i < VE; ++i)
-          if (e0 + i >= lo && e0 + i < hi) out[e0 + i] = v[i];
+    };
+    __syncthreads();
+    if (!overflow) {
+      finish();
+    } else {  // more tokens than slots: a range of kSlots tokens at a time
+      for (int g0 = lo; g0 < hi; g0 += kSlots) {
+        __syncthreads();
+        clear();
+        __syncthreads();
+        gather(std::true_type{}, g0, min(g0 + kSlots, hi));
+        __syncthreads();
+        compute(out);
+        finish();
       }
     }
   }
+  if (a.tokens == nullptr) return;
+  const int warp = threadIdx.x >> 5;
   best = warp_best(best);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = best;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    best = threadIdx.x < kThreads / 32 ? part[threadIdx.x] : Best{-INFINITY, -1};
-    best = warp_best(best);
-    if (threadIdx.x == 0) mine = best;
+  if (ranks == 1) {
+    if ((threadIdx.x & 31) == 0) from[warp] = best;
+    __syncthreads();
+    if (warp != 0) return;
+  } else {
+    cluster_wait();  // the first CTA's barrier is ready since its start
+    if ((threadIdx.x & 31) == 0) send_best(best, &from[rank * kWarps + warp], &arrived);
+    if (rank != 0 || warp != 0) return;
+    // The copies are on their way from CTAs that wait for nothing: bounded all the same.
+    bool here = false;
+    for (int i = 0; i < (1 << 24) && !here; ++i) here = ptx::mbar_try_wait(&arrived, 0);
+    here = __all_sync(0xffffffffu, here);
+    if (!here) {
+      if (threadIdx.x == 0) atomicCAS(err, 0, kLogitsWait);
+      return;
+    }
   }
-  cluster.sync();
-  if (rank == 0 && threadIdx.x < 32) {
-    best = threadIdx.x < kCluster ? *cluster.map_shared_rank(&mine, (int)threadIdx.x) : Best{-INFINITY, -1};
-    best = warp_best(best);
-    if (threadIdx.x == 0 && a.tokens) a.tokens[row] = best.i;
-  }
-  cluster.sync();  // the others' shared memory stays until it was read
+  best = Best{-INFINITY, -1};
+  for (int i = threadIdx.x; i < ranks * kWarps; i += 32) best = pick(best, from[i]);
+  best = warp_best(best);
+  if (threadIdx.x == 0) a.tokens[row] = best.i;
 }
 
 template <typename T>
 void launch(const fa_logits_args& a, cudaStream_t stream) {
-  const int rounds = (a.vocab + kCluster * kWindow - 1) / (kCluster * kWindow);
-  int window = (a.vocab + kCluster * rounds - 1) / (kCluster * rounds);
-  window = (window + 127) / 128 * 128;
-  const int windows = (a.vocab + window - 1) / window;
-  const int words = (a.history ? window : 0) + (a.bias_tokens ? window : 0);
-  FA_CUDA(cudaFuncSetAttribute(adjust_logits_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * 4 * kWindow));
-  adjust_logits_kernel<T><<<(unsigned)a.rows * kCluster, kThreads, words * 4, stream>>>(a, window, windows);
-  FA_CUDA(cudaGetLastError());
+  int ranks = 1;
+  while (ranks < kMaxCluster && (a.rows * (int64_t)ranks < kWanted || a.vocab > ranks * kMaxSpan) &&
+         a.vocab > ranks * kMinSpan)
+    ranks *= 2;
+  const int span = ((a.vocab + ranks - 1) / ranks + 31) / 32 * 32;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = (unsigned)a.rows * ranks;
+  cfg.blockDim = kThreads;
+  cfg.dynamicSmemBytes = a.history || a.bias_tokens ? span / 8 : 0;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ranks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  FA_CUDA(cudaFuncSetAttribute(adjust_logits_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               FA_LOGITS_MAX_VOCAB / kMaxCluster / 8));
+  FA_CUDA(cudaFuncSetAttribute(adjust_logits_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  FA_CUDA(cudaLaunchKernelEx(&cfg, adjust_logits_kernel<T>, a, span, device_error_word()));
 }
 
 }  // namespace

@@ -29,6 +29,8 @@ void launch_attention_packed(const fa_attention_packed_args& a, cudaStream_t str
 void launch_attention_shared(const fa_attention_shared_args& a, cudaStream_t stream);
 void launch_adjust_logits(const fa_logits_args& a, cudaStream_t stream);
 
+// The current context's error word, which a bounded wait that gives up sets.
+int* device_error_word();
 // Waits for the device, then the error word of its current context's kernels
 // (0: no bounded wait gave up), cleared by the read.
 int take_device_error();

@@ -41,7 +41,7 @@ constexpr uint64_t kWaitNs = 2000000000ull;  // one wait gives up after 2 s
 // Bounded wait on an mbarrier phase.  Gives up when the CTA's abort flag is up
 // or after kWaitNs, raising the flag and recording `code` in *err.
 // honour_abort = false for the drains, which outlast the copies in flight.
-__device__ __noinline__ bool wait_phase_slow(uint64_t* bar, unsigned parity, volatile int* abort_flag, int* err,
+static __device__ __noinline__ bool wait_phase_slow(uint64_t* bar, unsigned parity, volatile int* abort_flag, int* err,
                                              int code, bool honour_abort) {
   const uint64_t t0 = globaltimer();
   for (unsigned it = 1;; ++it) {
