@@ -10,6 +10,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -17,6 +18,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libfunasr_cuda.so"
+BINDING = PKG / "_torch_ops.so"  # CPython module of device_ops.py
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # -fmad=false: every a*b+c stays two roundings unless a kernel asks for an FMA
@@ -58,9 +60,10 @@ def _compile(src: Path, obj: Path) -> str:
 
 def build_library(verbose: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
-    deps = sorted(CSRC.glob("*")) + [ROOT / "include" / "funasr_cuda.h"]
+    deps = [p for p in sorted(CSRC.glob("*")) if p.name != "torch_binding.cpp"] + [ROOT / "include" / "funasr_cuda.h"]
     newest = max(p.stat().st_mtime for p in deps)
     if LIB.exists() and LIB.stat().st_mtime >= newest and os.environ.get("FA_FORCE_BUILD") != "1":
+        build_binding()
         return LIB
     objs = []
     with cf.ThreadPoolExecutor(max_workers=len(SOURCES)) as ex:
@@ -80,7 +83,35 @@ def build_library(verbose: bool = False) -> Path:
     if r.returncode != 0:
         raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
     tmp.replace(LIB)
+    build_binding()
     return LIB
+
+
+def build_binding() -> Path:
+    """_torch_ops: the CPython binding of the device-pointer operators for torch tensors.  It calls the library
+    next to it and the installed torch's C++ interface, so it is rebuilt when torch's version changes."""
+    import torch
+
+    src = CSRC / "torch_binding.cpp"
+    stamp = BUILD / "torch_version"
+    newest = max(src.stat().st_mtime, (ROOT / "include" / "funasr_cuda.h").stat().st_mtime)
+    if (BINDING.exists() and BINDING.stat().st_mtime >= newest and stamp.exists()
+            and stamp.read_text() == torch.__version__):
+        return BINDING
+    BUILD.mkdir(exist_ok=True)
+    home = Path(torch.__file__).parent
+    gxx = "/usr/bin/g++" if Path("/usr/bin/g++").exists() else shutil.which("g++")
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-isystem", str(home / "include"), "-isystem", str(home / "include" / "torch" / "csrc" / "api" / "include"),
+           "-isystem", sysconfig.get_path("include"), str(src), "-o", str(tmp), "-L", str(PKG), f"-l:{LIB.name}",
+           "-Wl,-rpath,$ORIGIN", "-L", str(home / "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"binding build failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    tmp.replace(BINDING)
+    stamp.write_text(torch.__version__)
+    return BINDING
 
 
 def build_oracle() -> Path:

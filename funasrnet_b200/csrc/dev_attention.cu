@@ -854,8 +854,6 @@ void launch_after(void (*kernel)(P...), unsigned grid, unsigned block, cudaStrea
 
 template <int D, bool BF16>
 void launch_tc_as(const TcArgs& t, const TcMaps& maps, cudaStream_t stream) {
-  FA_CUDA(cudaFuncSetAttribute(attention_tc_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               TcLayout<D>::kTotal));
   const unsigned grid = (unsigned)t.tiles * t.kv_heads * t.splits;
   attention_tc_kernel<D, BF16><<<grid, kTcThreads, TcLayout<D>::kTotal, stream>>>(t, maps);
   FA_CUDA(cudaGetLastError());
@@ -994,7 +992,17 @@ int64_t attention_shared_workspace(int64_t prefix_len, int64_t suffix_capacity, 
   return part_bytes(p.parts(), (int64_t)sequences * heads, head_size);
 }
 
-void launch_attention_packed(const fa_attention_packed_args& a, cudaStream_t stream) {
+void prepare_dev_attention() {
+  auto set = [](auto kernel, int bytes) {
+    FA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  };
+  set(attention_tc_kernel<64, false>, TcLayout<64>::kTotal);
+  set(attention_tc_kernel<64, true>, TcLayout<64>::kTotal);
+  set(attention_tc_kernel<128, false>, TcLayout<128>::kTotal);
+  set(attention_tc_kernel<128, true>, TcLayout<128>::kTotal);
+}
+
+void launch_attention_packed(const fa_attention_packed_args& a, int* err, cudaStream_t stream) {
   if (a.total_q == 0 || a.sequences == 0) return;
   TcArgs t;
   t.q_off = a.q_offsets;
@@ -1016,7 +1024,7 @@ void launch_attention_packed(const fa_attention_packed_args& a, cudaStream_t str
   t.out_token = a.out_stride[0];
   t.out_head = a.out_stride[1];
   t.lse = a.lse;
-  t.err = device_error_word();
+  t.err = err;
   if (t.splits > 1) {
     t.part_o = static_cast<float*>(a.workspace);
     t.part_lse = t.part_o + t.splits * a.total_q * a.heads * a.head_size;
@@ -1048,7 +1056,7 @@ void launch_attention_packed(const fa_attention_packed_args& a, cudaStream_t str
   }
 }
 
-void launch_attention_shared(const fa_attention_shared_args& a, cudaStream_t stream) {
+void launch_attention_shared(const fa_attention_shared_args& a, int* err, cudaStream_t stream) {
   if (a.sequences == 0) return;
   const SharedPlan plan = shared_plan(a.prefix_len, a.suffix_capacity, a.sequences, a.heads, a.kv_heads);
   const int64_t rows = (int64_t)a.sequences * a.heads;
@@ -1071,7 +1079,7 @@ void launch_attention_shared(const fa_attention_shared_args& a, cudaStream_t str
     t.scale_log2 = scale_log2;
     t.part_o = part_o;
     t.part_lse = part_lse;
-    t.err = device_error_word();
+    t.err = err;
     TcMaps maps;
     encode_q(&maps.q, a.dtype, a.q, a.head_size, group, a.kv_heads, a.sequences, a.q_stride, t.tokens);
     encode_kv(&maps.k, a.dtype, a.prefix_k, a.head_size, a.kv_heads, a.prefix_len, a.prefix_k_stride);

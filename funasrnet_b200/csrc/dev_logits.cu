@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 2) adjust_logits_kernel(const fa_log
 }
 
 template <typename T>
-void launch(const fa_logits_args& a, cudaStream_t stream) {
+void launch(const fa_logits_args& a, int* err, cudaStream_t stream) {
   int ranks = 1;
   while (ranks < kMaxCluster && (a.rows * (int64_t)ranks < kWanted || a.vocab > ranks * kMaxSpan) &&
          a.vocab > ranks * kMinSpan)
@@ -358,13 +358,23 @@ void launch(const fa_logits_args& a, cudaStream_t stream) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
+  FA_CUDA(cudaLaunchKernelEx(&cfg, adjust_logits_kernel<T>, a, span, err));
+}
+
+template <typename T>
+void prepare() {
   FA_CUDA(cudaFuncSetAttribute(adjust_logits_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                FA_LOGITS_MAX_VOCAB / kMaxCluster / 8));
   FA_CUDA(cudaFuncSetAttribute(adjust_logits_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-  FA_CUDA(cudaLaunchKernelEx(&cfg, adjust_logits_kernel<T>, a, span, device_error_word()));
 }
 
 }  // namespace
+
+void prepare_dev_logits() {
+  prepare<float>();
+  prepare<__half>();
+  prepare<__nv_bfloat16>();
+}
 
 int check_logits(const fa_logits_args* a) {
   need(a != nullptr, "null arguments");
@@ -384,14 +394,14 @@ int check_logits(const fa_logits_args* a) {
   return kHandled;
 }
 
-void launch_adjust_logits(const fa_logits_args& a, cudaStream_t stream) {
+void launch_adjust_logits(const fa_logits_args& a, int* err, cudaStream_t stream) {
   if (a.rows == 0) return;
   if (a.dtype == FA_DTYPE_F32)
-    launch<float>(a, stream);
+    launch<float>(a, err, stream);
   else if (a.dtype == FA_DTYPE_F16)
-    launch<__half>(a, stream);
+    launch<__half>(a, err, stream);
   else
-    launch<__nv_bfloat16>(a, stream);
+    launch<__nv_bfloat16>(a, err, stream);
 }
 
 }  // namespace fa

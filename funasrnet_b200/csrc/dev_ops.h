@@ -25,10 +25,14 @@ int64_t attention_packed_workspace(int64_t total_q, int64_t total_k, int sequenc
 int64_t attention_shared_workspace(int64_t prefix_len, int64_t suffix_capacity, int sequences, int heads, int kv_heads,
                                    int head_size);
 
-void launch_attention_packed(const fa_attention_packed_args& a, cudaStream_t stream);
-void launch_attention_shared(const fa_attention_shared_args& a, cudaStream_t stream);
-void launch_adjust_logits(const fa_logits_args& a, cudaStream_t stream);
+// `err`: device_error_word() of the current device.
+void launch_attention_packed(const fa_attention_packed_args& a, int* err, cudaStream_t stream);
+void launch_attention_shared(const fa_attention_shared_args& a, int* err, cudaStream_t stream);
+void launch_adjust_logits(const fa_logits_args& a, int* err, cudaStream_t stream);
 
+// Function attributes of these kernels on the current device; before any launch.
+void prepare_dev_attention();
+void prepare_dev_logits();
 // The current context's error word, which a bounded wait that gives up sets.
 int* device_error_word();
 // Waits for the device, then the error word of its current context's kernels

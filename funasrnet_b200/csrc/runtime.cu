@@ -113,6 +113,7 @@ struct fa_backend {
   int models = 0;
   DevBuf in, out, aux, aux2;
   DevBuf bxq, bxs, berr;  // frame-tile operands of multi-frame projections
+  int* dev_error = nullptr;  // error word of the device-pointer operators
   std::vector<float> staging;
 };
 
@@ -240,6 +241,9 @@ int fa_backend_create(int device, fa_backend** out) {
     if (prop.major < 10) throw Error(kErrCuda, std::string("sm_100a build needs a Blackwell GPU, found ") + prop.name);
     FA_CUDA(cudaStreamCreateWithFlags(&b->stream, cudaStreamNonBlocking));
     prepare_kernels();
+    prepare_dev_attention();
+    prepare_dev_logits();
+    b->dev_error = device_error_word();
     b->name = std::string("CUDA ") + prop.name + " (sm_" + std::to_string(prop.major) + std::to_string(prop.minor) + ")";
     *out = b.release();
     return (int)kHandled;
@@ -719,7 +723,7 @@ int fa_lm_head_argmax_noalloc(fa_backend* b, const fa_weight* w, const float* x,
 // The arguments are checked before the backend, so that a refusal needs no device.
 template <typename Args>
 static int enqueue_dev(fa_backend* b, const Args* args, void* stream, int (*check)(const Args*),
-                       void (*launch)(const Args&, cudaStream_t)) {
+                       void (*launch)(const Args&, int*, cudaStream_t)) {
   return guarded([&] {
     const int rc = check(args);
     if (rc != kHandled) return rc;
@@ -727,7 +731,7 @@ static int enqueue_dev(fa_backend* b, const Args* args, void* stream, int (*chec
     std::lock_guard<std::mutex> lk(b->mu);
     if (b->disposed) throw Error(kErrDisposed, "backend disposed");
     DeviceGuard g(b->device);
-    launch(*args, stream != nullptr ? static_cast<cudaStream_t>(stream) : b->stream);
+    launch(*args, b->dev_error, stream != nullptr ? static_cast<cudaStream_t>(stream) : b->stream);
     return (int)kHandled;
   });
 }
