@@ -528,19 +528,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const TcArg
 
 // ------------------------------------------------------ one query a sequence ----
 
-constexpr int kRowWarps = 4;   // warps of a CTA, each with its own keys and softmax state
-constexpr int kChunk = 16;     // keys per step of a warp: the MMA's M
-constexpr int kRowHeads = 8;   // query heads of a CTA: the MMA's N
-
-struct Run {  // keys and values of one KV head: row i at k + i * k_row
-  const void *k = nullptr, *v = nullptr;
-  long long k_row = 0, v_row = 0, k_head = 0, v_head = 0, k_seq = 0, v_seq = 0;
-};
+constexpr int kRowWarps = 4;       // warps that compute, each 16 keys of a stage: the MMA's M
+constexpr int kRowThreads = 32 * (kRowWarps + 1);
+constexpr int kStageKeys = 16 * kRowWarps;
+constexpr int kRowHeads = 8;       // query heads of a CTA: the MMA's N
 
 struct RowsArgs {
   const void* q = nullptr;
   long long q_seq = 0, q_head = 0;
-  Run prefix, suffix;
   int prefix_len = 0;             // keys of the prefix that this kernel reads (0: attention_tc_kernel does)
   const int* suffix_lens = nullptr;
   int capacity = 0;
@@ -554,6 +549,23 @@ struct RowsArgs {
   float* part_o = nullptr;        // [splits x sequences x heads x head_size]
   float* part_lse = nullptr;      // [splits x sequences x heads]
   int wait = 0;                   // the launch before this one must be over when this one is
+  int* err = nullptr;
+};
+struct RowsMaps {
+  CUtensorMap pk, pv;  // prefix: (channel, KV head, key), 64 keys a copy
+  CUtensorMap sk, sv;  // suffix: (channel, KV head, key, sequence), 16 keys a copy: none behind the length but in the last
+};
+
+template <int D>
+struct RowsLayout {
+  static constexpr int kHalf = kStageKeys * 128;  // 64 keys x 64 channels, 128-byte swizzle
+  static constexpr int kTile = D / 64 * kHalf;
+  static constexpr int kStages = D == 128 ? 3 : 4;
+  static constexpr int kBars = kStages * 2 * kTile;
+  static constexpr int kMisc = kBars + 8 * 3 * kStages;
+  static constexpr int kTotal = kMisc + 16 + 1024;
+  static constexpr int kOut = kRowWarps * kRowHeads * (D + 4) * 4;  // the warps' sums, over the ring
+  static_assert(kOut + 2 * kRowWarps * kRowHeads * 4 <= kBars, "joining the warps");
 };
 
 // D (m16n8) += A (m16k16) x B (k16n8), f32 accumulator.
@@ -575,32 +587,39 @@ __device__ __forceinline__ unsigned transpose8(unsigned x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint4 load16(const void* p) {
+__device__ __forceinline__ uint4 lds16(unsigned addr) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
   return v;
 }
 
 // One query token of one sequence, up to 8 of the heads that share a KV head.
-// The keys stream from global memory straight into MMA operands: a warp takes
-// 16 keys a step and lane (g = lane / 4, t = lane % 4) loads
-//   K rows g and g + 8, channels 32b + 8t .. + 7   (16 bytes each),
-//   V rows 2t, 2t + 1, 2t + 8, 2t + 9, channels 64h + 8g .. + 7.
-// S^T = K Q^T sums over channels, whose order is free as long as Q has the same:
-// the four words of a 16-byte load serve as the k index of two MMAs.  O^T = V^T P^T
-// needs pairs of keys in a word: two rows' words interleaved by prmt, so that
-// the MMA of word r has channels 64h + 8g + 2r and + 2r + 1 as its rows g and g + 8.
-// P^T goes from S^T's layout to the operand's through movmatrix.  No shared
-// memory until the warps' sums are joined at the end.  Bound: the bytes of K
-// and V; the heads share them, so N = 8 serves groups up to 8 in one pass.
+// Warp 4 streams the keys through a ring of 64-key stages (TMA); warp w takes
+// keys 16w .. 16w + 15 of a stage, and lane (g = lane / 4, t = lane % 4) reads
+//   K rows g and g + 8, chunks 2t and 2t + 1 of each 64 channels (16 bytes each),
+//   V rows 2t, 2t + 1, 2t + 8, 2t + 9, chunk g,
+// all without bank conflicts under the 128-byte swizzle.  S^T = K Q^T sums over
+// channels, whose order is free as long as Q has the same: the four words of a
+// chunk serve as the k index of two MMAs.  O^T = V^T P^T needs pairs of keys in
+// a word: two rows' words interleaved by prmt, so that the MMA of word r has
+// channels 64h + 8g + 2r and + 2r + 1 as its rows g and g + 8.  P^T goes from
+// S^T's layout to the operand's through movmatrix.  Bound: the bytes of K and V;
+// the heads share them, so N = 8 serves groups up to 8 in one pass.  (Loads from
+// global memory into registers needed the L1 for what was in flight: they ran at
+// half the rate on an SM whose memory the tensor-core kernel had claimed.)
 template <int D, bool BF16>
-__global__ void __launch_bounds__(32 * kRowWarps, 4) attention_rows_kernel(const RowsArgs a) {
+__global__ void __launch_bounds__(kRowThreads, 2) attention_rows_kernel(const RowsArgs a,
+                                                                        const __grid_constant__ RowsMaps maps) {
+  using L = RowsLayout<D>;
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   constexpr int KB = D / 32, VB = D / 64, NO = D / 16;
-  __shared__ float sm_o[kRowWarps][kRowHeads][D + 4];
-  __shared__ float sm_m[kRowWarps][kRowHeads], sm_l[kRowWarps][kRowHeads];
+  extern __shared__ uint8_t sm_raw[];
+  uint8_t* sm = sm_raw + ((1024 - (ptx::saddr(sm_raw) & 1023)) & 1023);
+  const unsigned sbase = ptx::saddr(sm);
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(sm + L::kBars);
+  uint64_t* v_full = k_full + L::kStages;
+  uint64_t* empty = v_full + L::kStages;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::kMisc);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   unsigned id = blockIdx.x;
   const int kvh = id % a.kv_heads;
@@ -610,23 +629,66 @@ __global__ void __launch_bounds__(32 * kRowWarps, 4) attention_rows_kernel(const
   const int split = id % a.splits;
   const int seq = id / a.splits;
   const int head0 = kvh * a.group + block * kRowHeads, n_heads = min(kRowHeads, a.group - block * kRowHeads);
-  const int own = a.suffix_lens ? clamp_to(a.suffix_lens[seq], a.capacity) : 0;
   ptx::griddep_launch();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < L::kStages; ++s) {
+      ptx::mbar_init(&k_full[s], 1);
+      ptx::mbar_init(&v_full[s], 1);
+      ptx::mbar_init(&empty[s], kRowWarps);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  const int own = a.suffix_lens ? clamp_to(a.suffix_lens[seq], a.capacity) : 0;
+  // Stages of 64 keys: the prefix's, then the sequence's own.
+  const int ps = (a.prefix_len + kStageKeys - 1) / kStageKeys, all = ps + (own + kStageKeys - 1) / kStageKeys;
+  const int s0 = (int)((long long)all * split / a.splits), s1 = (int)((long long)all * (split + 1) / a.splits);
+  __syncthreads();
 
-  // Chunks of 16 keys: the prefix's, then the sequence's own.
-  const int pc = (a.prefix_len + kChunk - 1) / kChunk, chunks = pc + (own + kChunk - 1) / kChunk;
-  const int c0 = (int)((long long)chunks * split / a.splits), c1 = (int)((long long)chunks * (split + 1) / a.splits);
-  const T* pk = static_cast<const T*>(a.prefix.k) + kvh * a.prefix.k_head;
-  const T* pv = static_cast<const T*>(a.prefix.v) + kvh * a.prefix.v_head;
-  const T* sk = static_cast<const T*>(a.suffix.k) + seq * a.suffix.k_seq + kvh * a.suffix.k_head;
-  const T* sv = static_cast<const T*>(a.suffix.v) + seq * a.suffix.v_seq + kvh * a.suffix.v_head;
+  if (warp == kRowWarps) {
+    // ---- copies ----
+    if (lane == 0) {
+      bool ok = true;
+      int n = 0;
+      for (int s = s0; s < s1 && ok; ++s, ++n) {
+        const int st = n % L::kStages;
+        if (n >= L::kStages)
+          ok = ptx::wait_phase(&empty[st], (n / L::kStages - 1) & 1, abort_flag, a.err, kAttnWaitFree);
+        if (!ok) break;
+        const bool prefix = s < ps;
+        const int key0 = (prefix ? s : s - ps) * kStageKeys;
+        const int copies = prefix ? 1 : min(kRowWarps, (own - key0 + 15) / 16);
+        const unsigned bytes = prefix ? L::kTile : copies * (L::kTile / kRowWarps);
+        for (int v = 0; v < 2; ++v) {
+          uint64_t* bar = v ? &v_full[st] : &k_full[st];
+          const unsigned dst = sbase + (2 * st + v) * L::kTile;
+          ptx::mbar_expect_tx(bar, bytes);
+          for (int h = 0; h < VB; ++h) {
+            if (prefix)
+              ptx::tma_load_3d(dst + h * L::kHalf, v ? &maps.pv : &maps.pk, h * 64, kvh, key0, bar);
+            else
+              for (int c = 0; c < copies; ++c)
+                ptx::tma_load_4d(dst + h * L::kHalf + c * 2048, v ? &maps.sv : &maps.sk, h * 64, kvh, key0 + 16 * c, seq,
+                                 bar);
+          }
+        }
+      }
+      for (int i = max(0, n - L::kStages); i < n; ++i) {  // copies in flight land before the CTA exits
+        ptx::wait_phase(&k_full[i % L::kStages], (i / L::kStages) & 1, abort_flag, a.err, kAttnWaitLoad, false);
+        ptx::wait_phase(&v_full[i % L::kStages], (i / L::kStages) & 1, abort_flag, a.err, kAttnWaitLoad, false);
+      }
+      if (a.wait && blockIdx.x == gridDim.x - 1) ptx::griddep_wait();
+    }
+    return;
+  }
 
-  unsigned q[KB][4];  // the B operand of S^T: head g, channels 32b + 8t .. + 7
+  unsigned q[KB][4];  // the B operand of S^T: head g, chunk 2t + (b & 1) of channels 64 (b / 2) ..
 #pragma unroll
   for (int b = 0; b < KB; ++b) {
+    const int c0 = 64 * (b >> 1) + 8 * (2 * t + (b & 1));
     uint4 v = make_uint4(0, 0, 0, 0);
-    if (g < n_heads && 32 * b + 8 * t < a.head_size)
-      v = load16(static_cast<const T*>(a.q) + seq * a.q_seq + (head0 + g) * a.q_head + 32 * b + 8 * t);
+    if (g < n_heads && c0 < a.head_size)
+      v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + seq * a.q_seq + (head0 + g) * a.q_head + c0);
     q[b][0] = v.x;
     q[b][1] = v.y;
     q[b][2] = v.z;
@@ -637,51 +699,28 @@ __global__ void __launch_bounds__(32 * kRowWarps, 4) attention_rows_kernel(const
   for (int i = 0; i < NO; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};  // heads 2t, 2t + 1
   const float c = a.scale_log2;
+  bool ok = true;
+  const unsigned k_row = sbase + (16 * warp + g) * 128, v_row = sbase + (16 * warp + 2 * t) * 128;
 
-  uint4 kx[2][KB];
-  auto load_k = [&](int ch) {
-    const bool own_keys = ch >= pc;
-    const int key0 = (own_keys ? ch - pc : ch) * kChunk, n = own_keys ? own : a.prefix_len;
-    const T* base = own_keys ? sk : pk;
-    const long long row = own_keys ? a.suffix.k_row : a.prefix.k_row;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int key = key0 + g + 8 * i;
-#pragma unroll
-      for (int b = 0; b < KB; ++b)
-        kx[i][b] = key < n && 32 * b + 8 * t < a.head_size ? load16(base + key * row + 32 * b + 8 * t)
-                                                           : make_uint4(0, 0, 0, 0);
-    }
-  };
-  int ch = c0 + warp;
-  if (ch < c1) load_k(ch);
-  for (; ch < c1; ch += kRowWarps) {
-    const bool own_keys = ch >= pc;
-    const int key0 = (own_keys ? ch - pc : ch) * kChunk, n = own_keys ? own : a.prefix_len;
-    uint4 vx[4][VB];
-    {
-      const T* base = own_keys ? sv : pv;
-      const long long row = own_keys ? a.suffix.v_row : a.prefix.v_row;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = key0 + 2 * t + (i & 1) + 8 * (i >> 1);
-#pragma unroll
-        for (int h = 0; h < VB; ++h)
-          vx[i][h] = key < n && 64 * h + 8 * g < a.head_size ? load16(base + key * row + 64 * h + 8 * g)
-                                                             : make_uint4(0, 0, 0, 0);
-      }
-    }
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // key g: heads 2t, 2t + 1; key g + 8: the same heads
+  for (int s = s0, n = 0; s < s1; ++s, ++n) {
+    const int st = n % L::kStages;
+    const unsigned ph = (n / L::kStages) & 1;
+    // Keys of this warp's 16 that exist; the rest of the stage holds what was there before.
+    const int left = (s < ps ? a.prefix_len - s * kStageKeys : own - (s - ps) * kStageKeys) - 16 * warp;
+    ok = __all_sync(0xffffffffu, ptx::wait_phase(&k_full[st], ph, abort_flag, a.err, kAttnWaitLoad));
+    if (!ok) break;
+    float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // key g: heads 2t, 2t + 1; key g + 8: the same heads
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
-      mma16816<BF16>(s, kx[0][b].x, kx[1][b].x, kx[0][b].y, kx[1][b].y, q[b][0], q[b][1]);
-      mma16816<BF16>(s, kx[0][b].z, kx[1][b].z, kx[0][b].w, kx[1][b].w, q[b][2], q[b][3]);
+      const unsigned at = k_row + 2 * st * L::kTile + (b >> 1) * L::kHalf + (((2 * t + (b & 1)) ^ g) << 4);
+      const uint4 k0 = lds16(at), k1 = lds16(at + 8 * 128);
+      mma16816<BF16>(sc, k0.x, k1.x, k0.y, k1.y, q[b][0], q[b][1]);
+      mma16816<BF16>(sc, k0.z, k1.z, k0.w, k1.w, q[b][2], q[b][3]);
     }
-    if (ch + kRowWarps < c1) load_k(ch + kRowWarps);
-    if (key0 + g >= n) s[0] = s[1] = -INFINITY;
-    if (key0 + g + 8 >= n) s[2] = s[3] = -INFINITY;
+    if (g >= left) sc[0] = sc[1] = -INFINITY;
+    if (g + 8 >= left) sc[2] = sc[3] = -INFINITY;
     // The maximum moves only when a score is 2^kSlack above it.
-    const float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
+    const float x0 = fmaxf(sc[0], sc[2]), x1 = fmaxf(sc[1], sc[3]);
     if (__any_sync(0xffffffffu, x0 * c > m[0] * c + kSlack || x1 * c > m[1] * c + kSlack)) {
       float x[2] = {x0, x1};
 #pragma unroll
@@ -700,53 +739,72 @@ __global__ void __launch_bounds__(32 * kRowWarps, 4) attention_rows_kernel(const
       }
     }
     const float base0 = m[0] == -INFINITY ? 0.0f : m[0] * c, base1 = m[1] == -INFINITY ? 0.0f : m[1] * c;
-    const float p0 = ptx::ex2(fmaf(s[0], c, -base0)), p1 = ptx::ex2(fmaf(s[1], c, -base1));
-    const float p2 = ptx::ex2(fmaf(s[2], c, -base0)), p3 = ptx::ex2(fmaf(s[3], c, -base1));
+    const float p0 = ptx::ex2(fmaf(sc[0], c, -base0)), p1 = ptx::ex2(fmaf(sc[1], c, -base1));
+    const float p2 = ptx::ex2(fmaf(sc[2], c, -base0)), p3 = ptx::ex2(fmaf(sc[3], c, -base1));
     l[0] += p0 + p2;
     l[1] += p1 + p3;
     const unsigned b0 = transpose8(ptx::pack16<BF16>(p0, p1)), b1 = transpose8(ptx::pack16<BF16>(p2, p3));
+    ok = __all_sync(0xffffffffu, ptx::wait_phase(&v_full[st], ph, abort_flag, a.err, kAttnWaitLoad));
+    if (!ok) break;
 #pragma unroll
     for (int h = 0; h < VB; ++h) {
-      const unsigned* v0 = reinterpret_cast<const unsigned*>(&vx[0][h]);
-      const unsigned* v1 = reinterpret_cast<const unsigned*>(&vx[1][h]);
-      const unsigned* v2 = reinterpret_cast<const unsigned*>(&vx[2][h]);
-      const unsigned* v3 = reinterpret_cast<const unsigned*>(&vx[3][h]);
+      uint4 vx[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = 2 * t + (i & 1) + 8 * (i >> 1);
+        const unsigned at = v_row + (2 * st + 1) * L::kTile + h * L::kHalf + ((i & 1) + 8 * (i >> 1)) * 128 + ((g ^ (key & 7)) << 4);
+        vx[i] = key < left ? lds16(at) : make_uint4(0, 0, 0, 0);
+      }
+      const unsigned* v0 = reinterpret_cast<const unsigned*>(&vx[0]);
+      const unsigned* v1 = reinterpret_cast<const unsigned*>(&vx[1]);
+      const unsigned* v2 = reinterpret_cast<const unsigned*>(&vx[2]);
+      const unsigned* v3 = reinterpret_cast<const unsigned*>(&vx[3]);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         mma16816<BF16>(o[4 * h + r], __byte_perm(v0[r], v1[r], 0x5410), __byte_perm(v0[r], v1[r], 0x7632),
                        __byte_perm(v2[r], v3[r], 0x5410), __byte_perm(v2[r], v3[r], 0x7632), b0, b1);
     }
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(&empty[st]);
   }
 
-  // ---- join the warps ----
+  // ---- join the warps, over the ring ----
+  float* sm_o = reinterpret_cast<float*>(sm);  // [warp][head][D + 4]
+  float* sm_m = sm_o + kRowWarps * kRowHeads * (D + 4);
+  float* sm_l = sm_m + kRowWarps * kRowHeads;
+  asm volatile("bar.sync 1, %0;" ::"n"(32 * kRowWarps) : "memory");  // every stage is used up
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
 #pragma unroll
     for (int d = 4; d < 32; d <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
     if (g == 0) {
-      sm_m[warp][2 * t + i] = m[i];
-      sm_l[warp][2 * t + i] = l[i];
+      sm_m[warp * kRowHeads + 2 * t + i] = m[i];
+      sm_l[warp * kRowHeads + 2 * t + i] = l[i];
     }
 #pragma unroll
     for (int h = 0; h < VB; ++h)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        *reinterpret_cast<float2*>(&sm_o[warp][2 * t + i][64 * h + 8 * g + 2 * r]) =
+        *reinterpret_cast<float2*>(sm_o + (warp * kRowHeads + 2 * t + i) * (D + 4) + 64 * h + 8 * g + 2 * r) =
             make_float2(o[4 * h + r][i], o[4 * h + r][2 + i]);
   }
-  __syncthreads();
+  asm volatile("bar.sync 1, %0;" ::"n"(32 * kRowWarps) : "memory");
+  if (*abort_flag) return;
   for (int e = threadIdx.x; e < n_heads * (D / 4); e += 32 * kRowWarps) {
     const int h = e / (D / 4), ch0 = (e % (D / 4)) * 4;
     float top = -INFINITY, sum = 0.0f, v[4] = {};
 #pragma unroll
-    for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, sm_m[w][h]);
+    for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, sm_m[w * kRowHeads + h]);
     const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
     for (int w = 0; w < kRowWarps; ++w) {
-      const float f = ptx::ex2((sm_m[w][h] - base) * c);
-      sum = fmaf(f, sm_l[w][h], sum);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = fmaf(f, sm_o[w][h][ch0 + i], v[i]);
+      const float f = ptx::ex2((sm_m[w * kRowHeads + h] - base) * c);
+      sum = fmaf(f, sm_l[w * kRowHeads + h], sum);
+      const float4 x = *reinterpret_cast<const float4*>(sm_o + (w * kRowHeads + h) * (D + 4) + ch0);
+      v[0] = fmaf(f, x.x, v[0]);
+      v[1] = fmaf(f, x.y, v[1]);
+      v[2] = fmaf(f, x.z, v[2]);
+      v[3] = fmaf(f, x.w, v[3]);
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
@@ -765,11 +823,11 @@ __global__ void __launch_bounds__(32 * kRowWarps, 4) attention_rows_kernel(const
       else if (a.lse) a.lse[row] = lse;
     }
   }
-  if (a.wait && blockIdx.x == gridDim.x - 1) ptx::griddep_wait();
 }
 
 // Joins the parts of a row: lse = log sum_s e^lse_s, out = sum_s e^(lse_s - lse) o_s,
-// in the order of the parts.  One warp per row.
+// in a fixed order.  W warps per row, each taking every W-th part: one walks 74
+// parts in 26 us, four in a quarter of it.
 struct JoinArgs {
   const int* q_off = nullptr;  // rows of [q_off[0], q_off[sequences]) only (null: all)
   int sequences = 0;
@@ -782,34 +840,56 @@ struct JoinArgs {
   float* lse = nullptr;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(128) join_kernel(const JoinArgs a) {
-  const long long rows = a.tokens * a.heads, row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+constexpr int kJoinWarps = 4;
+
+template <typename T, int W>
+__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const JoinArgs a) {
+  __shared__ float4 sm_o[kJoinWarps][32];
+  __shared__ float sm_sum[kJoinWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long rows = a.tokens * a.heads, row = (long long)blockIdx.x * (kJoinWarps / W) + warp / W;
+  const int part = warp % W, c = lane * 4;
   ptx::griddep_wait();
-  if (row >= rows) return;
   const long long t = row / a.heads;
   const int h = (int)(row - t * a.heads);
-  if (a.q_off && (t < a.q_off[0] || t >= a.q_off[a.sequences])) return;
-  float top = -INFINITY;
-  for (int s = lane; s < a.parts; s += 32) top = fmaxf(top, a.part_lse[s * rows + row]);
+  const bool live = row < rows && (!a.q_off || (t >= a.q_off[0] && t < a.q_off[a.sequences]));
+  float top = -INFINITY, sum = 0.0f, o[4] = {};
+  if (live) {
+    for (int s = lane; s < a.parts; s += 32) top = fmaxf(top, a.part_lse[s * rows + row]);
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  }
   const float base = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f, o[4] = {};
-  const int c = lane * 4;
-#pragma unroll 4
-  for (int s = 0; s < a.parts; ++s) {
-    const float f = expf(a.part_lse[s * rows + row] - base);
-    sum += f;
-    if (c < a.head_size) {
-      const float4 v = *reinterpret_cast<const float4*>(a.part_o + (s * rows + row) * a.head_size + c);
-      o[0] = fmaf(f, v.x, o[0]);
-      o[1] = fmaf(f, v.y, o[1]);
-      o[2] = fmaf(f, v.z, o[2]);
-      o[3] = fmaf(f, v.w, o[3]);
+  if (live) {
+#pragma unroll 8
+    for (int s = part; s < a.parts; s += W) {
+      const float f = expf(a.part_lse[s * rows + row] - base);
+      sum += f;
+      if (c < a.head_size) {
+        const float4 v = *reinterpret_cast<const float4*>(a.part_o + (s * rows + row) * a.head_size + c);
+        o[0] = fmaf(f, v.x, o[0]);
+        o[1] = fmaf(f, v.y, o[1]);
+        o[2] = fmaf(f, v.z, o[2]);
+        o[3] = fmaf(f, v.w, o[3]);
+      }
     }
   }
+  if (W > 1) {
+    sm_o[warp][lane] = make_float4(o[0], o[1], o[2], o[3]);
+    if (lane == 0) sm_sum[warp] = sum;
+    __syncthreads();
+    if (part != 0) return;
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      const float4 v = sm_o[warp + w][lane];
+      sum += sm_sum[warp + w];
+      o[0] += v.x;
+      o[1] += v.y;
+      o[2] += v.z;
+      o[3] += v.w;
+    }
+  }
+  if (!live) return;
   if (c < a.head_size) {
     T* out = static_cast<T*>(a.out) + t * a.out_token + h * a.out_head;
     T v[4];
@@ -830,25 +910,38 @@ CUtensorMapDataType map_type(int dtype) {
 }
 
 // K or V: (channel, KV head, key), 64 channels x 128 keys a copy.
-void encode_kv(CUtensorMap* m, int dtype, const void* base, int head_size, int kv_heads, int64_t keys, const int64_t* stride) {
+void encode_kv(CUtensorMap* m, int dtype, const void* base, int head_size, int kv_heads, int64_t keys,
+               const int64_t* stride, int box_keys = kKeys) {
   const cuuint64_t dims[3] = {(cuuint64_t)head_size, (cuuint64_t)kv_heads, (cuuint64_t)keys};
   const cuuint64_t strides[2] = {map_stride(kv_heads, stride[1]), map_stride(keys, stride[0])};
-  const cuuint32_t box[3] = {64, 1, kKeys};
+  const cuuint32_t box[3] = {64, 1, (cuuint32_t)box_keys};
   encode_tensor_map(m, map_type(dtype), 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Launches behind a kernel of this file that signals its dependents early.
+// The sequences' own K or V: (channel, KV head, key, sequence), 64 channels x 16 keys a copy.
+void encode_suffix(CUtensorMap* m, int dtype, const void* base, int head_size, int kv_heads, int64_t keys,
+                   int64_t sequences, const int64_t* stride) {
+  const cuuint64_t dims[4] = {(cuuint64_t)head_size, (cuuint64_t)kv_heads, (cuuint64_t)keys, (cuuint64_t)sequences};
+  const cuuint64_t strides[3] = {map_stride(kv_heads, stride[2]), map_stride(keys, stride[1]),
+                                 map_stride(sequences, stride[0])};
+  const cuuint32_t box[4] = {64, 1, 16, 1};
+  encode_tensor_map(m, map_type(dtype), 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// Launches, with `after` behind a kernel of this file that signals its dependents early.
 template <typename... P, typename... A>
-void launch_after(void (*kernel)(P...), unsigned grid, unsigned block, cudaStream_t stream, A&&... args) {
+void launch_after(void (*kernel)(P...), unsigned grid, unsigned block, int shared, bool after, cudaStream_t stream,
+                  A&&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = block;
+  cfg.dynamicSmemBytes = shared;
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = after ? 1 : 0;
   FA_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...));
 }
 
@@ -867,8 +960,12 @@ void launch_tc(const TcArgs& t, const TcMaps& maps, int dtype, cudaStream_t stre
 }
 
 void launch_join(const JoinArgs& j, int dtype, cudaStream_t stream) {
-  const unsigned grid = (unsigned)((j.tokens * j.heads + 3) / 4);
-  launch_after(dtype == FA_DTYPE_BF16 ? join_kernel<__nv_bfloat16> : join_kernel<__half>, grid, 128, stream, j);
+  const int w = j.parts > 8 ? kJoinWarps : 1;
+  const unsigned grid = (unsigned)((j.tokens * j.heads * w + kJoinWarps - 1) / kJoinWarps);
+  const bool bf16 = dtype == FA_DTYPE_BF16;
+  launch_after(w > 1 ? (bf16 ? join_kernel<__nv_bfloat16, kJoinWarps> : join_kernel<__half, kJoinWarps>)
+                     : (bf16 ? join_kernel<__nv_bfloat16, 1> : join_kernel<__half, 1>),
+               grid, 32 * kJoinWarps, 0, true, stream, j);
 }
 
 // Query rows as (channel, head of the group, KV head, token).
@@ -956,6 +1053,7 @@ int packed_splits(int64_t total_q, int64_t total_k, int sequences, int heads, in
   return (int)std::max<int64_t>(1, std::min({kSms / ctas, steps / 4, (int64_t)64}));
 }
 
+constexpr int kTcCtas = 74, kRowCtas = 2, kRowMin = 3;
 // How a shared-prefix call is cut.
 struct SharedPlan {
   bool tc = false;      // the prefix on the tensor cores, for all sequences at once
@@ -969,11 +1067,11 @@ SharedPlan shared_plan(int64_t prefix_len, int64_t capacity, int sequences, int 
   p.tc = sequences >= 4 && prefix_len >= 256;
   if (p.tc) {
     const int64_t ctas = ((int64_t)sequences * group + 2 * kRows - 1) / (2 * kRows) * kv_heads;
-    p.tc_splits = (int)std::max<int64_t>(1, std::min<int64_t>(kSms / ctas, (prefix_len + kKeys - 1) / kKeys));
+    p.tc_splits = (int)std::max<int64_t>(1, std::min<int64_t>(kTcCtas / ctas, (prefix_len + kKeys - 1) / kKeys));
   }
   const int64_t ctas = (int64_t)sequences * kv_heads * ((group + kRowHeads - 1) / kRowHeads);
-  const int64_t chunks = ((p.tc ? 0 : prefix_len) + capacity) / kChunk;
-  p.row_splits = (int)std::max<int64_t>(1, std::min<int64_t>(4 * kSms / ctas, chunks / (4 * kRowWarps)));
+  const int64_t stages = ((p.tc ? 0 : prefix_len) + capacity) / kStageKeys;
+  p.row_splits = (int)std::max<int64_t>(1, std::min<int64_t>(kRowCtas * kSms / ctas, stages / kRowMin));
   return p;
 }
 
@@ -996,6 +1094,10 @@ void prepare_dev_attention() {
   auto set = [](auto kernel, int bytes) {
     FA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
   };
+  set(attention_rows_kernel<64, false>, RowsLayout<64>::kTotal);
+  set(attention_rows_kernel<64, true>, RowsLayout<64>::kTotal);
+  set(attention_rows_kernel<128, false>, RowsLayout<128>::kTotal);
+  set(attention_rows_kernel<128, true>, RowsLayout<128>::kTotal);
   set(attention_tc_kernel<64, false>, TcLayout<64>::kTotal);
   set(attention_tc_kernel<64, true>, TcLayout<64>::kTotal);
   set(attention_tc_kernel<128, false>, TcLayout<128>::kTotal);
@@ -1090,20 +1192,6 @@ void launch_attention_shared(const fa_attention_shared_args& a, int* err, cudaSt
   r.q = a.q;
   r.q_seq = a.q_stride[0];
   r.q_head = a.q_stride[1];
-  r.prefix.k = a.prefix_k;
-  r.prefix.v = a.prefix_v;
-  r.prefix.k_row = a.prefix_k_stride[0];
-  r.prefix.v_row = a.prefix_v_stride[0];
-  r.prefix.k_head = a.prefix_k_stride[1];
-  r.prefix.v_head = a.prefix_v_stride[1];
-  r.suffix.k = a.suffix_k;
-  r.suffix.v = a.suffix_v;
-  r.suffix.k_seq = a.suffix_k_stride[0];
-  r.suffix.v_seq = a.suffix_v_stride[0];
-  r.suffix.k_row = a.suffix_k_stride[1];
-  r.suffix.v_row = a.suffix_v_stride[1];
-  r.suffix.k_head = a.suffix_k_stride[2];
-  r.suffix.v_head = a.suffix_v_stride[2];
   r.prefix_len = plan.tc ? 0 : (int)a.prefix_len;
   r.suffix_lens = a.suffix_capacity > 0 ? a.suffix_lens : nullptr;
   r.capacity = (int)a.suffix_capacity;
@@ -1125,16 +1213,21 @@ void launch_attention_shared(const fa_attention_shared_args& a, int* err, cudaSt
     r.part_o = part_o + plan.tc_splits * rows * a.head_size;
     r.part_lse = part_lse + plan.tc_splits * rows;
   }
-  const unsigned grid = (unsigned)((int64_t)a.sequences * a.kv_heads * r.blocks * r.splits);
-  const bool bf16 = a.dtype == FA_DTYPE_BF16;
-  auto kernel = a.head_size <= 64 ? (bf16 ? attention_rows_kernel<64, true> : attention_rows_kernel<64, false>)
-                                  : (bf16 ? attention_rows_kernel<128, true> : attention_rows_kernel<128, false>);
-  if (plan.tc) {
-    launch_after(kernel, grid, 32 * kRowWarps, stream, r);
-  } else {
-    kernel<<<grid, 32 * kRowWarps, 0, stream>>>(r);
-    FA_CUDA(cudaGetLastError());
+  r.err = err;
+  RowsMaps maps;
+  if (r.prefix_len > 0) {
+    encode_kv(&maps.pk, a.dtype, a.prefix_k, a.head_size, a.kv_heads, a.prefix_len, a.prefix_k_stride, kStageKeys);
+    encode_kv(&maps.pv, a.dtype, a.prefix_v, a.head_size, a.kv_heads, a.prefix_len, a.prefix_v_stride, kStageKeys);
   }
+  if (r.suffix_lens) {
+    encode_suffix(&maps.sk, a.dtype, a.suffix_k, a.head_size, a.kv_heads, a.suffix_capacity, a.sequences, a.suffix_k_stride);
+    encode_suffix(&maps.sv, a.dtype, a.suffix_v, a.head_size, a.kv_heads, a.suffix_capacity, a.sequences, a.suffix_v_stride);
+  }
+  const unsigned grid = (unsigned)((int64_t)a.sequences * a.kv_heads * r.blocks * r.splits);
+  const bool bf16 = a.dtype == FA_DTYPE_BF16, small = a.head_size <= 64;
+  launch_after(small ? (bf16 ? attention_rows_kernel<64, true> : attention_rows_kernel<64, false>)
+                     : (bf16 ? attention_rows_kernel<128, true> : attention_rows_kernel<128, false>),
+               grid, kRowThreads, small ? RowsLayout<64>::kTotal : RowsLayout<128>::kTotal, plan.tc, stream, r, maps);
   if (parts) {
     JoinArgs j;
     j.tokens = a.sequences;
