@@ -560,7 +560,7 @@ template <int D>
 struct RowsLayout {
   static constexpr int kHalf = kStageKeys * 128;  // 64 keys x 64 channels, 128-byte swizzle
   static constexpr int kTile = D / 64 * kHalf;
-  static constexpr int kStages = D == 128 ? 3 : 4;
+  static constexpr int kStages = D == 128 ? 2 : 4;
   static constexpr int kBars = kStages * 2 * kTile;
   static constexpr int kMisc = kBars + 8 * 3 * kStages;
   static constexpr int kTotal = kMisc + 16 + 1024;
@@ -608,7 +608,7 @@ __device__ __forceinline__ uint4 lds16(unsigned addr) {
 // global memory into registers needed the L1 for what was in flight: they ran at
 // half the rate on an SM whose memory the tensor-core kernel had claimed.)
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kRowThreads, 2) attention_rows_kernel(const RowsArgs a,
+__global__ void __launch_bounds__(kRowThreads, 3) attention_rows_kernel(const RowsArgs a,
                                                                         const __grid_constant__ RowsMaps maps) {
   using L = RowsLayout<D>;
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
@@ -1045,6 +1045,8 @@ int check_attention_shared(const fa_attention_shared_args* a) {
 
 namespace {
 
+constexpr double kShare = 0.6;
+constexpr int kRowTc = 8, kRowAlone = 2, kRowMin = 4;
 // Key ranges that a packed call is cut into: when its tiles leave SMs idle and
 // the sequences are long enough on average that a part has at least 4 steps.
 int packed_splits(int64_t total_q, int64_t total_k, int sequences, int heads, int kv_heads) {
@@ -1053,7 +1055,6 @@ int packed_splits(int64_t total_q, int64_t total_k, int sequences, int heads, in
   return (int)std::max<int64_t>(1, std::min({kSms / ctas, steps / 4, (int64_t)64}));
 }
 
-constexpr int kTcCtas = 74, kRowCtas = 2, kRowMin = 3;
 // How a shared-prefix call is cut.
 struct SharedPlan {
   bool tc = false;      // the prefix on the tensor cores, for all sequences at once
@@ -1061,17 +1062,24 @@ struct SharedPlan {
   int row_splits = 1;   // key ranges of attention_rows_kernel
   int parts() const { return tc || row_splits > 1 ? tc_splits + row_splits : 0; }
 };
-SharedPlan shared_plan(int64_t prefix_len, int64_t capacity, int sequences, int heads, int kv_heads) {
+SharedPlan shared_plan(int64_t prefix_len, int64_t capacity, int sequences, int heads, int kv_heads, int head_size) {
   SharedPlan p;
   const int group = heads / kv_heads;
   p.tc = sequences >= 4 && prefix_len >= 256;
   if (p.tc) {
+    // The two kernels run side by side, the prefix's bound by its MMAs and the
+    // own keys' by their bytes: as few CTAs for the prefix as let it end about
+    // when those (half of the capacity, at 6.2 TB/s) are through; a key tile
+    // takes about 1.4 us there.
     const int64_t ctas = ((int64_t)sequences * group + 2 * kRows - 1) / (2 * kRows) * kv_heads;
-    p.tc_splits = (int)std::max<int64_t>(1, std::min<int64_t>(kTcCtas / ctas, (prefix_len + kKeys - 1) / kKeys));
+    const int64_t tiles = (prefix_len + kKeys - 1) / kKeys;
+    const double own_us = 2.0 * sequences * capacity * kv_heads * head_size / 6.2e6;
+    const int64_t each = std::max<int64_t>(2, (int64_t)(own_us * kShare));
+    p.tc_splits = (int)std::max<int64_t>(1, std::min<int64_t>(kSms / ctas, (tiles + each - 1) / each));
   }
   const int64_t ctas = (int64_t)sequences * kv_heads * ((group + kRowHeads - 1) / kRowHeads);
   const int64_t stages = ((p.tc ? 0 : prefix_len) + capacity) / kStageKeys;
-  p.row_splits = (int)std::max<int64_t>(1, std::min<int64_t>(kRowCtas * kSms / ctas, stages / kRowMin));
+  p.row_splits = (int)std::max<int64_t>(1, std::min<int64_t>((p.tc ? kRowTc : kRowAlone) * kSms / ctas, stages / kRowMin));
   return p;
 }
 
@@ -1086,7 +1094,7 @@ int64_t attention_packed_workspace(int64_t total_q, int64_t total_k, int sequenc
 int64_t attention_shared_workspace(int64_t prefix_len, int64_t suffix_capacity, int sequences, int heads, int kv_heads,
                                    int head_size) {
   if (sequences <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > 64) return 0;
-  const SharedPlan p = shared_plan(prefix_len, suffix_capacity, sequences, heads, kv_heads);
+  const SharedPlan p = shared_plan(prefix_len, suffix_capacity, sequences, heads, kv_heads, head_size);
   return part_bytes(p.parts(), (int64_t)sequences * heads, head_size);
 }
 
@@ -1160,7 +1168,7 @@ void launch_attention_packed(const fa_attention_packed_args& a, int* err, cudaSt
 
 void launch_attention_shared(const fa_attention_shared_args& a, int* err, cudaStream_t stream) {
   if (a.sequences == 0) return;
-  const SharedPlan plan = shared_plan(a.prefix_len, a.suffix_capacity, a.sequences, a.heads, a.kv_heads);
+  const SharedPlan plan = shared_plan(a.prefix_len, a.suffix_capacity, a.sequences, a.heads, a.kv_heads, a.head_size);
   const int64_t rows = (int64_t)a.sequences * a.heads;
   const int group = a.heads / a.kv_heads, parts = plan.parts();
   float* part_o = parts ? static_cast<float*>(a.workspace) : nullptr;
