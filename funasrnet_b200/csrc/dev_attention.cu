@@ -327,7 +327,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const TcArg
       // Waits, and releases below, also for tiles that only the other issuer uses:
       // one that ran ahead would release a slot's next use.
       wait(&kv_full[vs.st], vs.ph, kAttnWaitLoad);
-      if (n0 + 2 < cnt) wait(&kv_full[ks.st], ks.ph, kAttnWaitLoad);
       if (!ok) break;
       // Value rows behind the last key that a row sees are not the sequence's
       // own, or masked for every row here: 0 x what they hold must stay 0.
@@ -347,8 +346,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const TcArg
         wait(&p_full[2 * w + b], (n0 >> 1) & 1, kAttnWaitSoftmax);
         if (!ok) continue;
         values(b, (min(end[w] - key0 - n * kUnit, kUnit) + 15) / 16, n > 0);
-        if (n + 2 < mine) scores(b);
+        if (b == 0 && n0 + 2 < mine) wait(&kv_full[ks.st], ks.ph, kAttnWaitLoad);
+        if (ok && n + 2 < mine) scores(b);
       }
+      if (ok && n0 + 2 < cnt && n0 + 2 >= mine) wait(&kv_full[ks.st], ks.ph, kAttnWaitLoad);
       if (ok && ptx::elect()) {
         ptx::tc_commit(&kv_empty[vs.st]);
         if (n0 + 2 < cnt) ptx::tc_commit(&kv_empty[ks.st]);
@@ -420,16 +421,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const TcArg
         }
       }
       if (!done) {
-        float mx = -INFINITY;
-#pragma unroll 1
-        for (int k = 0; k < kUnit; k += 32) {
-          unsigned u[32];
-          ptx::tmem_ld32(s_addr + k, u);
-          ptx::tc_wait_ld();
+        // The first step, masked keys, or a maximum that may move: all scores first.
+        unsigned u[64];
+        ptx::tmem_ld32(s_addr, u);
+        ptx::tmem_ld32(s_addr + 32, u + 32);
+        ptx::tc_wait_ld();
+        if (__any_sync(0xffffffffu, lim < kUnit)) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (k + e < lim) mx = fmaxf(mx, __uint_as_float(u[e]));
+          for (int e = 0; e < kUnit; ++e)
+            if (e >= lim) u[e] = 0xff800000u;  // -inf
         }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < kUnit; e += 2)
+          top[(e >> 1) & 3] = ptx::max3(top[(e >> 1) & 3], __uint_as_float(u[e]), __uint_as_float(u[e + 1]));
+        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         if (n == 0) {
           m = mx;
         } else {
@@ -457,21 +463,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const TcArg
         }
         const float base = m == -INFINITY ? 0.0f : m * c;
         float sum[2] = {0.0f, 0.0f};
-#pragma unroll 1
-        for (int k = 0; k < kUnit; k += 32) {
-          unsigned u[32], p[16];
-          ptx::tmem_ld32(s_addr + k, u);
-          ptx::tc_wait_ld();
+        unsigned p[32];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float p0 = k + 2 * e < lim ? ptx::ex2(fmaf(__uint_as_float(u[2 * e]), c, -base)) : 0.0f;
-            const float p1 = k + 2 * e + 1 < lim ? ptx::ex2(fmaf(__uint_as_float(u[2 * e + 1]), c, -base)) : 0.0f;
-            sum[0] += p0;
-            sum[1] += p1;
-            p[e] = ptx::pack16<BF16>(p0, p1);
-          }
-          ptx::tmem_st16(s_addr + k / 2, p);
+        for (int e = 0; e < 32; ++e) {
+          const float p0 = ptx::ex2(fmaf(__uint_as_float(u[2 * e]), c, -base));
+          const float p1 = ptx::ex2(fmaf(__uint_as_float(u[2 * e + 1]), c, -base));
+          sum[0] += p0;
+          sum[1] += p1;
+          p[e] = ptx::pack16<BF16>(p0, p1);
         }
+        ptx::tmem_st32(s_addr, p);
         l += sum[0] + sum[1];
       }
       ptx::tc_wait_st();
