@@ -61,10 +61,6 @@ constexpr int kKeys = 128;     // keys of a K or V tile in shared memory
 constexpr int kUnit = 64;      // keys per softmax step: half a tile
 constexpr float kSlack = 8.0f; // powers of two by which a row's maximum may rise before its sums are rescaled
 
-constexpr unsigned kTmS = 0, kTmO = 256;  // TMEM columns of S and O
-
-constexpr int kTcThreads = 352;  // 8 softmax warps, 2 that issue MMAs, 1 that copies
-
 enum AttnError : int { kAttnWaitLoad = 41, kAttnWaitMma = 42, kAttnWaitSoftmax = 43, kAttnWaitFree = 44 };
 
 struct TcArgs {
@@ -91,20 +87,23 @@ struct TcMaps {
   CUtensorMap v;
 };
 
-template <int D>
+// W tiles of kRows query rows per CTA.
+template <int D, int W>
 struct TcLayout {
-  static constexpr int kHalf = kRows * 128;       // 128 rows x 64 channels, 128-byte swizzle
+  static constexpr int kThreads = W * 160 + 32;     // per tile 4 softmax warps and 1 that issues MMAs; 1 that copies
+  static constexpr int kHalf = kRows * 128;         // 128 rows x 64 channels, 128-byte swizzle
   static constexpr int kHalves = D / 64;
   static constexpr int kTile = kHalves * kHalf;
-  static constexpr int kStages = D == 128 ? 5 : 8;  // K and V tiles in flight
-  static constexpr int kKv = 2 * kTile;
+  static constexpr int kStages = W == 2 ? (D == 128 ? 5 : 8) : (D == 128 ? 2 : 5);  // K and V tiles in flight
+  static constexpr int kKv = W * kTile;
   static constexpr int kBars = kKv + kStages * kTile;
-  // TMEM columns (all 512 are allocated, so they start at 0): tile 0's S buffers
-  // 0 and 64, tile 1's 128 and 192, O0 256, O1 256 + D.
   static constexpr int kNumBars = 2 * kStages + 2 + 4 + 4 + 4 + 2;
   static constexpr int kMisc = kBars + 8 * kNumBars;
   static constexpr int kTotal = kMisc + 16 + 1024;  // 1024: the tiles start on a swizzle atom
-  static_assert(kTotal <= 227 * 1024, "shared memory");
+  // TMEM columns: tile w's S buffers at 128 w and 128 w + 64, its O at kO + w D.
+  static constexpr int kO = W * 128, kColumns = W * 256;
+  static_assert(kO + W * D <= kColumns, "TMEM");
+  static_assert(kTotal <= (W == 2 ? 227 : 113) * 1024, "shared memory of one or two CTAs an SM");
 };
 
 // Tile t of the call -> its sequence.  Sequence b's tiles start at
@@ -125,23 +124,27 @@ __device__ __forceinline__ int tile_sequence(const TcArgs& a, int tile, int span
   return lo;
 }
 
-// One CTA: two tiles of 128 query rows (tokens x the heads that share a KV
-// head) against the keys of their sequence, 64 keys a step:
-//   warp 10  copies Q, then K and V tiles through a ring (TMA);
-//   warps 8 and 9, one per tile: issue S = Q K^T into TMEM and O += P V with P
-//            from TMEM (tcgen05.mma; one thread issues an MMA per ~62 cycles, an
-//            MMA of 64 keys lasts 32 to 48: one issuer for both tiles was the bound);
-//   warps 0-3 and 4-7, one thread per row: running maximum, p = 2^(s - m),
-//            P in 16 bits over S's columns, row sums in 32 bits.
+// One CTA: W tiles of 128 query rows (tokens x the heads that share a KV head)
+// against the keys of their sequence, 64 keys a step:
+//   the last warp copies Q, then K and V tiles through a ring (TMA);
+//   one warp per tile issues S = Q K^T into TMEM and O += P V with P from TMEM
+//     (tcgen05.mma; one thread issues an MMA per ~62 cycles, an MMA of 64 keys
+//     lasts 32 to 48: one issuer for both tiles was the bound);
+//   four warps per tile, one thread per row: running maximum, p = 2^(s - m),
+//     P in 16 bits over S's columns, row sums in 32 bits.
+// W = 2: K and V tiles are read once for 256 rows.  W = 1: two CTAs share an SM,
+// so that one's start and end (its first copies, its last rows' way out) pass
+// while the other computes; for sequences of few steps.
 // TMEM holds two S buffers of 64 keys per tile next to the two O: while a tile's
 // softmax works on one buffer, the tensor core turns the other's P into O and
 // refills it, so neither waits for the other's whole step.  (With one buffer of
 // 128 keys a step was the sum softmax + P V + Q K^T + the hand-offs: 3490 cycles
 // against 2048 of MMA.)  The row maximum that the exponents subtract only moves
 // when it rises by more than 2^kSlack, so O (in TMEM) is rescaled rarely.
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const TcArgs a, const __grid_constant__ TcMaps maps) {
-  using L = TcLayout<D>;
+template <int D, int W, bool BF16>
+__global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
+    attention_tc_kernel(const TcArgs a, const __grid_constant__ TcMaps maps) {
+  using L = TcLayout<D, W>;
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   extern __shared__ uint8_t sm_raw[];
   uint8_t* sm = sm_raw + ((1024 - (ptx::saddr(sm_raw) & 1023)) & 1023);
@@ -161,7 +164,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const TcArg
   const int kvh = blockIdx.x % a.kv_heads;
   const int split = (blockIdx.x / a.kv_heads) % a.splits;
   const int tile = a.tiles - 1 - blockIdx.x / (a.kv_heads * a.splits);  // causal: long tiles first
-  const int span = 2 * a.tokens;
+  const int span = W * a.tokens;
   ptx::griddep_launch();
   int seq = 0, q0 = 0, q_len = (int)a.total_q, k0 = 0, k_len = (int)a.total_k, first = 0;
   if (a.q_off) {
@@ -175,9 +178,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const TcArg
   }
   const int tok0 = (tile - first) * span;  // first token of the pair within the sequence
   if (tok0 < 0 || tok0 >= q_len) return;
-  int end[2];  // keys that some row of the tile sees
+  int end[2] = {0, 0};  // keys that some row of the tile sees
 #pragma unroll
-  for (int w = 0; w < 2; ++w) {
+  for (int w = 0; w < W; ++w) {
     const int t_end = min(tok0 + (w + 1) * a.tokens, q_len);
     const bool any = tok0 + w * a.tokens < q_len;
     end[w] = !any ? 0 : a.causal ? max(0, min(k_len, t_end + k_len - q_len)) : k_len;
@@ -192,7 +195,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const TcArg
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::kStages; ++s) {
       ptx::mbar_init(&kv_full[s], 1);
-      ptx::mbar_init(&kv_empty[s], 2);  // both issuers
+      ptx::mbar_init(&kv_empty[s], W);  // every issuer
     }
     for (int w = 0; w < 2; ++w) {
       ptx::mbar_init(&q_full[w], 1);
@@ -206,16 +209,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const TcArg
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(ptx::saddr(tmem_slot))
+  if (warp == 4 * W) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ptx::saddr(tmem_slot)),
+                 "n"(L::kColumns)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
+  // All 512 columns start at 0; half of them where the SM's other CTA is not.
+  const unsigned tm = W == 2 ? 0 : __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
-  if (warp == 10) {
+  if (warp == 5 * W) {
     // ---- copies: ring number of K tile i: 2i, of V tile i: 2i + 1 ----
     if (lane == 0) {
       int n = 0;  // ring tiles issued
@@ -252,10 +258,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const TcArg
       if (cnt1 > 0) ptx::wait_phase(&q_full[1], 0, abort_flag, a.err, kAttnWaitLoad, false);
     }
     __syncwarp();
-  } else if (warp >= 8) {
+  } else if (warp >= 4 * W) {
     // ---- MMAs of one tile: uniform values, constant offsets and no arithmetic
     // between the MMAs of a step ----
-    const int w = warp - 8, mine = w ? cnt1 : cnt0;
+    const int w = W == 2 ? warp - 8 : 0, mine = w ? cnt1 : cnt0;
     const unsigned id_s = ptx::idesc_f16(BF16, false, kRows, kUnit);
     const int n_o = (a.head_size + 15) / 16 * 16;  // channels past head_size are zeros (TMA fill)
     const unsigned id_o = ptx::idesc_f16(BF16, true, kRows, n_o);
@@ -287,12 +293,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const TcArg
 #pragma unroll
           for (int s = 0; s < D / 16; ++s) {
             const unsigned off = ((s >> 2) * L::kHalf + (s & 3) * 32) >> 4;
-            ptx::tc_mma_ss(kTmS + w * 128 + b * kUnit, q + off, k + off, id_s, s > 0);
+            ptx::tc_mma_ss(tm + w * 128 + b * kUnit, q + off, k + off, id_s, s > 0);
           }
         } else {
           for (int s = 0; s < k_s; ++s) {
             const unsigned off = ((s >> 2) * L::kHalf + (s & 3) * 32) >> 4;
-            ptx::tc_mma_ss(kTmS + w * 128 + b * kUnit, q + off, k + off, id_s, s > 0);
+            ptx::tc_mma_ss(tm + w * 128 + b * kUnit, q + off, k + off, id_s, s > 0);
           }
         }
         ptx::tc_commit(&s_full[2 * w + b]);
@@ -305,10 +311,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const TcArg
         if (steps == kUnit / 16) {
 #pragma unroll
           for (int s = 0; s < kUnit / 16; ++s)
-            ptx::tc_mma_ts(kTmO + w * D, kTmS + w * 128 + b * kUnit + s * 8, v + (s * 2048 >> 4), id_o, acc || s > 0);
+            ptx::tc_mma_ts(tm + L::kO + w * D, tm + w * 128 + b * kUnit + s * 8, v + (s * 2048 >> 4), id_o, acc || s > 0);
         } else {
           for (int s = 0; s < steps; ++s)
-            ptx::tc_mma_ts(kTmO + w * D, kTmS + w * 128 + b * kUnit + s * 8, v + (s * 2048 >> 4), id_o, acc || s > 0);
+            ptx::tc_mma_ts(tm + L::kO + w * D, tm + w * 128 + b * kUnit + s * 8, v + (s * 2048 >> 4), id_o, acc || s > 0);
         }
         ptx::tc_commit(&pv_done[2 * w + b]);
       }
@@ -368,7 +374,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const TcArg
     const int w = warp >> 2;
     const int r = threadIdx.x & 127;
     const unsigned lanes = (unsigned)(32 * (warp & 3)) << 16;
-    const unsigned o_addr = lanes + kTmO + w * D;
+    const unsigned o_addr = tm + lanes + L::kO + w * D;
     const int tok_in = r / a.group, g = r - tok_in * a.group;
     const int tok = tok0 + w * a.tokens + tok_in;
     const bool live = tok_in < a.tokens && tok < q_len;
@@ -382,7 +388,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const TcArg
                       ptx::wait_phase(&s_full[2 * w + (n & 1)], (n >> 1) & 1, abort_flag, a.err, kAttnWaitMma));
       if (!ok) break;
       ptx::tc_fence_after();
-      const unsigned s_addr = lanes + kTmS + w * 128 + (n & 1) * kUnit;
+      const unsigned s_addr = tm + lanes + w * 128 + (n & 1) * kUnit;
       const int lim = sees - key0 - n * kUnit;  // keys of this step that the row sees
       bool done = false;
       if (n > 0 && __all_sync(0xffffffffu, lim >= kUnit)) {
@@ -521,9 +527,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const TcArg
   }
   ptx::tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 4 * W) {
     ptx::tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(*tmem_slot) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "n"(L::kColumns) : "memory");
   }
 }
 
@@ -946,18 +952,23 @@ void launch_after(void (*kernel)(P...), unsigned grid, unsigned block, int share
   FA_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...));
 }
 
-template <int D, bool BF16>
+template <int D, int W, bool BF16>
 void launch_tc_as(const TcArgs& t, const TcMaps& maps, cudaStream_t stream) {
+  using L = TcLayout<D, W>;
   const unsigned grid = (unsigned)t.tiles * t.kv_heads * t.splits;
-  attention_tc_kernel<D, BF16><<<grid, kTcThreads, TcLayout<D>::kTotal, stream>>>(t, maps);
+  attention_tc_kernel<D, W, BF16><<<grid, L::kThreads, L::kTotal, stream>>>(t, maps);
   FA_CUDA(cudaGetLastError());
 }
-void launch_tc(const TcArgs& t, const TcMaps& maps, int dtype, cudaStream_t stream) {
-  const bool bf16 = dtype == FA_DTYPE_BF16;
+template <int D, int W>
+void launch_tc_of(const TcArgs& t, const TcMaps& maps, int dtype, cudaStream_t stream) {
+  dtype == FA_DTYPE_BF16 ? launch_tc_as<D, W, true>(t, maps, stream) : launch_tc_as<D, W, false>(t, maps, stream);
+}
+// W: tiles of a CTA, for which t.tiles was counted.
+void launch_tc(const TcArgs& t, const TcMaps& maps, int w, int dtype, cudaStream_t stream) {
   if (t.head_size <= 64)
-    bf16 ? launch_tc_as<64, true>(t, maps, stream) : launch_tc_as<64, false>(t, maps, stream);
+    w == 2 ? launch_tc_of<64, 2>(t, maps, dtype, stream) : launch_tc_of<64, 1>(t, maps, dtype, stream);
   else
-    bf16 ? launch_tc_as<128, true>(t, maps, stream) : launch_tc_as<128, false>(t, maps, stream);
+    w == 2 ? launch_tc_of<128, 2>(t, maps, dtype, stream) : launch_tc_of<128, 1>(t, maps, dtype, stream);
 }
 
 void launch_join(const JoinArgs& j, int dtype, cudaStream_t stream) {
@@ -980,12 +991,16 @@ void encode_q(CUtensorMap* m, int dtype, const void* base, int head_size, int gr
 }
 
 constexpr int kSms = 148;
+constexpr double kShort = 8.0;   // key tiles up to which a CTA takes one tile of rows
+constexpr double kStepUs = 1.8;  // one key tile against two tiles of rows
 
 // Bytes of `parts` partial results of `rows` rows.
 int64_t part_bytes(int64_t parts, int64_t rows, int head_size) { return parts * rows * (head_size + 4) * 4; }
 
-// Tile pairs of a packed call, an upper bound (tile_sequence).
-int64_t tile_pairs(int64_t total_q, int sequences, int group) { return total_q / (2 * (kRows / group)) + sequences; }
+// CTAs per KV head of a packed call with w tiles each, an upper bound (tile_sequence).
+int64_t packed_tiles(int64_t total_q, int sequences, int group, int w) {
+  return total_q / (w * (kRows / group)) + sequences;
+}
 
 }  // namespace
 
@@ -1046,14 +1061,33 @@ int check_attention_shared(const fa_attention_shared_args* a) {
 
 namespace {
 
-constexpr double kShare = 0.6;
-constexpr int kRowTc = 8, kRowAlone = 2, kRowMin = 4;
-// Key ranges that a packed call is cut into: when its tiles leave SMs idle and
-// the sequences are long enough on average that a part has at least 4 steps.
-int packed_splits(int64_t total_q, int64_t total_k, int sequences, int heads, int kv_heads) {
-  const int64_t ctas = std::max<int64_t>(1, tile_pairs(total_q, sequences, heads / kv_heads) * kv_heads);
-  const int64_t steps = sequences > 0 ? total_k / sequences / kKeys : 0;
-  return (int)std::max<int64_t>(1, std::min({kSms / ctas, steps / 4, (int64_t)64}));
+// How a packed call is cut: tiles per CTA and key ranges.
+struct PackedPlan {
+  int w = 2, splits = 1;
+};
+PackedPlan packed_plan(int64_t total_q, int64_t total_k, int sequences, int heads, int kv_heads, int head_size) {
+  PackedPlan p;
+  const double steps = (double)total_k / sequences / kKeys;  // key tiles of a sequence, on average
+  p.w = steps <= kShort ? 1 : 2;
+  const double ctas = (double)packed_tiles(total_q, sequences, heads / kv_heads, p.w) * kv_heads;
+  // The longest sequence is taken for 1.5 times the average: its CTAs' steps, or
+  // all steps spread over the SMs, at kStepUs each; cutting the keys costs a
+  // second kernel and the parts' bytes, written and read.
+  auto cost = [&](int s) {
+    const double longest = std::max(1.0, (sequences > 1 ? 1.5 : 1.0) * steps / s);
+    const double each = p.w == 2 ? kStepUs : 0.7 * kStepUs, sms = p.w == 2 ? kSms : 2 * kSms;
+    const double parts = s > 1 ? 4.0 + 2.0 * s * total_q * heads * (head_size + 1) * 4 / 4e6 : 0.0;
+    return std::max(longest, ctas * steps / sms) * each + ctas * s / sms * 1.5 + parts;
+  };
+  double best = cost(1);
+  for (int s = 2; s <= 64 && s * 4 <= steps; s += s < 8 ? 1 : s / 4) {
+    const double c = cost(s);
+    if (c < best) {
+      best = c;
+      p.splits = s;
+    }
+  }
+  return p;
 }
 
 // How a shared-prefix call is cut.
@@ -1075,12 +1109,12 @@ SharedPlan shared_plan(int64_t prefix_len, int64_t capacity, int sequences, int 
     const int64_t ctas = ((int64_t)sequences * group + 2 * kRows - 1) / (2 * kRows) * kv_heads;
     const int64_t tiles = (prefix_len + kKeys - 1) / kKeys;
     const double own_us = 2.0 * sequences * capacity * kv_heads * head_size / 6.2e6;
-    const int64_t each = std::max<int64_t>(2, (int64_t)(own_us * kShare));
+    const int64_t each = std::max<int64_t>(2, (int64_t)(own_us * 0.6));
     p.tc_splits = (int)std::max<int64_t>(1, std::min<int64_t>(kSms / ctas, (tiles + each - 1) / each));
   }
   const int64_t ctas = (int64_t)sequences * kv_heads * ((group + kRowHeads - 1) / kRowHeads);
   const int64_t stages = ((p.tc ? 0 : prefix_len) + capacity) / kStageKeys;
-  p.row_splits = (int)std::max<int64_t>(1, std::min<int64_t>((p.tc ? kRowTc : kRowAlone) * kSms / ctas, stages / kRowMin));
+  p.row_splits = (int)std::max<int64_t>(1, std::min<int64_t>((p.tc ? 8 : 2) * kSms / ctas, stages / 4));
   return p;
 }
 
@@ -1089,7 +1123,7 @@ SharedPlan shared_plan(int64_t prefix_len, int64_t capacity, int sequences, int 
 int64_t attention_packed_workspace(int64_t total_q, int64_t total_k, int sequences, int heads, int kv_heads,
                                    int head_size) {
   if (total_q <= 0 || sequences <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > 64) return 0;
-  const int splits = packed_splits(total_q, total_k, sequences, heads, kv_heads);
+  const int splits = packed_plan(total_q, total_k, sequences, heads, kv_heads, head_size).splits;
   return splits > 1 ? part_bytes(splits, total_q * heads, head_size) : 0;
 }
 int64_t attention_shared_workspace(int64_t prefix_len, int64_t suffix_capacity, int sequences, int heads, int kv_heads,
@@ -1107,10 +1141,14 @@ void prepare_dev_attention() {
   set(attention_rows_kernel<64, true>, RowsLayout<64>::kTotal);
   set(attention_rows_kernel<128, false>, RowsLayout<128>::kTotal);
   set(attention_rows_kernel<128, true>, RowsLayout<128>::kTotal);
-  set(attention_tc_kernel<64, false>, TcLayout<64>::kTotal);
-  set(attention_tc_kernel<64, true>, TcLayout<64>::kTotal);
-  set(attention_tc_kernel<128, false>, TcLayout<128>::kTotal);
-  set(attention_tc_kernel<128, true>, TcLayout<128>::kTotal);
+  set(attention_tc_kernel<64, 1, false>, TcLayout<64, 1>::kTotal);
+  set(attention_tc_kernel<64, 1, true>, TcLayout<64, 1>::kTotal);
+  set(attention_tc_kernel<64, 2, false>, TcLayout<64, 2>::kTotal);
+  set(attention_tc_kernel<64, 2, true>, TcLayout<64, 2>::kTotal);
+  set(attention_tc_kernel<128, 1, false>, TcLayout<128, 1>::kTotal);
+  set(attention_tc_kernel<128, 1, true>, TcLayout<128, 1>::kTotal);
+  set(attention_tc_kernel<128, 2, false>, TcLayout<128, 2>::kTotal);
+  set(attention_tc_kernel<128, 2, true>, TcLayout<128, 2>::kTotal);
 }
 
 void launch_attention_packed(const fa_attention_packed_args& a, int* err, cudaStream_t stream) {
@@ -1126,8 +1164,9 @@ void launch_attention_packed(const fa_attention_packed_args& a, int* err, cudaSt
   t.group = a.heads / a.kv_heads;
   t.head_size = a.head_size;
   t.tokens = kRows / t.group;
-  t.tiles = (int)tile_pairs(a.total_q, a.sequences, t.group);
-  t.splits = packed_splits(a.total_q, a.total_k, a.sequences, a.heads, a.kv_heads);
+  const PackedPlan plan = packed_plan(a.total_q, a.total_k, a.sequences, a.heads, a.kv_heads, a.head_size);
+  t.tiles = (int)packed_tiles(a.total_q, a.sequences, t.group, plan.w);
+  t.splits = plan.splits;
   t.causal = a.causal;
   t.scale = a.scale;
   t.scale_log2 = (float)(a.scale * 1.4426950408889634);
@@ -1148,7 +1187,7 @@ void launch_attention_packed(const fa_attention_packed_args& a, int* err, cudaSt
   } else {
     maps.k = maps.v = maps.q;  // never used: no sequence has a key
   }
-  launch_tc(t, maps, a.dtype, stream);
+  launch_tc(t, maps, plan.w, a.dtype, stream);
   if (t.splits > 1) {
     JoinArgs j;
     j.q_off = a.q_offsets;
@@ -1195,7 +1234,7 @@ void launch_attention_shared(const fa_attention_shared_args& a, int* err, cudaSt
     encode_q(&maps.q, a.dtype, a.q, a.head_size, group, a.kv_heads, a.sequences, a.q_stride, t.tokens);
     encode_kv(&maps.k, a.dtype, a.prefix_k, a.head_size, a.kv_heads, a.prefix_len, a.prefix_k_stride);
     encode_kv(&maps.v, a.dtype, a.prefix_v, a.head_size, a.kv_heads, a.prefix_len, a.prefix_v_stride);
-    launch_tc(t, maps, a.dtype, stream);
+    launch_tc(t, maps, 2, a.dtype, stream);
   }
   RowsArgs r;
   r.q = a.q;
