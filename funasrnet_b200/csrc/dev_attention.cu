@@ -91,15 +91,17 @@ struct TcMaps {
 template <int D, int W>
 struct TcLayout {
   static constexpr int kThreads = W * 160 + 32;     // per tile 4 softmax warps and 1 that issues MMAs; 1 that copies
-  static constexpr int kHalf = kRows * 128;         // 128 rows x 64 channels, 128-byte swizzle
-  static constexpr int kHalves = D / 64;
-  static constexpr int kTile = kHalves * kHalf;
-  static constexpr int kStages = W == 2 ? (D == 128 ? 5 : 8) : (D == 128 ? 2 : 5);  // K and V tiles in flight
-  static constexpr int kKv = W * kTile;
+  // A tile of Q: 128 rows in halves of 64 channels with 128-byte swizzle; of K
+  // and V: kTileKeys rows alike.
+  static constexpr int kHalves = D / 64, kQHalf = kRows * 128, kQ = kHalves * kQHalf;
+  static constexpr int kTileKeys = W == 2 ? 128 : kUnit;
+  static constexpr int kHalf = kTileKeys * 128, kTile = kHalves * kHalf;
+  static constexpr int kStages = W == 2 ? (D == 128 ? 5 : 8) : (D == 128 ? 5 : 8);  // K and V tiles in flight
+  static constexpr int kKv = W * kQ;
   static constexpr int kBars = kKv + kStages * kTile;
   static constexpr int kNumBars = 2 * kStages + 2 + 4 + 4 + 4 + 2;
   static constexpr int kMisc = kBars + 8 * kNumBars;
-  static constexpr int kTotal = kMisc + 16 + 1024;  // 1024: the tiles start on a swizzle atom
+  static constexpr int kTotal = kMisc + 16;
   // TMEM columns: tile w's S buffers at 128 w and 128 w + 64, its O at kO + w D.
   static constexpr int kO = W * 128, kColumns = W * 256;
   static_assert(kO + W * D <= kColumns, "TMEM");
@@ -146,8 +148,7 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
     attention_tc_kernel(const TcArgs a, const __grid_constant__ TcMaps maps) {
   using L = TcLayout<D, W>;
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-  extern __shared__ uint8_t sm_raw[];
-  uint8_t* sm = sm_raw + ((1024 - (ptx::saddr(sm_raw) & 1023)) & 1023);
+  extern __shared__ __align__(1024) uint8_t sm[];  // the tiles start on a swizzle atom
   const unsigned sbase = ptx::saddr(sm);
   uint64_t* kv_full = reinterpret_cast<uint64_t*>(sm + L::kBars);
   uint64_t* kv_empty = kv_full + L::kStages;
@@ -190,9 +191,19 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
   const int key0 = ja * kKeys;  // this split's first key
   const int cnt0 = max(0, (min(jb * kKeys, end[0]) - key0 + kUnit - 1) / kUnit);  // steps of the tiles
   const int cnt1 = max(0, (min(jb * kKeys, end[1]) - key0 + kUnit - 1) / kUnit);
-  const int cnt = max(cnt0, cnt1), kv_tiles = (cnt + 1) / 2;
+  const int cnt = max(cnt0, cnt1), ring = 2 * ((cnt * kUnit + L::kTileKeys - 1) / L::kTileKeys);  // copies of K and V
 
-  if (threadIdx.x == 0) {
+  // Ring number of K tile i: 2i, of V tile i: 2i + 1.
+  auto load_kv = [&](int n) {
+    const int st = n % L::kStages;
+    ptx::mbar_expect_tx(&kv_full[st], L::kTile);
+    for (int h = 0; h < L::kHalves; ++h)
+      ptx::tma_load_3d(sbase + L::kKv + st * L::kTile + h * L::kHalf, n & 1 ? &maps.v : &maps.k, h * 64, kvh,
+                       k0 + key0 + (n >> 1) * L::kTileKeys, &kv_full[st]);
+  };
+  // The first copies go out before the CTA meets, under the allocation of TMEM.
+  const int early = min(ring, L::kStages);
+  if (warp == 5 * W && lane == 0) {
     for (int s = 0; s < L::kStages; ++s) {
       ptx::mbar_init(&kv_full[s], 1);
       ptx::mbar_init(&kv_empty[s], W);  // every issuer
@@ -208,6 +219,15 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (early > 0) load_kv(0);
+    for (int w = 0; w < W; ++w)
+      if ((w == 0 ? cnt0 : cnt1) > 0) {
+        ptx::mbar_expect_tx(&q_full[w], (unsigned)(a.tokens * a.group * 128 * L::kHalves));
+        for (int h = 0; h < L::kHalves; ++h)
+          ptx::tma_load_4d(sbase + w * L::kQ + h * L::kQHalf, &maps.q, h * 64, 0, kvh, q0 + tok0 + w * a.tokens,
+                           &q_full[w]);
+      }
+    for (int n = 1; n < early; ++n) load_kv(n);
   }
   if (warp == 4 * W) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ptx::saddr(tmem_slot)),
@@ -222,34 +242,12 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
   const unsigned tm = W == 2 ? 0 : __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   if (warp == 5 * W) {
-    // ---- copies: ring number of K tile i: 2i, of V tile i: 2i + 1 ----
+    // ---- the other copies ----
     if (lane == 0) {
-      int n = 0;  // ring tiles issued
-      bool ok = true;
-      auto load_kv = [&](const CUtensorMap* map, int i) {
-        const int st = n % L::kStages;
-        if (n >= L::kStages)
-          ok = ok && ptx::wait_phase(&kv_empty[st], (n / L::kStages - 1) & 1, abort_flag, a.err, kAttnWaitFree);
-        if (!ok) return;
-        ptx::mbar_expect_tx(&kv_full[st], L::kTile);
-        for (int h = 0; h < L::kHalves; ++h)
-          ptx::tma_load_3d(sbase + L::kKv + st * L::kTile + h * L::kHalf, map, h * 64, kvh, k0 + key0 + i * kKeys,
-                           &kv_full[st]);
-        ++n;
-      };
-      auto load_q = [&](int w) {
-        if ((w == 0 ? cnt0 : cnt1) == 0) return;
-        ptx::mbar_expect_tx(&q_full[w], (unsigned)(a.tokens * a.group * 128 * L::kHalves));
-        for (int h = 0; h < L::kHalves; ++h)
-          ptx::tma_load_4d(sbase + w * L::kTile + h * L::kHalf, &maps.q, h * 64, 0, kvh, q0 + tok0 + w * a.tokens,
-                           &q_full[w]);
-      };
-      load_q(0);
-      if (cnt > 0) load_kv(&maps.k, 0);
-      load_q(1);
-      for (int i = 0; i < kv_tiles && ok; ++i) {
-        load_kv(&maps.v, i);
-        if (i + 1 < kv_tiles && ok) load_kv(&maps.k, i + 1);
+      int n = early;
+      for (; n < ring; ++n) {
+        if (!ptx::wait_phase(&kv_empty[n % L::kStages], (n / L::kStages - 1) & 1, abort_flag, a.err, kAttnWaitFree)) break;
+        load_kv(n);
       }
       // Copies in flight land before the CTA exits.
       for (int s = max(0, n - L::kStages); s < n; ++s)
@@ -285,28 +283,29 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
       }
     };
     Slot ks{0, 0}, vs{1, 0};
-    auto scores = [&](int b) {  // S_w of the K tile's half b into buffer b
-      const unsigned q = q_low + w * (L::kTile >> 4);
-      const unsigned k = k_low + ks.st * (L::kTile >> 4) + b * (kUnit * 128 >> 4);
+    constexpr int kPart = W == 2 ? kUnit * 128 : 0;  // bytes between the steps of a tile
+    auto scores = [&](int b) {  // S_w of the K tile (W = 2: of its half b) into buffer b
+      const unsigned q = q_low + w * (L::kQ >> 4);
+      const unsigned k = k_low + ks.st * (L::kTile >> 4) + b * (kPart >> 4);
       if (ptx::elect()) {
         if (k_s == D / 16) {
 #pragma unroll
           for (int s = 0; s < D / 16; ++s) {
-            const unsigned off = ((s >> 2) * L::kHalf + (s & 3) * 32) >> 4;
-            ptx::tc_mma_ss(tm + w * 128 + b * kUnit, q + off, k + off, id_s, s > 0);
+            ptx::tc_mma_ss(tm + w * 128 + b * kUnit, q + (((s >> 2) * L::kQHalf + (s & 3) * 32) >> 4),
+                           k + (((s >> 2) * L::kHalf + (s & 3) * 32) >> 4), id_s, s > 0);
           }
         } else {
           for (int s = 0; s < k_s; ++s) {
-            const unsigned off = ((s >> 2) * L::kHalf + (s & 3) * 32) >> 4;
-            ptx::tc_mma_ss(tm + w * 128 + b * kUnit, q + off, k + off, id_s, s > 0);
+            ptx::tc_mma_ss(tm + w * 128 + b * kUnit, q + (((s >> 2) * L::kQHalf + (s & 3) * 32) >> 4),
+                           k + (((s >> 2) * L::kHalf + (s & 3) * 32) >> 4), id_s, s > 0);
           }
         }
         ptx::tc_commit(&s_full[2 * w + b]);
       }
       __syncwarp();
     };
-    auto values = [&](int b, int steps, bool acc) {  // O_w += P_w (buffer b) x the V tile's half b
-      const unsigned v = v_low + vs.st * (L::kTile >> 4) + b * (kUnit * 128 >> 4);
+    auto values = [&](int b, int steps, bool acc) {  // O_w += P_w (buffer b) x the V tile (its half b)
+      const unsigned v = v_low + vs.st * (L::kTile >> 4) + b * (kPart >> 4);
       if (ptx::elect()) {
         if (steps == kUnit / 16) {
 #pragma unroll
@@ -320,49 +319,79 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
       }
       __syncwarp();
     };
+    auto release = [&](int st) {
+      if (ok && ptx::elect()) ptx::tc_commit(&kv_empty[st]);
+      __syncwarp();
+    };
+    // Value rows behind the last key that a row sees are not the sequence's own,
+    // or masked for every row here: 0 x what they hold must stay 0.
+    auto clear_tail = [&](int key) {
+      const int most = min(max(end[0], end[1]) - key0 - key, L::kTileKeys), padded = (most + 15) / 16 * 16;
+      if (most >= padded) return;
+      uint8_t* v = sm + L::kKv + vs.st * L::kTile;
+      for (int c = lane; c < (padded - most) * 8; c += 32)
+        for (int h = 0; h < L::kHalves; ++h)
+          *reinterpret_cast<uint4*>(v + h * L::kHalf + (most + c / 8) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+    };
+    auto steps_of = [&](int n) { return (min(end[w] - key0 - n * kUnit, kUnit) + 15) / 16; };
     if (cnt > 0) wait(&kv_full[0], 0, kAttnWaitLoad);
-    if (mine > 0) {
-      wait(&q_full[w], 0, kAttnWaitLoad);
-      if (ok) scores(0);
-      if (ok && mine > 1) scores(1);
-    }
-    if (ok && cnt > 0 && ptx::elect()) ptx::tc_commit(&kv_empty[0]);
-    __syncwarp();
-    ks.next();
-    for (int n0 = 0; n0 < cnt && ok; n0 += 2) {  // one V tile, and the K tile after its own
-      // Waits, and releases below, also for tiles that only the other issuer uses:
-      // one that ran ahead would release a slot's next use.
-      wait(&kv_full[vs.st], vs.ph, kAttnWaitLoad);
-      if (!ok) break;
-      // Value rows behind the last key that a row sees are not the sequence's
-      // own, or masked for every row here: 0 x what they hold must stay 0.
-      const int most = min(max(end[0], end[1]) - key0 - n0 * kUnit, kKeys), padded = (most + 15) / 16 * 16;
-      if (n0 < mine && most < padded) {
-        uint8_t* v = sm + L::kKv + vs.st * L::kTile;
-        for (int c = lane; c < (padded - most) * 8; c += 32)
-          for (int h = 0; h < L::kHalves; ++h)
-            *reinterpret_cast<uint4*>(v + h * L::kHalf + (most + c / 8) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-      }
+    if (mine > 0) wait(&q_full[w], 0, kAttnWaitLoad);
+    if (W == 1) {  // a tile a step
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const int n = n0 + b;
-        if (!ok || n >= mine) continue;
-        wait(&p_full[2 * w + b], (n0 >> 1) & 1, kAttnWaitSoftmax);
-        if (!ok) continue;
-        values(b, (min(end[w] - key0 - n * kUnit, kUnit) + 15) / 16, n > 0);
-        if (b == 0 && n0 + 2 < mine) wait(&kv_full[ks.st], ks.ph, kAttnWaitLoad);
-        if (ok && n + 2 < mine) scores(b);
+        if (!ok || b >= mine) continue;
+        if (b == 1) wait(&kv_full[ks.st], ks.ph, kAttnWaitLoad);
+        if (ok) scores(b);
+        release(ks.st);
+        ks.next();
       }
-      if (ok && n0 + 2 < cnt && n0 + 2 >= mine) wait(&kv_full[ks.st], ks.ph, kAttnWaitLoad);
-      if (ok && ptx::elect()) {
-        ptx::tc_commit(&kv_empty[vs.st]);
-        if (n0 + 2 < cnt) ptx::tc_commit(&kv_empty[ks.st]);
-      }
-      __syncwarp();
-      vs.next();
+      for (int n0 = 0; n0 < mine && ok; n0 += 2)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int n = n0 + b;
+          if (!ok || n >= mine) continue;
+          wait(&kv_full[vs.st], vs.ph, kAttnWaitLoad);
+          if (ok) clear_tail(n * kUnit);
+          wait(&p_full[b], (n0 >> 1) & 1, kAttnWaitSoftmax);
+          if (!ok) continue;
+          values(b, steps_of(n), n > 0);
+          release(vs.st);
+          vs.next();
+          if (n + 2 >= mine) continue;
+          wait(&kv_full[ks.st], ks.ph, kAttnWaitLoad);
+          if (ok) scores(b);
+          release(ks.st);
+          ks.next();
+        }
+    } else {
+      if (ok && mine > 0) scores(0);
+      if (ok && mine > 1) scores(1);
+      if (cnt > 0) release(0);
       ks.next();
+      for (int n0 = 0; n0 < cnt && ok; n0 += 2) {  // one V tile, and the K tile after its own
+        // Waits, and releases below, also for tiles that only the other issuer uses:
+        // one that ran ahead would release a slot's next use.
+        wait(&kv_full[vs.st], vs.ph, kAttnWaitLoad);
+        if (!ok) break;
+        if (n0 < mine) clear_tail(n0 * kUnit);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int n = n0 + b;
+          if (!ok || n >= mine) continue;
+          wait(&p_full[2 * w + b], (n0 >> 1) & 1, kAttnWaitSoftmax);
+          if (!ok) continue;
+          values(b, steps_of(n), n > 0);
+          if (b == 0 && n0 + 2 < mine) wait(&kv_full[ks.st], ks.ph, kAttnWaitLoad);
+          if (ok && n + 2 < mine) scores(b);
+        }
+        if (ok && n0 + 2 < cnt && n0 + 2 >= mine) wait(&kv_full[ks.st], ks.ph, kAttnWaitLoad);
+        release(vs.st);
+        if (n0 + 2 < cnt) release(ks.st);
+        vs.next();
+        ks.next();
+      }
     }
     if (!ok && ptx::elect()) {  // MMAs in flight finish before their memory is freed
       ptx::tc_commit(&drained[w]);
@@ -495,30 +524,60 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
       const long long t = q0 + tok;
       const int h = kvh * a.group + g;
       const long long row = t * a.heads + h;
-      T* out = static_cast<T*>(a.out) + t * a.out_token + h * a.out_head;
-      float* part = a.part_o + (split * a.total_q * a.heads + row) * a.head_size;
+      const bool parts = a.part_o != nullptr;
+      // The rows leave through this warp's share of Q's place, 16 bytes a lane and
+      // whole rows at a time (a lane that stores its own row alone touches 32
+      // lines an instruction: 2000 cycles for a tile, now under 700).
+      constexpr int kRowBytes = L::kQ / kRows, kChunks = kRowBytes / 16;
+      const unsigned stage = sbase + w * L::kQ + (warp & 3) * 32 * kRowBytes;
+      const unsigned long long to =
+          parts ? reinterpret_cast<unsigned long long>(a.part_o + (split * a.total_q * a.heads + row) * a.head_size)
+                : reinterpret_cast<unsigned long long>(static_cast<T*>(a.out) + t * a.out_token + h * a.out_head);
+      const unsigned lives = __ballot_sync(0xffffffffu, live);
+      auto put = [&](int chunk, unsigned x, unsigned y, unsigned z, unsigned u) {
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * kRowBytes + ((chunk ^ (lane & 7)) << 4)),
+                     "r"(x), "r"(y), "r"(z), "r"(u)
+                     : "memory");
+      };
+      const int width = parts ? D / 2 : D;  // channels of a pass: as many as fill a row of the stage
 #pragma unroll 1
-      for (int k = 0; k < a.head_size; k += 32) {
-        unsigned o[32];
-        if (mine > 0) {
-          ptx::tmem_ld32(o_addr + k, o);
-          ptx::tc_wait_ld();
-        }
-        float v[32];
+      for (int from = 0; from < a.head_size; from += width) {
+#pragma unroll 1
+        for (int k = 0; k < width; k += 32) {
+          unsigned o[32];
+          if (mine > 0) {
+            ptx::tmem_ld32(o_addr + from + k, o);
+            ptx::tc_wait_ld();
+          }
+          float v[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = l == 0.0f ? 0.0f : __uint_as_float(o[e]) * inv;
+          for (int e = 0; e < 32; ++e) v[e] = l == 0.0f ? 0.0f : __uint_as_float(o[e]) * inv;
+          if (parts) {
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          if (!live || k + e >= a.head_size) continue;
-          if (a.part_o) {
-            *reinterpret_cast<float4*>(part + k + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-            *reinterpret_cast<float4*>(part + k + e + 4) = make_float4(v[e + 4], v[e + 5], v[e + 6], v[e + 7]);
+            for (int e = 0; e < 32; e += 4)
+              put((k + e) / 4, __float_as_uint(v[e]), __float_as_uint(v[e + 1]), __float_as_uint(v[e + 2]),
+                  __float_as_uint(v[e + 3]));
           } else {
-            *reinterpret_cast<uint4*>(out + k + e) =
-                make_uint4(ptx::pack16<BF16>(v[e], v[e + 1]), ptx::pack16<BF16>(v[e + 2], v[e + 3]),
-                           ptx::pack16<BF16>(v[e + 4], v[e + 5]), ptx::pack16<BF16>(v[e + 6], v[e + 7]));
+#pragma unroll
+            for (int e = 0; e < 32; e += 8)
+              put((k + e) / 8, ptx::pack16<BF16>(v[e], v[e + 1]), ptx::pack16<BF16>(v[e + 2], v[e + 3]),
+                  ptx::pack16<BF16>(v[e + 4], v[e + 5]), ptx::pack16<BF16>(v[e + 6], v[e + 7]));
           }
         }
+        __syncwarp();
+        const int chunk = lane % kChunks, channel = from + chunk * (parts ? 4 : 8);
+#pragma unroll 4
+        for (int i = 0; i < 32; i += 32 / kChunks) {
+          const int r2 = i + lane / kChunks;
+          const unsigned long long dst = __shfl_sync(0xffffffffu, to, r2);
+          uint4 v;
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                       : "r"(stage + r2 * kRowBytes + ((chunk ^ (r2 & 7)) << 4)));
+          if (((lives >> r2) & 1u) && channel < a.head_size)
+            *reinterpret_cast<uint4*>(dst + (unsigned long long)channel * (parts ? 4 : 2)) = v;
+        }
+        __syncwarp();
       }
       const float lse = (m == -INFINITY ? 0.0f : m * a.scale) + logf(l);
       if (live && a.part_o) a.part_lse[split * a.total_q * a.heads + row] = lse;
@@ -918,7 +977,7 @@ CUtensorMapDataType map_type(int dtype) {
 
 // K or V: (channel, KV head, key), 64 channels x 128 keys a copy.
 void encode_kv(CUtensorMap* m, int dtype, const void* base, int head_size, int kv_heads, int64_t keys,
-               const int64_t* stride, int box_keys = kKeys) {
+               const int64_t* stride, int box_keys) {
   const cuuint64_t dims[3] = {(cuuint64_t)head_size, (cuuint64_t)kv_heads, (cuuint64_t)keys};
   const cuuint64_t strides[2] = {map_stride(kv_heads, stride[1]), map_stride(keys, stride[0])};
   const cuuint32_t box[3] = {64, 1, (cuuint32_t)box_keys};
@@ -1182,8 +1241,9 @@ void launch_attention_packed(const fa_attention_packed_args& a, int* err, cudaSt
   TcMaps maps;
   encode_q(&maps.q, a.dtype, a.q, a.head_size, t.group, a.kv_heads, a.total_q, a.q_stride, t.tokens);
   if (a.total_k > 0) {
-    encode_kv(&maps.k, a.dtype, a.k, a.head_size, a.kv_heads, a.total_k, a.k_stride);
-    encode_kv(&maps.v, a.dtype, a.v, a.head_size, a.kv_heads, a.total_k, a.v_stride);
+    const int keys = plan.w == 2 ? TcLayout<128, 2>::kTileKeys : TcLayout<128, 1>::kTileKeys;
+    encode_kv(&maps.k, a.dtype, a.k, a.head_size, a.kv_heads, a.total_k, a.k_stride, keys);
+    encode_kv(&maps.v, a.dtype, a.v, a.head_size, a.kv_heads, a.total_k, a.v_stride, keys);
   } else {
     maps.k = maps.v = maps.q;  // never used: no sequence has a key
   }
@@ -1232,8 +1292,8 @@ void launch_attention_shared(const fa_attention_shared_args& a, int* err, cudaSt
     t.err = err;
     TcMaps maps;
     encode_q(&maps.q, a.dtype, a.q, a.head_size, group, a.kv_heads, a.sequences, a.q_stride, t.tokens);
-    encode_kv(&maps.k, a.dtype, a.prefix_k, a.head_size, a.kv_heads, a.prefix_len, a.prefix_k_stride);
-    encode_kv(&maps.v, a.dtype, a.prefix_v, a.head_size, a.kv_heads, a.prefix_len, a.prefix_v_stride);
+    encode_kv(&maps.k, a.dtype, a.prefix_k, a.head_size, a.kv_heads, a.prefix_len, a.prefix_k_stride, kKeys);
+    encode_kv(&maps.v, a.dtype, a.prefix_v, a.head_size, a.kv_heads, a.prefix_len, a.prefix_v_stride, kKeys);
     launch_tc(t, maps, 2, a.dtype, stream);
   }
   RowsArgs r;
