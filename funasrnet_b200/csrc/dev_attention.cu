@@ -162,9 +162,13 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   // ---- which rows and keys ----
-  const int kvh = blockIdx.x % a.kv_heads;
-  const int split = (blockIdx.x / a.kv_heads) % a.splits;
-  const int tile = a.tiles - 1 - blockIdx.x / (a.kv_heads * a.splits);  // causal: long tiles first
+  if (warp == 5 * W && lane == 0) {
+    ptx::prefetch_map(&maps.k);
+    ptx::prefetch_map(&maps.q);
+    ptx::prefetch_map(&maps.v);
+  }
+  const int kvh = blockIdx.x % a.kv_heads, split = blockIdx.y;
+  const int tile = a.tiles - 1 - blockIdx.x / a.kv_heads;  // causal: long tiles first
   const int span = W * a.tokens;
   ptx::griddep_launch();
   int seq = 0, q0 = 0, q_len = (int)a.total_q, k0 = 0, k_len = (int)a.total_k, first = 0;
@@ -187,7 +191,12 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
     end[w] = !any ? 0 : a.causal ? max(0, min(k_len, t_end + k_len - q_len)) : k_len;
   }
   const int steps_all = (max(end[0], end[1]) + kKeys - 1) / kKeys;
-  const int ja = (int)((long long)steps_all * split / a.splits), jb = (int)((long long)steps_all * (split + 1) / a.splits);
+  int ja = 0, jb = steps_all;
+  if (a.splits > 1) {  // as even as tiles allow: the first `over` splits have one more
+    const int each = steps_all / a.splits, over = steps_all - each * a.splits;
+    ja = split * each + min(split, over);
+    jb = ja + each + (split < over);
+  }
   const int key0 = ja * kKeys;  // this split's first key
   const int cnt0 = max(0, (min(jb * kKeys, end[0]) - key0 + kUnit - 1) / kUnit);  // steps of the tiles
   const int cnt1 = max(0, (min(jb * kKeys, end[1]) - key0 + kUnit - 1) / kUnit);
@@ -202,7 +211,6 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
                        k0 + key0 + (n >> 1) * L::kTileKeys, &kv_full[st]);
   };
   // The first copies go out before the CTA meets, under the allocation of TMEM.
-  const int early = min(ring, L::kStages);
   if (warp == 5 * W && lane == 0) {
     for (int s = 0; s < L::kStages; ++s) {
       ptx::mbar_init(&kv_full[s], 1);
@@ -219,7 +227,7 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    if (early > 0) load_kv(0);
+    if (ring > 0) load_kv(0);
     for (int w = 0; w < W; ++w)
       if ((w == 0 ? cnt0 : cnt1) > 0) {
         ptx::mbar_expect_tx(&q_full[w], (unsigned)(a.tokens * a.group * 128 * L::kHalves));
@@ -227,7 +235,6 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
           ptx::tma_load_4d(sbase + w * L::kQ + h * L::kQHalf, &maps.q, h * 64, 0, kvh, q0 + tok0 + w * a.tokens,
                            &q_full[w]);
       }
-    for (int n = 1; n < early; ++n) load_kv(n);
   }
   if (warp == 4 * W) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ptx::saddr(tmem_slot)),
@@ -244,9 +251,9 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
   if (warp == 5 * W) {
     // ---- the other copies ----
     if (lane == 0) {
-      int n = early;
+      int n = min(ring, 1);
       for (; n < ring; ++n) {
-        if (!ptx::wait_phase(&kv_empty[n % L::kStages], (n / L::kStages - 1) & 1, abort_flag, a.err, kAttnWaitFree)) break;
+        if (n >= L::kStages && !ptx::wait_phase(&kv_empty[n % L::kStages], (n / L::kStages - 1) & 1, abort_flag, a.err, kAttnWaitFree)) break;
         load_kv(n);
       }
       // Copies in flight land before the CTA exits.
@@ -543,30 +550,29 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
 #pragma unroll 1
       for (int from = 0; from < a.head_size; from += width) {
 #pragma unroll 1
-        for (int k = 0; k < width; k += 32) {
-          unsigned o[32];
+        for (int k = 0; k < width; k += D / 2) {
+          unsigned o[D / 2];
           if (mine > 0) {
-            ptx::tmem_ld32(o_addr + from + k, o);
+#pragma unroll
+            for (int e = 0; e < D / 2; e += 32) ptx::tmem_ld32(o_addr + from + k + e, o + e);
             ptx::tc_wait_ld();
           }
-          float v[32];
+          float* v = reinterpret_cast<float*>(o);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = l == 0.0f ? 0.0f : __uint_as_float(o[e]) * inv;
+          for (int e = 0; e < D / 2; ++e) v[e] = l == 0.0f ? 0.0f : v[e] * inv;
           if (parts) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              put((k + e) / 4, __float_as_uint(v[e]), __float_as_uint(v[e + 1]), __float_as_uint(v[e + 2]),
-                  __float_as_uint(v[e + 3]));
+            for (int e = 0; e < D / 2; e += 4) put((k + e) / 4, o[e], o[e + 1], o[e + 2], o[e + 3]);
           } else {
 #pragma unroll
-            for (int e = 0; e < 32; e += 8)
+            for (int e = 0; e < D / 2; e += 8)
               put((k + e) / 8, ptx::pack16<BF16>(v[e], v[e + 1]), ptx::pack16<BF16>(v[e + 2], v[e + 3]),
                   ptx::pack16<BF16>(v[e + 4], v[e + 5]), ptx::pack16<BF16>(v[e + 6], v[e + 7]));
           }
         }
         __syncwarp();
         const int chunk = lane % kChunks, channel = from + chunk * (parts ? 4 : 8);
-#pragma unroll 4
+#pragma unroll
         for (int i = 0; i < 32; i += 32 / kChunks) {
           const int r2 = i + lane / kChunks;
           const unsigned long long dst = __shfl_sync(0xffffffffu, to, r2);
@@ -1014,7 +1020,7 @@ void launch_after(void (*kernel)(P...), unsigned grid, unsigned block, int share
 template <int D, int W, bool BF16>
 void launch_tc_as(const TcArgs& t, const TcMaps& maps, cudaStream_t stream) {
   using L = TcLayout<D, W>;
-  const unsigned grid = (unsigned)t.tiles * t.kv_heads * t.splits;
+  const dim3 grid((unsigned)t.tiles * t.kv_heads, t.splits);
   attention_tc_kernel<D, W, BF16><<<grid, L::kThreads, L::kTotal, stream>>>(t, maps);
   FA_CUDA(cudaGetLastError());
 }

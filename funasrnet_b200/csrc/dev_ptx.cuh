@@ -62,6 +62,9 @@ __device__ __forceinline__ bool wait_phase(uint64_t* bar, unsigned parity, volat
   return wait_phase_slow(bar, parity, abort_flag, err, code, honour_abort);
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 // Tiled tensor loads completing on an mbarrier.
 __device__ __forceinline__ void tma_load_3d(unsigned dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
