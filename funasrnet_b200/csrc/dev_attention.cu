@@ -126,6 +126,12 @@ __device__ __forceinline__ int tile_sequence(const TcArgs& a, int tile, int span
   return lo;
 }
 
+__device__ __forceinline__ uint4 lds16(unsigned addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+
 // One CTA: W tiles of 128 query rows (tokens x the heads that share a KV head)
 // against the keys of their sequence, 64 keys a step:
 //   the last warp copies Q, then K and V tiles through a ring (TMA);
@@ -166,6 +172,21 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
     ptx::prefetch_map(&maps.k);
     ptx::prefetch_map(&maps.q);
     ptx::prefetch_map(&maps.v);
+    for (int s = 0; s < L::kStages; ++s) {
+      ptx::mbar_init(&kv_full[s], 1);
+      ptx::mbar_init(&kv_empty[s], W);  // every issuer
+    }
+    for (int w = 0; w < 2; ++w) {
+      ptx::mbar_init(&q_full[w], 1);
+      ptx::mbar_init(&drained[w], 1);
+    }
+    for (int b = 0; b < 4; ++b) {
+      ptx::mbar_init(&s_full[b], 1);
+      ptx::mbar_init(&p_full[b], 4);
+      ptx::mbar_init(&pv_done[b], 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   const int kvh = blockIdx.x % a.kv_heads, split = blockIdx.y;
   const int tile = a.tiles - 1 - blockIdx.x / a.kv_heads;  // causal: long tiles first
@@ -212,21 +233,6 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
   };
   // The first copies go out before the CTA meets, under the allocation of TMEM.
   if (warp == 5 * W && lane == 0) {
-    for (int s = 0; s < L::kStages; ++s) {
-      ptx::mbar_init(&kv_full[s], 1);
-      ptx::mbar_init(&kv_empty[s], W);  // every issuer
-    }
-    for (int w = 0; w < 2; ++w) {
-      ptx::mbar_init(&q_full[w], 1);
-      ptx::mbar_init(&drained[w], 1);
-    }
-    for (int b = 0; b < 4; ++b) {
-      ptx::mbar_init(&s_full[b], 1);
-      ptx::mbar_init(&p_full[b], 4);
-      ptx::mbar_init(&pv_done[b], 1);
-    }
-    *abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (ring > 0) load_kv(0);
     for (int w = 0; w < W; ++w)
       if ((w == 0 ? cnt0 : cnt1) > 0) {
@@ -546,44 +552,63 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
                      "r"(x), "r"(y), "r"(z), "r"(u)
                      : "memory");
       };
-      const int width = parts ? D / 2 : D;  // channels of a pass: as many as fill a row of the stage
-#pragma unroll 1
-      for (int from = 0; from < a.head_size; from += width) {
-#pragma unroll 1
-        for (int k = 0; k < width; k += D / 2) {
-          unsigned o[D / 2];
-          if (mine > 0) {
+      // Rows of the stage to their places, 16 bytes a lane, eight loads before the stores.
+      auto drain = [&](int from, int size) {
+        __syncwarp();
+        const int chunk = lane % kChunks, channel = from + chunk * (16 / size);
+        constexpr int kEach = 32 / kChunks, kBatch = 8;
 #pragma unroll
-            for (int e = 0; e < D / 2; e += 32) ptx::tmem_ld32(o_addr + from + k + e, o + e);
-            ptx::tc_wait_ld();
+        for (int i = 0; i < kChunks; i += kBatch) {
+          uint4 v[kBatch];
+          unsigned long long dst[kBatch];
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+            const int r2 = (i + b) * kEach + lane / kChunks;
+            dst[b] = __shfl_sync(0xffffffffu, to, r2);
+            v[b] = lds16(stage + r2 * kRowBytes + ((chunk ^ (r2 & 7)) << 4));
           }
-          float* v = reinterpret_cast<float*>(o);
 #pragma unroll
-          for (int e = 0; e < D / 2; ++e) v[e] = l == 0.0f ? 0.0f : v[e] * inv;
-          if (parts) {
-#pragma unroll
-            for (int e = 0; e < D / 2; e += 4) put((k + e) / 4, o[e], o[e + 1], o[e + 2], o[e + 3]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < D / 2; e += 8)
-              put((k + e) / 8, ptx::pack16<BF16>(v[e], v[e + 1]), ptx::pack16<BF16>(v[e + 2], v[e + 3]),
-                  ptx::pack16<BF16>(v[e + 4], v[e + 5]), ptx::pack16<BF16>(v[e + 6], v[e + 7]));
+          for (int b = 0; b < kBatch; ++b) {
+            const int r2 = (i + b) * kEach + lane / kChunks;
+            if (((lives >> r2) & 1u) && channel < a.head_size)
+              *reinterpret_cast<uint4*>(dst[b] + (unsigned long long)channel * size) = v[b];
           }
         }
         __syncwarp();
-        const int chunk = lane % kChunks, channel = from + chunk * (parts ? 4 : 8);
+      };
+      const bool blank = __any_sync(0xffffffffu, l == 0.0f);  // rows whose O means nothing
+      auto take = [&](int from, auto count, float* v) {  // columns of O, divided by the row's sum
+        constexpr int N = decltype(count)::value;
+        if (mine > 0) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 32 / kChunks) {
-          const int r2 = i + lane / kChunks;
-          const unsigned long long dst = __shfl_sync(0xffffffffu, to, r2);
-          uint4 v;
-          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                       : "r"(stage + r2 * kRowBytes + ((chunk ^ (r2 & 7)) << 4)));
-          if (((lives >> r2) & 1u) && channel < a.head_size)
-            *reinterpret_cast<uint4*>(dst + (unsigned long long)channel * (parts ? 4 : 2)) = v;
+          for (int e = 0; e < N; e += 32) ptx::tmem_ld32(o_addr + from + e, reinterpret_cast<unsigned*>(v) + e);
+          ptx::tc_wait_ld();
         }
-        __syncwarp();
+        if (blank) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) v[e] = l == 0.0f ? 0.0f : v[e];
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] *= inv;
+      };
+      if (parts) {
+#pragma unroll 1
+        for (int from = 0; from < a.head_size; from += D / 2) {
+          float v[D / 2];
+          take(from, std::integral_constant<int, D / 2>{}, v);
+#pragma unroll
+          for (int e = 0; e < D / 2; e += 4)
+            put(e / 4, __float_as_uint(v[e]), __float_as_uint(v[e + 1]), __float_as_uint(v[e + 2]), __float_as_uint(v[e + 3]));
+          drain(from, 4);
+        }
+      } else {
+        float v[D];
+        take(0, std::integral_constant<int, D>{}, v);
+#pragma unroll
+        for (int e = 0; e < D; e += 8)
+          put(e / 8, ptx::pack16<BF16>(v[e], v[e + 1]), ptx::pack16<BF16>(v[e + 2], v[e + 3]),
+              ptx::pack16<BF16>(v[e + 4], v[e + 5]), ptx::pack16<BF16>(v[e + 6], v[e + 7]));
+        drain(0, 2);
       }
       const float lse = (m == -INFINITY ? 0.0f : m * a.scale) + logf(l);
       if (live && a.part_o) a.part_lse[split * a.total_q * a.heads + row] = lse;
@@ -659,12 +684,6 @@ __device__ __forceinline__ unsigned transpose8(unsigned x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint4 lds16(unsigned addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
-}
-
 // One query token of one sequence, up to 8 of the heads that share a KV head.
 // Warp 4 streams the keys through a ring of 64-key stages (TMA); warp w takes
 // keys 16w .. 16w + 15 of a stage, and lane (g = lane / 4, t = lane % 4) reads
