@@ -270,145 +270,136 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
     }
     __syncwarp();
   } else if (warp >= 4 * W) {
-    // ---- MMAs of one tile: uniform values, constant offsets and no arithmetic
-    // between the MMAs of a step ----
-    const int w = W == 2 ? warp - 8 : 0, mine = w ? cnt1 : cnt0;
-    const unsigned id_s = ptx::idesc_f16(BF16, false, kRows, kUnit);
-    const int n_o = (a.head_size + 15) / 16 * 16;  // channels past head_size are zeros (TMA fill)
-    const unsigned id_o = ptx::idesc_f16(BF16, true, kRows, n_o);
-    const int k_s = n_o / 16;
-    bool ok = true;
-    auto wait = [&](uint64_t* bar, unsigned parity, int code) {
-      ok = ok && __all_sync(0xffffffffu, ptx::wait_phase(bar, parity, abort_flag, a.err, code));
-      ptx::tc_fence_after();
-    };
-    const unsigned q_low = ptx::smem_desc_low(sbase, 16), k_low = ptx::smem_desc_low(sbase + L::kKv, 16),
-                   v_low = ptx::smem_desc_low(sbase + L::kKv, L::kHalf);
-    struct Slot {  // a tile's place in the ring; K tiles have even numbers, V tiles odd ones
-      int st;
-      unsigned ph;
-      __device__ __forceinline__ void next() {
-        st += 2;
-        if (st >= L::kStages) {
-          st -= L::kStages;
-          ph ^= 1;
+    // ---- MMAs of one tile, by one thread: constant offsets and no arithmetic
+    // between the MMAs of a step, no votes between the waits ----
+    if (ptx::elect()) {
+      const int w = W == 2 ? warp - 8 : 0, mine = w ? cnt1 : cnt0;
+      const unsigned id_s = ptx::idesc_f16(BF16, false, kRows, kUnit);
+      const int n_o = (a.head_size + 15) / 16 * 16;  // channels past head_size are zeros (TMA fill)
+      const unsigned id_o = ptx::idesc_f16(BF16, true, kRows, n_o);
+      const int k_s = n_o / 16;
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, unsigned parity, int code) {
+        ok = ok && ptx::wait_phase(bar, parity, abort_flag, a.err, code);
+      };
+      const unsigned q_low = ptx::smem_desc_low(sbase + w * L::kQ, 16), k_low = ptx::smem_desc_low(sbase + L::kKv, 16),
+                     v_low = ptx::smem_desc_low(sbase + L::kKv, L::kHalf);
+      struct Slot {  // a tile's place in the ring; K tiles have even numbers, V tiles odd ones
+        int st;
+        unsigned ph;
+        __device__ __forceinline__ void next() {
+          st += 2;
+          if (st >= L::kStages) {
+            st -= L::kStages;
+            ph ^= 1;
+          }
         }
-      }
-    };
-    Slot ks{0, 0}, vs{1, 0};
-    constexpr int kPart = W == 2 ? kUnit * 128 : 0;  // bytes between the steps of a tile
-    auto scores = [&](int b) {  // S_w of the K tile (W = 2: of its half b) into buffer b
-      const unsigned q = q_low + w * (L::kQ >> 4);
-      const unsigned k = k_low + ks.st * (L::kTile >> 4) + b * (kPart >> 4);
-      if (ptx::elect()) {
+      };
+      Slot ks{0, 0}, vs{1, 0};
+      constexpr int kPart = W == 2 ? kUnit * 128 : 0;  // bytes between the steps of a tile
+      const unsigned s_at = tm + w * 128, o_at = tm + L::kO + w * D;
+      auto scores = [&](int b) {  // S_w of the K tile (W = 2: of its half b) into buffer b
+        const unsigned k = k_low + ks.st * (L::kTile >> 4) + b * (kPart >> 4);
         if (k_s == D / 16) {
 #pragma unroll
-          for (int s = 0; s < D / 16; ++s) {
-            ptx::tc_mma_ss(tm + w * 128 + b * kUnit, q + (((s >> 2) * L::kQHalf + (s & 3) * 32) >> 4),
+          for (int s = 0; s < D / 16; ++s)
+            ptx::tc_mma_ss(s_at + b * kUnit, q_low + (((s >> 2) * L::kQHalf + (s & 3) * 32) >> 4),
                            k + (((s >> 2) * L::kHalf + (s & 3) * 32) >> 4), id_s, s > 0);
-          }
         } else {
-          for (int s = 0; s < k_s; ++s) {
-            ptx::tc_mma_ss(tm + w * 128 + b * kUnit, q + (((s >> 2) * L::kQHalf + (s & 3) * 32) >> 4),
+          for (int s = 0; s < k_s; ++s)
+            ptx::tc_mma_ss(s_at + b * kUnit, q_low + (((s >> 2) * L::kQHalf + (s & 3) * 32) >> 4),
                            k + (((s >> 2) * L::kHalf + (s & 3) * 32) >> 4), id_s, s > 0);
-          }
         }
         ptx::tc_commit(&s_full[2 * w + b]);
-      }
-      __syncwarp();
-    };
-    auto values = [&](int b, int steps, bool acc) {  // O_w += P_w (buffer b) x the V tile (its half b)
-      const unsigned v = v_low + vs.st * (L::kTile >> 4) + b * (kPart >> 4);
-      if (ptx::elect()) {
+      };
+      auto values = [&](int b, int steps, bool acc) {  // O_w += P_w (buffer b) x the V tile (its half b)
+        const unsigned v = v_low + vs.st * (L::kTile >> 4) + b * (kPart >> 4);
+        ptx::tc_fence_after();
         if (steps == kUnit / 16) {
 #pragma unroll
           for (int s = 0; s < kUnit / 16; ++s)
-            ptx::tc_mma_ts(tm + L::kO + w * D, tm + w * 128 + b * kUnit + s * 8, v + (s * 2048 >> 4), id_o, acc || s > 0);
+            ptx::tc_mma_ts(o_at, s_at + b * kUnit + s * 8, v + (s * 2048 >> 4), id_o, acc || s > 0);
         } else {
           for (int s = 0; s < steps; ++s)
-            ptx::tc_mma_ts(tm + L::kO + w * D, tm + w * 128 + b * kUnit + s * 8, v + (s * 2048 >> 4), id_o, acc || s > 0);
+            ptx::tc_mma_ts(o_at, s_at + b * kUnit + s * 8, v + (s * 2048 >> 4), id_o, acc || s > 0);
         }
         ptx::tc_commit(&pv_done[2 * w + b]);
-      }
-      __syncwarp();
-    };
-    auto release = [&](int st) {
-      if (ok && ptx::elect()) ptx::tc_commit(&kv_empty[st]);
-      __syncwarp();
-    };
-    // Value rows behind the last key that a row sees are not the sequence's own,
-    // or masked for every row here: 0 x what they hold must stay 0.
-    auto clear_tail = [&](int key) {
-      const int most = min(max(end[0], end[1]) - key0 - key, L::kTileKeys), padded = (most + 15) / 16 * 16;
-      if (most >= padded) return;
-      uint8_t* v = sm + L::kKv + vs.st * L::kTile;
-      for (int c = lane; c < (padded - most) * 8; c += 32)
-        for (int h = 0; h < L::kHalves; ++h)
-          *reinterpret_cast<uint4*>(v + h * L::kHalf + (most + c / 8) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-    };
-    auto steps_of = [&](int n) { return (min(end[w] - key0 - n * kUnit, kUnit) + 15) / 16; };
-    if (cnt > 0) wait(&kv_full[0], 0, kAttnWaitLoad);
-    if (mine > 0) wait(&q_full[w], 0, kAttnWaitLoad);
-    if (W == 1) {  // a tile a step
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        if (!ok || b >= mine) continue;
-        if (b == 1) wait(&kv_full[ks.st], ks.ph, kAttnWaitLoad);
-        if (ok) scores(b);
-        release(ks.st);
-        ks.next();
-      }
-      for (int n0 = 0; n0 < mine && ok; n0 += 2)
+      };
+      auto release = [&](int st) {
+        if (ok) ptx::tc_commit(&kv_empty[st]);
+      };
+      // Value rows behind the last key that a row sees are not the sequence's own,
+      // or masked for every row here: 0 x what they hold must stay 0.
+      auto clear_tail = [&](int key) {
+        const int most = min(max(end[0], end[1]) - key0 - key, L::kTileKeys), padded = (most + 15) / 16 * 16;
+        if (most >= padded) return;
+        uint8_t* v = sm + L::kKv + vs.st * L::kTile;
+        for (int c = 0; c < (padded - most) * 8; ++c)
+          for (int h = 0; h < L::kHalves; ++h)
+            *reinterpret_cast<uint4*>(v + h * L::kHalf + (most + c / 8) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      };
+      auto steps_of = [&](int n) { return (min(end[w] - key0 - n * kUnit, kUnit) + 15) / 16; };
+      if (cnt > 0) wait(&kv_full[0], 0, kAttnWaitLoad);
+      if (mine > 0) wait(&q_full[w], 0, kAttnWaitLoad);
+      if (W == 1) {  // a tile a step
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const int n = n0 + b;
-          if (!ok || n >= mine) continue;
-          wait(&kv_full[vs.st], vs.ph, kAttnWaitLoad);
-          if (ok) clear_tail(n * kUnit);
-          wait(&p_full[b], (n0 >> 1) & 1, kAttnWaitSoftmax);
-          if (!ok) continue;
-          values(b, steps_of(n), n > 0);
-          release(vs.st);
-          vs.next();
-          if (n + 2 >= mine) continue;
-          wait(&kv_full[ks.st], ks.ph, kAttnWaitLoad);
+          if (!ok || b >= mine) continue;
+          if (b == 1) wait(&kv_full[ks.st], ks.ph, kAttnWaitLoad);
           if (ok) scores(b);
           release(ks.st);
           ks.next();
         }
-    } else {
-      if (ok && mine > 0) scores(0);
-      if (ok && mine > 1) scores(1);
-      if (cnt > 0) release(0);
-      ks.next();
-      for (int n0 = 0; n0 < cnt && ok; n0 += 2) {  // one V tile, and the K tile after its own
-        // Waits, and releases below, also for tiles that only the other issuer uses:
-        // one that ran ahead would release a slot's next use.
-        wait(&kv_full[vs.st], vs.ph, kAttnWaitLoad);
-        if (!ok) break;
-        if (n0 < mine) clear_tail(n0 * kUnit);
+        for (int n0 = 0; n0 < mine && ok; n0 += 2)
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const int n = n0 + b;
-          if (!ok || n >= mine) continue;
-          wait(&p_full[2 * w + b], (n0 >> 1) & 1, kAttnWaitSoftmax);
-          if (!ok) continue;
-          values(b, steps_of(n), n > 0);
-          if (b == 0 && n0 + 2 < mine) wait(&kv_full[ks.st], ks.ph, kAttnWaitLoad);
-          if (ok && n + 2 < mine) scores(b);
-        }
-        if (ok && n0 + 2 < cnt && n0 + 2 >= mine) wait(&kv_full[ks.st], ks.ph, kAttnWaitLoad);
-        release(vs.st);
-        if (n0 + 2 < cnt) release(ks.st);
-        vs.next();
+          for (int b = 0; b < 2; ++b) {
+            const int n = n0 + b;
+            if (!ok || n >= mine) continue;
+            wait(&kv_full[vs.st], vs.ph, kAttnWaitLoad);
+            if (ok) clear_tail(n * kUnit);
+            wait(&p_full[b], (n0 >> 1) & 1, kAttnWaitSoftmax);
+            if (!ok) continue;
+            values(b, steps_of(n), n > 0);
+            release(vs.st);
+            vs.next();
+            if (n + 2 >= mine) continue;
+            wait(&kv_full[ks.st], ks.ph, kAttnWaitLoad);
+            if (ok) scores(b);
+            release(ks.st);
+            ks.next();
+          }
+      } else {
+        if (ok && mine > 0) scores(0);
+        if (ok && mine > 1) scores(1);
+        if (cnt > 0) release(0);
         ks.next();
+        for (int n0 = 0; n0 < cnt && ok; n0 += 2) {  // one V tile, and the K tile after its own
+          // Waits, and releases below, also for tiles that only the other issuer uses:
+          // one that ran ahead would release a slot's next use.
+          wait(&kv_full[vs.st], vs.ph, kAttnWaitLoad);
+          if (!ok) break;
+          if (n0 < mine) clear_tail(n0 * kUnit);
+          if (n0 + 2 < cnt) wait(&kv_full[ks.st], ks.ph, kAttnWaitLoad);
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const int n = n0 + b;
+            if (!ok || n >= mine) continue;
+            wait(&p_full[2 * w + b], (n0 >> 1) & 1, kAttnWaitSoftmax);
+            if (!ok) continue;
+            values(b, steps_of(n), n > 0);
+            if (n + 2 < mine) scores(b);
+          }
+          release(vs.st);
+          if (n0 + 2 < cnt) release(ks.st);
+          vs.next();
+          ks.next();
+        }
       }
-    }
-    if (!ok && ptx::elect()) {  // MMAs in flight finish before their memory is freed
-      ptx::tc_commit(&drained[w]);
-      ptx::wait_phase(&drained[w], 0, abort_flag, a.err, kAttnWaitMma, false);
+      if (!ok) {  // MMAs in flight finish before their memory is freed
+        ptx::tc_commit(&drained[w]);
+        ptx::wait_phase(&drained[w], 0, abort_flag, a.err, kAttnWaitMma, false);
+      }
     }
     __syncwarp();
   } else {
@@ -934,7 +925,7 @@ struct JoinArgs {
 constexpr int kJoinWarps = 4;
 
 template <typename T, int W>
-__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const JoinArgs a) {
+__global__ void __launch_bounds__(32 * kJoinWarps, 8) join_kernel(const JoinArgs a) {
   __shared__ float4 sm_o[kJoinWarps][32];
   __shared__ float sm_sum[kJoinWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -949,22 +940,22 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const JoinArgs a)
     for (int s = lane; s < a.parts; s += 32) top = fmaxf(top, a.part_lse[s * rows + row]);
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  }
-  const float base = top == -INFINITY ? 0.0f : top;
-  if (live) {
-#pragma unroll 8
-    for (int s = part; s < a.parts; s += W) {
-      const float f = expf(a.part_lse[s * rows + row] - base);
+    const float base = top == -INFINITY ? 0.0f : top;
+    const long long step = W * rows;
+    const float* lse = a.part_lse + part * rows + row;
+    const float* from = a.part_o + (part * rows + row) * a.head_size + (c < a.head_size ? c : 0);
+#pragma unroll 4
+    for (int s = part; s < a.parts; s += W, lse += step, from += step * a.head_size) {
+      const float4 v = *reinterpret_cast<const float4*>(from);
+      const float f = expf(*lse - base);
       sum += f;
-      if (c < a.head_size) {
-        const float4 v = *reinterpret_cast<const float4*>(a.part_o + (s * rows + row) * a.head_size + c);
-        o[0] = fmaf(f, v.x, o[0]);
-        o[1] = fmaf(f, v.y, o[1]);
-        o[2] = fmaf(f, v.z, o[2]);
-        o[3] = fmaf(f, v.w, o[3]);
-      }
+      o[0] = fmaf(f, v.x, o[0]);
+      o[1] = fmaf(f, v.y, o[1]);
+      o[2] = fmaf(f, v.z, o[2]);
+      o[3] = fmaf(f, v.w, o[3]);
     }
   }
+  const float base = top == -INFINITY ? 0.0f : top;
   if (W > 1) {
     sm_o[warp][lane] = make_float4(o[0], o[1], o[2], o[3]);
     if (lane == 0) sm_sum[warp] = sum;
@@ -1154,11 +1145,11 @@ PackedPlan packed_plan(int64_t total_q, int64_t total_k, int sequences, int head
   const double steps = (double)total_k / sequences / kKeys;  // key tiles of a sequence, on average
   p.w = steps <= kShort ? 1 : 2;
   const double ctas = (double)packed_tiles(total_q, sequences, heads / kv_heads, p.w) * kv_heads;
-  // The longest sequence is taken for 1.5 times the average: its CTAs' steps, or
+  // The longest sequence is taken for 2.5 times the average: its CTAs' steps, or
   // all steps spread over the SMs, at kStepUs each; cutting the keys costs a
   // second kernel and the parts' bytes, written and read.
   auto cost = [&](int s) {
-    const double longest = std::max(1.0, (sequences > 1 ? 1.5 : 1.0) * steps / s);
+    const double longest = std::max(1.0, (sequences > 1 ? 2.5 : 1.0) * steps / s);
     const double each = p.w == 2 ? kStepUs : 0.7 * kStepUs, sms = p.w == 2 ? kSms : 2 * kSms;
     const double parts = s > 1 ? 4.0 + 2.0 * s * total_q * heads * (head_size + 1) * 4 / 4e6 : 0.0;
     return std::max(longest, ctas * steps / sms) * each + ctas * s / sms * 1.5 + parts;
