@@ -108,22 +108,65 @@ struct TcLayout {
   static_assert(kTotal <= (W == 2 ? 227 : 113) * 1024, "shared memory of one or two CTAs an SM");
 };
 
-// Tile t of the call -> its sequence.  Sequence b's tiles start at
-// floor(off[b] / span) + b, which leaves room for its ceil(length / span) tiles
-// without a sum over the sequences before it; a few numbers stay unused.
-__device__ __forceinline__ int tile_sequence(const TcArgs& a, int tile, int span) {
+// Where a CTA works: its sequence's queries and keys, and its first query token.
+struct Place {
+  int q0 = 0, q_len = 0, k0 = 0, k_len = 0, token = -1;  // token < 0: nowhere
+};
+
+// Number t of the call -> its place, for up to 32 sequences: a lane per sequence.
+// Sequences with more keys come first, and in each the last tile first (it sees
+// the most keys): the SMs that finish early take the short ones.
+__device__ __forceinline__ Place place_sorted(const TcArgs& a, int t, int span) {
   const int lane = threadIdx.x & 31;
+  Place p;
+  if (lane < a.sequences) {
+    p.q0 = clamp_to(a.q_off[lane], a.total_q);
+    p.q_len = clamp_to(a.q_off[lane + 1], a.total_q) - p.q0;
+    p.k0 = clamp_to(a.k_off[lane], a.total_k);
+    p.k_len = max(0, clamp_to(a.k_off[lane + 1], a.total_k) - p.k0);
+  }
+  const int mine = p.q_len > 0 ? (p.q_len + span - 1) / span : 0;
+  int start = 0;  // tiles of the sequences before this lane's
+  for (int j = 0; j < a.sequences; ++j) {
+    const int k = __shfl_sync(0xffffffffu, p.k_len, j), n = __shfl_sync(0xffffffffu, mine, j);
+    if (k > p.k_len || (k == p.k_len && j < lane)) start += n;
+  }
+  const unsigned here = __ballot_sync(0xffffffffu, t >= start && t < start + mine);
+  if (here == 0) return Place{};
+  const int b = __ffs(here) - 1;
+  p.token = (mine - 1 - (t - start)) * span;
+  p.q0 = __shfl_sync(0xffffffffu, p.q0, b);
+  p.q_len = __shfl_sync(0xffffffffu, p.q_len, b);
+  p.k0 = __shfl_sync(0xffffffffu, p.k0, b);
+  p.k_len = __shfl_sync(0xffffffffu, p.k_len, b);
+  p.token = __shfl_sync(0xffffffffu, p.token, b);
+  return p;
+}
+
+// The same for any number of sequences, in their own order from the last tile
+// on.  Sequence b's tiles start at floor(off[b] / span) + b, which leaves room
+// for its ceil(length / span) tiles without a sum over the sequences before it;
+// a few numbers stay unused.
+__device__ __forceinline__ Place place_searched(const TcArgs& a, int t, int span) {
+  const int lane = threadIdx.x & 31, tile = a.tiles - 1 - t;
   int lo = 0, hi = a.sequences;
   while (hi - lo > 1) {
     const int step = (hi - lo + 31) / 32, b = lo + lane * step;
     const bool before = b < hi && clamp_to(a.q_off[b], a.total_q) / span + b <= tile;
     const int n = __popc(__ballot_sync(0xffffffffu, before));
-    if (n == 0) return -1;
+    if (n == 0) return Place{};
     lo += (n - 1) * step;
     hi = min(hi, lo + step);
     if (step == 1) break;
   }
-  return lo;
+  Place p;
+  p.q0 = clamp_to(a.q_off[lo], a.total_q);
+  p.q_len = clamp_to(a.q_off[lo + 1], a.total_q) - p.q0;
+  p.k0 = clamp_to(a.k_off[lo], a.total_k);
+  p.k_len = max(0, clamp_to(a.k_off[lo + 1], a.total_k) - p.k0);
+  const int i = tile - (p.q0 / span + lo);
+  p.token = i >= 0 && i * (long long)span < p.q_len ? i * span : -1;
+  return p;
 }
 
 __device__ __forceinline__ uint4 lds16(unsigned addr) {
@@ -188,22 +231,23 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  const int kvh = blockIdx.x % a.kv_heads, split = blockIdx.y;
-  const int tile = a.tiles - 1 - blockIdx.x / a.kv_heads;  // causal: long tiles first
-  const int span = W * a.tokens;
-  ptx::griddep_launch();
-  int seq = 0, q0 = 0, q_len = (int)a.total_q, k0 = 0, k_len = (int)a.total_k, first = 0;
-  if (a.q_off) {
-    seq = tile_sequence(a, tile, span);
-    if (seq < 0) return;
-    q0 = clamp_to(a.q_off[seq], a.total_q);
-    q_len = clamp_to(a.q_off[seq + 1], a.total_q) - q0;
-    k0 = clamp_to(a.k_off[seq], a.total_k);
-    k_len = max(0, clamp_to(a.k_off[seq + 1], a.total_k) - k0);
-    first = q0 / span + seq;
+  const int span = W * a.tokens, kvh = blockIdx.x % a.kv_heads;
+  int number = blockIdx.x / a.kv_heads, split = 0;
+  if (a.splits > 1) {
+    split = number % a.splits;
+    number /= a.splits;
   }
-  const int tok0 = (tile - first) * span;  // first token of the pair within the sequence
-  if (tok0 < 0 || tok0 >= q_len) return;
+  ptx::griddep_launch();
+  Place at;
+  if (a.q_off) {
+    at = a.sequences <= 32 ? place_sorted(a, number, span) : place_searched(a, number, span);
+  } else {
+    at.q_len = (int)a.total_q;
+    at.k_len = (int)a.total_k;
+    at.token = number * span;
+  }
+  if (at.token < 0) return;
+  const int q0 = at.q0, q_len = at.q_len, k0 = at.k0, k_len = at.k_len, tok0 = at.token;
   int end[2] = {0, 0};  // keys that some row of the tile sees
 #pragma unroll
   for (int w = 0; w < W; ++w) {
@@ -1030,7 +1074,7 @@ void launch_after(void (*kernel)(P...), unsigned grid, unsigned block, int share
 template <int D, int W, bool BF16>
 void launch_tc_as(const TcArgs& t, const TcMaps& maps, cudaStream_t stream) {
   using L = TcLayout<D, W>;
-  const dim3 grid((unsigned)t.tiles * t.kv_heads, t.splits);
+  const unsigned grid = (unsigned)t.tiles * t.kv_heads * t.splits;
   attention_tc_kernel<D, W, BF16><<<grid, L::kThreads, L::kTotal, stream>>>(t, maps);
   FA_CUDA(cudaGetLastError());
 }
