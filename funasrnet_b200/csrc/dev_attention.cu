@@ -38,6 +38,19 @@ void need_strides(const int64_t* s, int n) {
   for (int i = 0; i < n; ++i) need(s[i] >= 0 && s[i] < (1ll << 38), "a stride is negative or beyond 2^38 elements");
 }
 
+// Whether no two elements of a strided output share a place.
+bool apart(const int64_t* strides, const int64_t* extents, int64_t inner) {
+  int order[2] = {0, 1};
+  if (strides[1] < strides[0]) std::swap(order[0], order[1]);
+  int64_t span = inner;
+  for (int d : order) {
+    if (extents[d] <= 1) continue;
+    if (strides[d] < span) return false;
+    span += strides[d] * (extents[d] - 1);
+  }
+  return true;
+}
+
 void check_heads(int dtype, int sequences, int heads, int kv_heads, int head_size, float scale) {
   need(dtype == FA_DTYPE_F32 || dtype == FA_DTYPE_F16 || dtype == FA_DTYPE_BF16, "unknown dtype");
   need(sequences >= 0, "negative sequence count");
@@ -80,6 +93,9 @@ struct TcArgs {
   float* part_o = nullptr;     // with part_o: [splits x total_q x heads x head_size], and the rows' lse
   float* part_lse = nullptr;
   int* err = nullptr;
+  // What the maps describe, for rows that a masked value spoiled (mend_rows).
+  const void *q = nullptr, *k = nullptr, *v = nullptr;
+  long long q_token = 0, q_head = 0, k_token = 0, k_head = 0, v_token = 0, v_head = 0;
 };
 struct TcMaps {
   CUtensorMap q;  // (channel, head of the group, KV head, token)
@@ -175,6 +191,69 @@ __device__ __forceinline__ uint4 lds16(unsigned addr) {
   return v;
 }
 
+// A masked key's probability is 0, but 0 x infinity and 0 x NaN are NaN: where a
+// value behind the keys that a row sees (in the tile at the causal border) is
+// not finite, the row is computed again without it.  All lanes of a warp, for
+// the rows in `bad`: row r's lane has what it sees, its maximum (times the
+// scale's log2), 1 / sum, its query and its head.  The result goes to the row's
+// place in the stage, 4 channels a lane, from channel `from` on.
+template <typename T, bool kParts>
+__device__ __noinline__ void mend_rows(const TcArgs& a, unsigned bad, int first_key, int end_key, int sees, float base,
+                                       float inv, long long token, int head, long long k0, int kvh, int from, int width,
+                                       unsigned stage, int row_bytes) {
+  const int lane = threadIdx.x & 31, c = from + lane * 4;
+  const bool on = lane * 4 < width && c < a.head_size;
+  auto load = [](const T* p, float* x) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = (float)reinterpret_cast<const T*>(&u)[i];
+  };
+  for (; bad; bad &= bad - 1) {
+    const int r = __ffs(bad) - 1;
+    const int seen = min(__shfl_sync(0xffffffffu, sees, r), end_key);
+    const float m = __shfl_sync(0xffffffffu, base, r), by = __shfl_sync(0xffffffffu, inv, r);
+    const long long tok = __shfl_sync(0xffffffffu, token, r);
+    const int h = __shfl_sync(0xffffffffu, head, r);
+    const T* k = static_cast<const T*>(a.k) + k0 * a.k_token + kvh * a.k_head;
+    const T* v = static_cast<const T*>(a.v) + k0 * a.v_token + kvh * a.v_head;
+    bool spoiled = false;
+    for (int j = max(seen, first_key); j < end_key; ++j) {
+      float x[4] = {};
+      if (on) load(v + j * a.v_token + c, x);
+      spoiled |= !(isfinite(x[0]) && isfinite(x[1]) && isfinite(x[2]) && isfinite(x[3]));
+    }
+    if (!__any_sync(0xffffffffu, spoiled)) continue;  // what it sees is not finite
+    const T* q = static_cast<const T*>(a.q) + tok * a.q_token + h * a.q_head;
+    float o[4] = {}, qx[4] = {};
+    const int cq = lane * 4;
+    if (cq < a.head_size) load(q + cq, qx);
+    for (int j = first_key; j < seen; ++j) {
+      float kx[4] = {}, vx[4] = {}, dot = 0.0f;
+      if (cq < a.head_size) load(k + j * a.k_token + cq, kx);
+      if (on) load(v + j * a.v_token + c, vx);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dot = fmaf(qx[i], kx[i], dot);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+      const float p = ptx::ex2(fmaf(dot, a.scale_log2, -m));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = fmaf(p, vx[i], o[i]);
+    }
+    if (lane * 4 >= width) continue;
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] *= by;
+    const int chunk = kParts ? lane : lane / 2;
+    const unsigned at = stage + r * row_bytes + ((chunk ^ (r & 7)) << 4) + (kParts ? 0 : (lane & 1) * 8);
+    if (kParts)
+      asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(o[0]), "f"(o[1]), "f"(o[2]), "f"(o[3]) : "memory");
+    else
+      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(ptx::pack16<kBf16>(o[0], o[1])),
+                   "r"(ptx::pack16<kBf16>(o[2], o[3]))
+                   : "memory");
+  }
+}
+
 // One CTA: W tiles of 128 query rows (tokens x the heads that share a KV head)
 // against the keys of their sequence, 64 keys a step:
 //   the last warp copies Q, then K and V tiles through a ring (TMA);
@@ -194,7 +273,7 @@ __device__ __forceinline__ uint4 lds16(unsigned addr) {
 // when it rises by more than 2^kSlack, so O (in TMEM) is rescaled rarely.
 template <int D, int W, bool BF16>
 __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
-    attention_tc_kernel(const TcArgs a, const __grid_constant__ TcMaps maps) {
+    attention_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ TcMaps maps) {
   using L = TcLayout<D, W>;
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   extern __shared__ __align__(1024) uint8_t sm[];  // the tiles start on a swizzle atom
@@ -625,24 +704,45 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
         }
 #pragma unroll
         for (int e = 0; e < N; ++e) v[e] *= inv;
+        uint64_t zero = 0;  // stays 0 while all are finite
+#pragma unroll
+        for (int e = 0; e < N; e += 2)
+          if (e < a.head_size - from) zero = ptx::fma2(ptx::pair(v[e], v[e + 1]), 0, zero);
+        float z0, z1;
+        ptx::unpair(zero, z0, z1);
+        return !(z0 == 0.0f && z1 == 0.0f);
       };
+      // Keys that the products took in, masked ones among them: whole steps of 16, cleared behind the last that any row sees.
+      const int last_key =
+          min(max(end[0], end[1]), key0 + (min(jb * kKeys, end[w]) - key0 + 15) / 16 * 16);
+      const float base = m == -INFINITY ? 0.0f : m * c;
       if (parts) {
 #pragma unroll 1
         for (int from = 0; from < a.head_size; from += D / 2) {
           float v[D / 2];
-          take(from, std::integral_constant<int, D / 2>{}, v);
+          const bool odd = take(from, std::integral_constant<int, D / 2>{}, v);
 #pragma unroll
           for (int e = 0; e < D / 2; e += 4)
             put(e / 4, __float_as_uint(v[e]), __float_as_uint(v[e + 1]), __float_as_uint(v[e + 2]), __float_as_uint(v[e + 3]));
+          const unsigned bad = __ballot_sync(0xffffffffu, odd && live && a.causal);
+          if (bad) {
+            __syncwarp();
+            mend_rows<T, true>(a, bad, key0, last_key, sees, base, inv, t, h, k0, kvh, from, D / 2, stage, kRowBytes);
+          }
           drain(from, 4);
         }
       } else {
         float v[D];
-        take(0, std::integral_constant<int, D>{}, v);
+        const bool odd = take(0, std::integral_constant<int, D>{}, v);
 #pragma unroll
         for (int e = 0; e < D; e += 8)
           put(e / 8, ptx::pack16<BF16>(v[e], v[e + 1]), ptx::pack16<BF16>(v[e + 2], v[e + 3]),
               ptx::pack16<BF16>(v[e + 4], v[e + 5]), ptx::pack16<BF16>(v[e + 6], v[e + 7]));
+        const unsigned bad = __ballot_sync(0xffffffffu, odd && live && a.causal);
+        if (bad) {
+          __syncwarp();
+          mend_rows<T, false>(a, bad, key0, last_key, sees, base, inv, t, h, k0, kvh, 0, D, stage, kRowBytes);
+        }
         drain(0, 2);
       }
       const float lse = (m == -INFINITY ? 0.0f : m * a.scale) + logf(l);
@@ -1136,6 +1236,8 @@ int check_attention_packed(const fa_attention_packed_args* a) {
   if (a->total_q == 0 || a->sequences == 0) return kHandled;
   need(a->q && a->out && a->q_offsets && a->k_offsets, "null q, out, q_offsets or k_offsets");
   need(a->total_k == 0 || (a->k && a->v), "null k or v");
+  const int64_t extents[2] = {a->total_q, a->heads};
+  need(apart(a->out_stride, extents, a->head_size), "rows of out overlap");
   if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out)) return kDeclined;
   if (!strides16(a->q_stride, 2) || !strides16(a->k_stride, 2) || !strides16(a->v_stride, 2) ||
       !strides16(a->out_stride, 2))
@@ -1165,6 +1267,8 @@ int check_attention_shared(const fa_attention_shared_args* a) {
   need(a->prefix_len == 0 || (a->prefix_k && a->prefix_v), "null prefix_k or prefix_v");
   need(a->suffix_capacity == 0 || (a->suffix_k && a->suffix_v && a->suffix_lens),
        "null suffix_k, suffix_v or suffix_lens");
+  const int64_t extents[2] = {a->sequences, a->heads};
+  need(apart(a->out_stride, extents, a->head_size), "rows of out overlap");
   if (!aligned16(a->q) || !aligned16(a->prefix_k) || !aligned16(a->prefix_v) || !aligned16(a->suffix_k) ||
       !aligned16(a->suffix_v) || !aligned16(a->out))
     return kDeclined;
@@ -1294,6 +1398,15 @@ void launch_attention_packed(const fa_attention_packed_args& a, int* err, cudaSt
   t.out_head = a.out_stride[1];
   t.lse = a.lse;
   t.err = err;
+  t.q = a.q;
+  t.k = a.k;
+  t.v = a.v;
+  t.q_token = a.q_stride[0];
+  t.q_head = a.q_stride[1];
+  t.k_token = a.k_stride[0];
+  t.k_head = a.k_stride[1];
+  t.v_token = a.v_stride[0];
+  t.v_head = a.v_stride[1];
   if (t.splits > 1) {
     t.part_o = static_cast<float*>(a.workspace);
     t.part_lse = t.part_o + t.splits * a.total_q * a.heads * a.head_size;

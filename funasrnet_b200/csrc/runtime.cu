@@ -731,6 +731,7 @@ static int enqueue_dev(fa_backend* b, const Args* args, void* stream, int (*chec
     std::lock_guard<std::mutex> lk(b->mu);
     if (b->disposed) throw Error(kErrDisposed, "backend disposed");
     DeviceGuard g(b->device);
+    FA_CUDA(cudaSetDevice(b->device));  // a thread's first call: tensor maps need the context to be current
     launch(*args, b->dev_error, stream != nullptr ? static_cast<cudaStream_t>(stream) : b->stream);
     return (int)kHandled;
   });

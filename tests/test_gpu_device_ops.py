@@ -324,3 +324,284 @@ def test_logits_ties_infinities_and_nan(dev):
     assert tokens.tolist() == [7, -1, -1, 151935, 99, 0]
     x[5, 10:12] = -math.inf
     assert torch.equal(out.nan_to_num(nan=4.0), x.nan_to_num(nan=4.0))
+
+
+# --------------------------------------------------------- the rest of packed ----
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("sequences", [33, 300, 1500])
+def test_packed_many_sequences(dev, dtype, sequences):
+    """More sequences than a warp holds, many of them empty, some with fewer keys than queries."""
+    torch = torch_()
+    rng = random.Random(sequences)
+    new = [rng.choice([0, 0, 1, 2, rng.randint(1, 40)]) for _ in range(sequences)]
+    new[-1] = 5
+    keys = [rng.choice([0, n, n + rng.randint(0, 90), max(0, n - 3)]) for n in new]
+    dt = dtype_of(dtype)
+    q, k, v = randn(1, sum(new), 4, 64, dtype=dt), randn(2, sum(keys), 2, 64, dtype=dt), randn(3, sum(keys), 2, 64, dtype=dt)
+    out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device="cuda")
+    qo, ko = i32(sums(new)), i32(sums(keys))
+    assert dev.attention_packed(q, k, v, qo, ko, out, lse=lse, workspace=packed_space(dev, q, k, qo), stream=here())
+    torch.cuda.synchronize()
+    check_packed(q, k, v, new, keys, True, 0.125, out, lse)
+    dev.status()
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,size,new,keys,causal", [
+    ("f16", 8, 1, 128, [1], [9000], True),
+    ("bf16", 4, 4, 64, [3, 1], [5000, 4100], True),
+    ("f16", 6, 2, 96, [40], [40 + 6000], True),
+    ("bf16", 2, 1, 128, [260], [3000], False),
+    ("f16", 2, 1, 40, [100, 1], [2100, 6000], True),
+])
+def test_packed_keys_cut_into_parts(dev, dtype, heads, kv_heads, size, new, keys, causal):
+    """Few rows and many keys: the call is cut over the keys and joined; rows of no sequence stay as they were."""
+    torch = torch_()
+    dt = dtype_of(dtype)
+    total = sum(new) + 3
+    q = randn(1, total, heads, size, dtype=dt)
+    k, v = randn(2, sum(keys), kv_heads, size, dtype=dt), randn(3, sum(keys), kv_heads, size, dtype=dt)
+    out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device="cuda")
+    qo, ko = i32([2 + n for n in sums(new)]), i32(sums(keys))
+    assert dev.attention_packed_workspace(q, k, qo) > 0
+    assert dev.attention_packed(q, k, v, qo, ko, out, causal=causal, lse=lse, workspace=packed_space(dev, q, k, qo),
+                                stream=here())
+    torch.cuda.synchronize()
+    check_packed(q, k, v, new, keys, causal, size ** -0.5, out, lse, start=(2, 0))
+    for t in (out, lse):
+        assert (t[:2] == 7.0).all() and (t[total - 1:] == 7.0).all()
+    dev.status()
+
+
+@pytest.mark.parametrize("size,keys", [(128, 300), (64, 300), (128, 6000)])
+def test_packed_masked_keys_that_are_not_finite(dev, size, keys):
+    """Keys and values behind the causal border are infinite or NaN: the queries before them do not see them, and those
+    at and after them do."""
+    torch = torch_()
+    new, at = 40, keys - 17
+    q, k, v = randn(1, new, 4, size, dtype=torch.float16), *(randn(i, keys, 2, size, dtype=torch.float16) for i in (2, 3))
+    k[at], v[at, 0], v[at + 3, 1, 5] = math.nan, math.inf, math.nan
+    out, lse = torch.zeros_like(q), torch.zeros(new, 4, device="cuda")
+    qo, ko = i32([0, new]), i32([0, keys])
+    assert dev.attention_packed(q, k, v, qo, ko, out, lse=lse, workspace=packed_space(dev, q, k, qo), stream=here())
+    torch.cuda.synchronize()
+    seen = new - 17  # the first query that sees key `at`
+    import dev_reference as R
+
+    want = R.attention(q[:seen], k[:at], v[:at], size ** -0.5, visible(new, keys, True)[:seen, :at], q.dtype)
+    R.check(out[:seen], want[0], want[2], "out")
+    R.check(lse[:seen], want[1], want[3], "lse")
+    assert torch.isnan(out[seen:]).all() and torch.isnan(lse[seen:]).all()
+    # Values alone: only the channels that they reach.
+    k[at] = 0.5
+    v[at, 0] = 1.0
+    assert dev.attention_packed(q, k, v, qo, ko, out, lse=lse, workspace=packed_space(dev, q, k, qo), stream=here())
+    torch.cuda.synchronize()
+    bad = torch.isnan(out)
+    assert bad[seen + 3:, 2:, 5].all()
+    bad[seen + 3:, 2:, 5] = False
+    assert not bad.any()
+    check_packed(q[:seen + 3], k[:at + 3], v[:at + 3], [seen + 3], [at + 3], True, size ** -0.5, out[:seen + 3], lse[:seen + 3])
+
+
+def test_packed_broadcast_heads_and_offsets_beyond_32_bits(dev):
+    """K and V expanded over heads (stride 0) are read in place or declined; a cache whose token stride passes 2^31
+    elements over its length is read where it lies."""
+    torch = torch_()
+    q = randn(1, 50, 4, 64, dtype=torch.float16)
+    k1, v1 = randn(2, 70, 1, 64, dtype=torch.float16), randn(3, 70, 1, 64, dtype=torch.float16)
+    k, v = k1.expand(70, 4, 64), v1.expand(70, 4, 64)
+    out, lse = torch.full_like(q, 7.0), torch.zeros(50, 4, device="cuda")
+    qo, ko = i32([0, 50]), i32([0, 70])
+    if dev.attention_packed(q, k, v, qo, ko, out, lse=lse, workspace=packed_space(dev, q, k, qo), stream=here()):
+        torch.cuda.synchronize()
+        check_packed(q, k, v, [50], [70], True, 0.125, out, lse)
+    else:
+        assert (out == 7.0).all()
+    store = torch.zeros(70 * (1 << 26), dtype=torch.float16, device="cuda")
+    far = store.as_strided((70, 1, 64), (1 << 26, 64, 1))
+    far.copy_(k1)
+    assert dev.attention_packed(q, far, v1, qo, ko, out, lse=lse, workspace=packed_space(dev, q, far, qo), stream=here())
+    torch.cuda.synchronize()
+    check_packed(q, far, v1, [50], [70], True, 0.125, out, lse)
+
+
+def test_shared_offsets_beyond_32_bits(dev):
+    torch = torch_()
+    store = torch.zeros(2 * (1 << 31) + 4096, dtype=torch.float16, device="cuda")
+    sk = store.as_strided((3, 30, 1, 64), ((1 << 31), 64, 64, 1))
+    sk.copy_(randn(1, 3, 30, 1, 64, dtype=torch.float16))
+    sv, q = randn(2, 3, 30, 1, 64, dtype=torch.float16), randn(3, 3, 2, 64, dtype=torch.float16)
+    pk, pv = randn(4, 10, 1, 64, dtype=torch.float16), randn(5, 10, 1, 64, dtype=torch.float16)
+    out, lse = torch.zeros_like(q), torch.zeros(3, 2, device="cuda")
+    assert dev.attention_shared(q, pk, pv, sk, sv, i32([30, 7, 22]), out, lse=lse, workspace=shared_space(dev, q, pk, sk),
+                                stream=here())
+    torch.cuda.synchronize()
+    check_shared(q, pk, pv, sk, sv, [30, 7, 22], 0.125, out, lse)
+
+
+def test_wrong_offsets_and_lengths_stay_in_bounds(dev):
+    """Offsets that decrease or pass the arrays, and lengths beyond the capacity, are clamped; the guard rows hold."""
+    torch = torch_()
+    q, k, v = (randn(i, 60, 2, 64, dtype=torch.float16) for i in range(3))
+    out = torch.full((64, 2, 64), 7.0, dtype=torch.float16, device="cuda")
+    for qo, ko in (([0, 50, 20, 90], [0, 80, -5, 60]), ([-3, 10, 10, 60], [0, 10, 70, 65]), ([60, 0, 60, 60], [60, 0, 0, 60])):
+        assert dev.attention_packed(q, k, v, i32(qo), i32(ko), out[2:62], stream=here(),
+                                    workspace=packed_space(dev, q, k, i32(qo)))
+    torch.cuda.synchronize()
+    assert (out[:2] == 7.0).all() and (out[62:] == 7.0).all()
+    sk = randn(4, 60, 9, 2, 64, dtype=torch.float16)
+    lens = i32([40, -3] * 30)
+    lse = torch.zeros(60, 2, device="cuda")
+    assert dev.attention_shared(q, k, v, sk, sk, lens, out[2:62], lse=lse, workspace=shared_space(dev, q, k, sk), stream=here())
+    torch.cuda.synchronize()
+    check_shared(q, k, v, sk, sk, [9, 0] * 30, 0.125, out[2:62], lse)
+    x = randn(5, 4, 100, dtype=torch.float32)
+    y = torch.full((6, 100), 7.0, device="cuda")
+    assert dev.adjust_logits(x, y[1:5], None, history=i32([5, 6, 7]), history_offsets=i32([-2, 3, 1, 9, 2]),
+                             bias_tokens=i32([1]), bias_values=torch.ones(1, device="cuda"), bias_offsets=i32([0, 5, -1, 1, 1]),
+                             stream=here())
+    torch.cuda.synchronize()
+    assert (y[0] == 7.0).all() and (y[5] == 7.0).all()
+    dev.status()
+
+
+# ----------------------------------------------------------- streams and graphs ----
+
+
+def test_streams_none_two_at_once_and_threads(dev):
+    """The backend's own stream; two streams with a workspace each; two host threads."""
+    import threading
+
+    torch = torch_()
+    q, k, v = randn(1, 30, 8, 128, dtype=torch.bfloat16), *(randn(i, 9000, 1, 128, dtype=torch.bfloat16) for i in (2, 3))
+    qo, ko = i32([0, 30]), i32([0, 9000])
+    outs = [torch.zeros_like(q) for _ in range(5)]
+    spaces = [packed_space(dev, q, k, qo) for _ in range(5)]
+    torch.cuda.synchronize()
+    assert dev.attention_packed(q, k, v, qo, ko, outs[0], workspace=spaces[0])  # the backend's own stream
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for i, s in enumerate(streams):
+        assert dev.attention_packed(q, k, v, qo, ko, outs[1 + i], workspace=spaces[1 + i], stream=s.cuda_stream)
+
+    def work(i):
+        for _ in range(20):
+            assert dev.attention_packed(q, k, v, qo, ko, outs[3 + i], workspace=spaces[3 + i], stream=streams[i].cuda_stream)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    dev.status()  # waits for the device
+    for o in outs[1:]:
+        assert torch.equal(o, outs[0])
+
+
+def test_a_decode_step_of_the_three_operators_captured_and_replayed(dev):
+    """Two prompts prefilled in one packed call, then decode steps of both on the shared prefix with their logits
+    adjusted, captured once and replayed with other lengths, tokens and histories in the same buffers."""
+    import dev_reference as R
+
+    torch = torch_()
+    heads, kv_heads, size, prefix, cap, vocab, n = 4, 2, 64, 300, 50, 2000, 6
+    dt = torch.bfloat16
+    # Prefill: the shared prompt and one more prompt, packed.
+    pq, pk, pv = randn(1, prefix + 40, heads, size, dtype=dt), *(randn(i, prefix + 40, kv_heads, size, dtype=dt) for i in (2, 3))
+    off = i32([0, prefix, prefix + 40])
+    pout, plse = torch.zeros_like(pq), torch.zeros(prefix + 40, heads, device="cuda")
+    assert dev.attention_packed(pq, pk, pv, off, off, pout, lse=plse, workspace=packed_space(dev, pq, pk, off), stream=here())
+    torch.cuda.synchronize()
+    check_packed(pq, pk, pv, [prefix, 40], [prefix, 40], True, 0.125, pout, plse)
+
+    # Decode: n sessions on the first prompt's keys.
+    k0, v0 = pk[:prefix], pv[:prefix]
+    sk, sv = (randn(i, n, cap, kv_heads, size, dtype=dt) for i in (4, 5))
+    q, lens = torch.zeros(n, heads, size, dtype=dt, device="cuda"), i32([0] * n)
+    out, lse = torch.zeros_like(q), torch.zeros(n, heads, device="cuda")
+    head = randn(6, heads * size, vocab, dtype=dt)
+    logits, adjusted, tokens = (torch.zeros(n, vocab, dtype=dt, device="cuda"), torch.zeros(n, vocab, dtype=dt, device="cuda"),
+                                i32([0] * n))
+    history, hoff = i32([0] * 60), i32([0] * (n + 1))
+    rep, pres, freq = (torch.full((n,), x, device="cuda") for x in (1.3, 0.2, 0.1))
+    space = shared_space(dev, q, k0, sk)
+
+    def step():
+        stream = here()
+        assert dev.attention_shared(q, k0, v0, sk, sv, lens, out, lse=lse, workspace=space, stream=stream)
+        torch.mm(out.view(n, -1), head, out=logits)
+        assert dev.adjust_logits(logits, adjusted, tokens, history=history, history_offsets=hoff, repetition=rep,
+                                 presence=pres, frequency=freq, stream=stream)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    rng = random.Random(3)
+    for turn in range(3):
+        own = [rng.randint(0, cap) for _ in range(n)]
+        hist = [[rng.randrange(vocab) for _ in range(rng.randint(0, 10))] for _ in range(n)]
+        q.copy_(randn(10 + turn, n, heads, size, dtype=dt))
+        lens.copy_(i32(own))
+        flat = [t for h in hist for t in h]
+        history[:len(flat)].copy_(i32(flat) if flat else history[:0])
+        hoff.copy_(i32(sums([len(h) for h in hist])))
+        graph.replay()
+        torch.cuda.synchronize()
+        check_shared(q, k0, v0, sk, sv, own, 0.125, out, lse)
+        for r in range(n):
+            y, tol32, tol = R.logits(logits[r].cpu(), hist[r], 0, np.float32(1.3).item(), np.float32(0.2).item(),
+                                     np.float32(0.1).item(), [], None, dt)
+            R.check(adjusted[r].cpu(), y, tol, f"turn {turn} row {r}")
+            assert y[int(tokens[r])] + 2 * tol32.max() >= y.max()
+    dev.status()
+
+
+def test_results_do_not_change_from_call_to_call(dev):
+    torch = torch_()
+    q, k, v = randn(1, 300, 16, 128, dtype=torch.float16), *(randn(i, 5000, 2, 128, dtype=torch.float16) for i in (2, 3))
+    qo, ko = i32([0, 100, 300]), i32([0, 2000, 5000])
+    outs = []
+    for _ in range(4):
+        out, lse = torch.zeros_like(q), torch.zeros(300, 16, device="cuda")
+        assert dev.attention_packed(q, k, v, qo, ko, out, lse=lse, workspace=packed_space(dev, q, k, qo), stream=here())
+        sout, slse = torch.zeros(20, 16, 128, dtype=q.dtype, device="cuda"), torch.zeros(20, 16, device="cuda")
+        sk = k[:4000].view(20, 200, 2, 128)
+        assert dev.attention_shared(q[:20], k, v, sk, sk, i32(list(range(20))), sout, lse=slse,
+                                    workspace=shared_space(dev, q[:20], k, sk), stream=here())
+        x = q[:40].float().reshape(40, -1)
+        y, t = torch.zeros_like(x), i32([0] * 40)
+        assert dev.adjust_logits(x, y, t, history=i32([3, 3, 9] * 40), history_offsets=i32([3 * i for i in range(41)]),
+                                 frequency=torch.ones(40, device="cuda"), stream=here())
+        torch.cuda.synchronize()
+        outs.append((out, lse, sout, slse, y, t))
+    for other in outs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(outs[0], other))
+
+
+@pytest.mark.parametrize("rows,vocab", [(160, 5000), (160, 70001), (40, 33000)])
+def test_logits_more_rows_than_the_gpu_has_sms(dev, rows, vocab):
+    adjust_case(dev, "bf16", rows, vocab, 21, hist_max=30)
+
+
+def test_logits_more_tokens_than_slots(dev):
+    """A history and biases that touch more tokens than a CTA's table holds, in one row of several."""
+    adjust_case(dev, "f32", 3, 9000, 22, hist_max=30000)
+    torch = torch_()
+    x = randn(1, 200, 9000, dtype=torch.float32)
+    every = torch.arange(9000, dtype=torch.int32, device="cuda")
+    y, t = torch.zeros_like(x), i32([0] * 200)
+    # Row 7 biases every token twice (the later entry counts) and lists every token in its history.
+    off = i32([0] * 8 + [9000] * 193)
+    assert dev.adjust_logits(x, y, t, history=every, history_offsets=off, presence=torch.full((200,), 0.5, device="cuda"),
+                             bias_tokens=torch.cat([every, every]), bias_offsets=i32([0] * 8 + [18000] * 193),
+                             bias_values=torch.cat([torch.full((9000,), 99.0, device="cuda"), every.float() / 64]), stream=here())
+    torch.cuda.synchronize()
+    want = x.clone()
+    want[7] = (x[7] - 0.5) + every.float() / 64
+    assert torch.equal(y, want) and torch.equal(t.long(), want.argmax(-1))
