@@ -704,13 +704,6 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
         }
 #pragma unroll
         for (int e = 0; e < N; ++e) v[e] *= inv;
-        uint64_t zero = 0;  // stays 0 while all are finite
-#pragma unroll
-        for (int e = 0; e < N; e += 2)
-          if (e < a.head_size - from) zero = ptx::fma2(ptx::pair(v[e], v[e + 1]), 0, zero);
-        float z0, z1;
-        ptx::unpair(zero, z0, z1);
-        return !(z0 == 0.0f && z1 == 0.0f);
       };
       // Keys that the products took in, masked ones among them: whole steps of 16, cleared behind the last that any row sees.
       const int last_key =
@@ -720,11 +713,20 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
 #pragma unroll 1
         for (int from = 0; from < a.head_size; from += D / 2) {
           float v[D / 2];
-          const bool odd = take(from, std::integral_constant<int, D / 2>{}, v);
+          take(from, std::integral_constant<int, D / 2>{}, v);
+          unsigned bad = 0;
+          if (a.causal) {
+            uint64_t zero = 0;  // stays 0 while all are finite
+#pragma unroll
+            for (int e = 0; e < D / 2; e += 2)
+              if (from + e < a.head_size) zero = ptx::fma2(ptx::pair(v[e], v[e + 1]), 0, zero);
+            float z0, z1;
+            ptx::unpair(zero, z0, z1);
+            bad = __ballot_sync(0xffffffffu, live && !(z0 == 0.0f && z1 == 0.0f));
+          }
 #pragma unroll
           for (int e = 0; e < D / 2; e += 4)
             put(e / 4, __float_as_uint(v[e]), __float_as_uint(v[e + 1]), __float_as_uint(v[e + 2]), __float_as_uint(v[e + 3]));
-          const unsigned bad = __ballot_sync(0xffffffffu, odd && live && a.causal);
           if (bad) {
             __syncwarp();
             mend_rows<T, true>(a, bad, key0, last_key, sees, base, inv, t, h, k0, kvh, from, D / 2, stage, kRowBytes);
@@ -733,12 +735,19 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
         }
       } else {
         float v[D];
-        const bool odd = take(0, std::integral_constant<int, D>{}, v);
+        take(0, std::integral_constant<int, D>{}, v);
+        unsigned x[D / 2], bad = 0;
 #pragma unroll
-        for (int e = 0; e < D; e += 8)
-          put(e / 8, ptx::pack16<BF16>(v[e], v[e + 1]), ptx::pack16<BF16>(v[e + 2], v[e + 3]),
-              ptx::pack16<BF16>(v[e + 4], v[e + 5]), ptx::pack16<BF16>(v[e + 6], v[e + 7]));
-        const unsigned bad = __ballot_sync(0xffffffffu, odd && live && a.causal);
+        for (int e = 0; e < D / 2; ++e) x[e] = ptx::pack16<BF16>(v[2 * e], v[2 * e + 1]);
+        if (a.causal) {
+          unsigned zero = 0;  // stays 0 while all are finite
+#pragma unroll
+          for (int e = 0; e < D / 2; ++e)
+            if (2 * e < a.head_size) zero = ptx::times_zero<BF16>(x[e], zero);
+          bad = __ballot_sync(0xffffffffu, live && (zero & 0x7fff7fffu) != 0);
+        }
+#pragma unroll
+        for (int e = 0; e < D / 2; e += 4) put(e / 4, x[e], x[e + 1], x[e + 2], x[e + 3]);
         if (bad) {
           __syncwarp();
           mend_rows<T, false>(a, bad, key0, last_key, sees, base, inv, t, h, k0, kvh, 0, D, stage, kRowBytes);

@@ -207,5 +207,16 @@ __device__ __forceinline__ unsigned pack16(float lo, float hi) {
   return r;
 }
 
+// x * 0 + y of two 16-bit floats each: y unless a part of x is infinite or NaN.
+template <bool BF16>
+__device__ __forceinline__ unsigned times_zero(unsigned x, unsigned y) {
+  unsigned r;
+  if (BF16)
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(y));
+  else
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(y));
+  return r;
+}
+
 }  // namespace ptx
 }  // namespace fa
