@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 
 #include "dev_ops.h"
 #include "dev_ptx.cuh"
@@ -27,10 +28,11 @@ void need(bool ok, const char* what) {
   if (!ok) throw Error(kErrArgument, what);
 }
 
-// Strides in elements of two bytes: every row must start on 16 bytes.
-bool strides16(const int64_t* s, int n) {
-  for (int i = 0; i < n; ++i)
-    if (s[i] % 8 != 0) return false;
+// Strides in elements of two bytes: every row must start on 16 bytes (a
+// dimension of length one has a single start).
+bool strides16(const int64_t* s, std::initializer_list<int64_t> extents) {
+  for (int64_t n : extents)
+    if (*s++ % 8 != 0 && n > 1) return false;
   return true;
 }
 
@@ -1248,8 +1250,9 @@ int check_attention_packed(const fa_attention_packed_args* a) {
   const int64_t extents[2] = {a->total_q, a->heads};
   need(apart(a->out_stride, extents, a->head_size), "rows of out overlap");
   if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out)) return kDeclined;
-  if (!strides16(a->q_stride, 2) || !strides16(a->k_stride, 2) || !strides16(a->v_stride, 2) ||
-      !strides16(a->out_stride, 2))
+  const auto rows = {a->total_q, (int64_t)a->heads}, keys = {a->total_k, (int64_t)a->kv_heads};
+  if (!strides16(a->q_stride, rows) || !strides16(a->k_stride, keys) || !strides16(a->v_stride, keys) ||
+      !strides16(a->out_stride, rows))
     return kDeclined;
   need(a->workspace_bytes >= attention_packed_workspace(a->total_q, a->total_k, a->sequences, a->heads, a->kv_heads,
                                                         a->head_size) &&
@@ -1281,8 +1284,10 @@ int check_attention_shared(const fa_attention_shared_args* a) {
   if (!aligned16(a->q) || !aligned16(a->prefix_k) || !aligned16(a->prefix_v) || !aligned16(a->suffix_k) ||
       !aligned16(a->suffix_v) || !aligned16(a->out))
     return kDeclined;
-  if (!strides16(a->q_stride, 2) || !strides16(a->prefix_k_stride, 2) || !strides16(a->prefix_v_stride, 2) ||
-      !strides16(a->suffix_k_stride, 3) || !strides16(a->suffix_v_stride, 3) || !strides16(a->out_stride, 2))
+  const int64_t n = a->sequences, kv = a->kv_heads;
+  const auto rows = {n, (int64_t)a->heads}, prefix = {a->prefix_len, kv}, suffix = {n, a->suffix_capacity, kv};
+  if (!strides16(a->q_stride, rows) || !strides16(a->prefix_k_stride, prefix) || !strides16(a->prefix_v_stride, prefix) ||
+      !strides16(a->suffix_k_stride, suffix) || !strides16(a->suffix_v_stride, suffix) || !strides16(a->out_stride, rows))
     return kDeclined;
   need(a->workspace_bytes >= attention_shared_workspace(a->prefix_len, a->suffix_capacity, a->sequences, a->heads,
                                                         a->kv_heads, a->head_size) &&

@@ -386,6 +386,17 @@ int check_logits(const fa_logits_args* a) {
   if (a->rows == 0) return kHandled;
   need(a->logits && a->out, "null logits or out");
   need(a->rows == 1 || (a->logits_stride >= a->vocab && a->out_stride >= a->vocab), "rows overlap: stride below vocab");
+  // In place, or apart: rows of out on other rows of the logits would be read changed.
+  const int64_t size = a->dtype == FA_DTYPE_F32 ? 4 : 2;
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a->logits), y = reinterpret_cast<uintptr_t>(a->out);
+  const uint64_t xn = ((a->rows - 1) * a->logits_stride + a->vocab) * size, yn = ((a->rows - 1) * a->out_stride + a->vocab) * size;
+  bool apart = x + xn <= y || y + yn <= x;
+  if (!apart && a->rows > 1 && a->logits_stride == a->out_stride) {  // columns of one array side by side
+    const int64_t stride = a->logits_stride * size, off = ((int64_t)(y - x) % stride + stride) % stride;
+    apart = off >= a->vocab * size && stride - off >= a->vocab * size;
+  }
+  need(apart || (x == y && (a->rows == 1 || a->logits_stride == a->out_stride)),
+       "out overlaps logits and is not the same rows");
   need(a->logits_stride >= 0 && a->out_stride >= 0 && a->mask_stride >= 0, "negative stride");
   need(!a->history || a->history_offsets, "history without history_offsets");
   need(!a->bias_tokens || (a->bias_values && a->bias_offsets), "bias_tokens without bias_values or bias_offsets");

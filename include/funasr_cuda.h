@@ -358,10 +358,13 @@ int fa_dev_status(fa_backend* backend);
  * head h / (heads / kv_heads).  Scores, softmax statistics and sums are 32-bit;
  * the probabilities are rounded to the type of v for their product with it.
  * Rows of out and lse outside q_offsets[0] .. q_offsets[sequences] stay as they were.
+ * Keys that a query does not see have no part in its result, NaN and infinities
+ * among them included.  out and lse must not overlap the inputs.
  * Limits (else FA_DECLINED): FA_DTYPE_F16 or FA_DTYPE_BF16; head_size a multiple
- * of 8 up to 128; heads / kv_heads up to 64; every base address and stride a
- * multiple of 16 bytes (the stride of a dimension of length one counts too); total_q * heads
- * below 2^31, total_k below 2^30. */
+ * of 8 up to 128; heads / kv_heads up to 64; every base address, and every stride
+ * of a dimension longer than one, a multiple of 16 bytes;
+ * total_q * heads below 2^31, total_k below 2^30; scale above 0 (else
+ * FA_ERR_ARGUMENT). */
 typedef struct fa_attention_packed_args {
   const void* q;            /* [total_q x heads x head_size] */
   const void* k;            /* [total_k x kv_heads x head_size] */
@@ -382,7 +385,9 @@ typedef struct fa_attention_packed_args {
   int32_t reserved;         /* 0 */
 } fa_attention_packed_args;
 int fa_dev_attention_packed(fa_backend* backend, const fa_attention_packed_args* args, void* stream);
-/* Bytes of workspace a call of these sizes needs (0: none). */
+/* Bytes of workspace a call of these sizes needs (0: none).  Smaller calls can need
+ * more than larger ones, which leave no SM idle: the maximum over a program's
+ * sizes serves them all. */
 int64_t fa_dev_attention_packed_workspace(int64_t total_q, int64_t total_k, int sequences, int heads, int kv_heads,
                                           int head_size);
 
@@ -424,7 +429,8 @@ int64_t fa_dev_attention_shared_workspace(int64_t prefix_len, int64_t suffix_cap
  *     x - (frequency * n + presence)            tokens that its generated part holds n > 0 times
  *     x + bias                                  tokens of its bias list (the last entry of a token counts)
  *     -inf                                      tokens whose bit in its mask is 0
- * out gets the result in the type of the logits (it may be the logits themselves);
+ * out gets the result in the type of the logits (it may be the logits themselves,
+ * with their stride, or must not overlap them);
  * tokens gets the lowest index of the row's largest 32-bit value, -1 when no
  * value is above -inf (NaN is above nothing).  A row's history is history_offsets[r] ..
  * history_offsets[r+1]; its first prompt_lens[r] tokens are the prompt, the rest
