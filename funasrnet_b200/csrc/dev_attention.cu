@@ -789,6 +789,9 @@ struct RowsArgs {
   void* out = nullptr;            // the result (part_o == nullptr), or parts:
   long long out_seq = 0, out_head = 0;
   float* lse = nullptr;
+  // merge: the splits of a row form a cluster, which joins them into the result;
+  // else with part_o they leave parts.
+  int merge = 0;
   float* part_o = nullptr;        // [splits x sequences x heads x head_size]
   float* part_lse = nullptr;      // [splits x sequences x heads]
   int wait = 0;                   // the launch before this one must be over when this one is
@@ -808,7 +811,8 @@ struct RowsLayout {
   static constexpr int kMisc = kBars + 8 * 3 * kStages;
   static constexpr int kTotal = kMisc + 16 + 1024;
   static constexpr int kOut = kRowWarps * kRowHeads * (D + 4) * 4;  // the warps' sums, over the ring
-  static_assert(kOut + 2 * kRowWarps * kRowHeads * 4 <= kBars, "joining the warps");
+  static constexpr int kFinal = kOut + 2 * kRowWarps * kRowHeads * 4;  // the CTA's sums, for its cluster
+  static_assert(kFinal + (kRowHeads * D + 2 * kRowHeads) * 4 <= kBars, "joining the warps");
 };
 
 // D (m16n8) += A (m16k16) x B (k16n8), f32 accumulator.
@@ -859,12 +863,11 @@ __global__ void __launch_bounds__(kRowThreads, 3) attention_rows_kernel(const Ro
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::kMisc);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   unsigned id = blockIdx.x;
+  const int split = id % a.splits;  // a merging call: the CTA's rank in its cluster
+  id /= a.splits;
   const int kvh = id % a.kv_heads;
   id /= a.kv_heads;
-  const int block = id % a.blocks;
-  id /= a.blocks;
-  const int split = id % a.splits;
-  const int seq = id / a.splits;
+  const int block = id % a.blocks, seq = id / a.blocks;
   const int head0 = kvh * a.group + block * kRowHeads, n_heads = min(kRowHeads, a.group - block * kRowHeads);
   ptx::griddep_launch();
   if (threadIdx.x == 0) {
@@ -1026,8 +1029,11 @@ __global__ void __launch_bounds__(kRowThreads, 3) attention_rows_kernel(const Ro
             make_float2(o[4 * h + r][i], o[4 * h + r][2 + i]);
   }
   asm volatile("bar.sync 1, %0;" ::"n"(32 * kRowWarps) : "memory");
-  if (*abort_flag) return;
-  for (int e = threadIdx.x; e < n_heads * (D / 4); e += 32 * kRowWarps) {
+  float* fin_o = reinterpret_cast<float*>(sm + L::kFinal);  // [head][D]: sums relative to the head's maximum
+  float* fin_top = fin_o + kRowHeads * D;                   // the maximum (log2), and the sum of exponentials
+  float* fin_sum = fin_top + kRowHeads;
+  const bool failed = *abort_flag != 0;
+  for (int e = threadIdx.x; e < n_heads * (D / 4) && !failed; e += 32 * kRowWarps) {
     const int h = e / (D / 4), ch0 = (e % (D / 4)) * 4;
     float top = -INFINITY, sum = 0.0f, v[4] = {};
 #pragma unroll
@@ -1042,6 +1048,14 @@ __global__ void __launch_bounds__(kRowThreads, 3) attention_rows_kernel(const Ro
       v[1] = fmaf(f, x.y, v[1]);
       v[2] = fmaf(f, x.z, v[2]);
       v[3] = fmaf(f, x.w, v[3]);
+    }
+    if (a.merge) {
+      *reinterpret_cast<float4*>(fin_o + h * D + ch0) = make_float4(v[0], v[1], v[2], v[3]);
+      if (ch0 == 0) {
+        fin_top[h] = top * c;
+        fin_sum[h] = sum;
+      }
+      continue;
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
@@ -1060,6 +1074,37 @@ __global__ void __launch_bounds__(kRowThreads, 3) attention_rows_kernel(const Ro
       else if (a.lse) a.lse[row] = lse;
     }
   }
+  if (!a.merge) return;
+
+  // ---- join the cluster's CTAs, a share of the row each ----
+  ptx::cluster_arrive();
+  ptx::cluster_wait();
+  for (int e = threadIdx.x * a.splits + split; e < n_heads * (D / 4) && !failed; e += 32 * kRowWarps * a.splits) {
+    const int h = e / (D / 4), ch0 = (e % (D / 4)) * 4;
+    const long long row = (long long)seq * a.heads + head0 + h;
+    float top = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ptx::remote_f32(ptx::map_rank(ptx::saddr(fin_top + h), s)));
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, v[4] = {};
+    for (int s = 0; s < a.splits; ++s) {
+      const float f = ptx::ex2(ptx::remote_f32(ptx::map_rank(ptx::saddr(fin_top + h), s)) - base);
+      const float4 x = ptx::remote_f32x4(ptx::map_rank(ptx::saddr(fin_o + h * D + ch0), s));
+      sum = fmaf(f, ptx::remote_f32(ptx::map_rank(ptx::saddr(fin_sum + h), s)), sum);
+      v[0] = fmaf(f, x.x, v[0]);
+      v[1] = fmaf(f, x.y, v[1]);
+      v[2] = fmaf(f, x.z, v[2]);
+      v[3] = fmaf(f, x.w, v[3]);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = sum == 0.0f ? 0.0f : v[i] * inv;
+    if (ch0 < a.head_size)
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + seq * a.out_seq + (head0 + h) * a.out_head + ch0) =
+          make_uint2(ptx::pack16<BF16>(v[0], v[1]), ptx::pack16<BF16>(v[2], v[3]));
+    if (ch0 == 0 && a.lse) a.lse[row] = base * 0.6931471805599453f + logf(sum);
+  }
+  ptx::cluster_arrive();
+  ptx::cluster_wait();  // the others' sums stay until they were read
 }
 
 // Joins the parts of a row: lse = log sum_s e^lse_s, out = sum_s e^(lse_s - lse) o_s,
@@ -1165,20 +1210,27 @@ void encode_suffix(CUtensorMap* m, int dtype, const void* base, int head_size, i
   encode_tensor_map(m, map_type(dtype), 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Launches, with `after` behind a kernel of this file that signals its dependents early.
+// Launches in clusters of `cluster` CTAs, with `after` behind a kernel of this file that signals its dependents early.
 template <typename... P, typename... A>
-void launch_after(void (*kernel)(P...), unsigned grid, unsigned block, int shared, bool after, cudaStream_t stream,
-                  A&&... args) {
+void launch_after(void (*kernel)(P...), unsigned grid, unsigned block, int shared, bool after, int cluster,
+                  cudaStream_t stream, A&&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = shared;
   cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = after ? 1 : 0;
+  cudaLaunchAttribute attrs[2];
+  if (after) {
+    attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attrs[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attrs[cfg.numAttrs].val.clusterDim.x = cluster;
+    attrs[cfg.numAttrs].val.clusterDim.y = attrs[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  cfg.attrs = attrs;
   FA_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...));
 }
 
@@ -1207,7 +1259,7 @@ void launch_join(const JoinArgs& j, int dtype, cudaStream_t stream) {
   const bool bf16 = dtype == FA_DTYPE_BF16;
   launch_after(w > 1 ? (bf16 ? join_kernel<__nv_bfloat16, kJoinWarps> : join_kernel<__half, kJoinWarps>)
                      : (bf16 ? join_kernel<__nv_bfloat16, 1> : join_kernel<__half, 1>),
-               grid, 32 * kJoinWarps, 0, true, stream, j);
+               grid, 32 * kJoinWarps, 0, true, 1, stream, j);
 }
 
 // Query rows as (channel, head of the group, KV head, token).
@@ -1221,6 +1273,7 @@ void encode_q(CUtensorMap* m, int dtype, const void* base, int head_size, int gr
 }
 
 constexpr int kSms = 148;
+constexpr int kMaxCluster = 8;   // splits of attention_rows_kernel that a cluster joins
 constexpr double kShort = 8.0;   // key tiles up to which a CTA takes one tile of rows
 constexpr double kStepUs = 1.8;  // one key tile against two tiles of rows
 
@@ -1332,12 +1385,18 @@ struct SharedPlan {
   bool tc = false;      // the prefix on the tensor cores, for all sequences at once
   int tc_splits = 0;    // its key ranges
   int row_splits = 1;   // key ranges of attention_rows_kernel
-  int parts() const { return tc || row_splits > 1 ? tc_splits + row_splits : 0; }
+  // Who brings the parts together: nobody (there is one), attention_rows_kernel
+  // with its splits in clusters, or a join_kernel.
+  enum { kOne, kMerge, kJoin } join = kOne;
+  int parts() const { return tc_splits + (join == kJoin ? row_splits : 0); }  // partial results in the workspace
 };
 SharedPlan shared_plan(int64_t prefix_len, int64_t capacity, int sequences, int heads, int kv_heads, int head_size) {
   SharedPlan p;
   const int group = heads / kv_heads;
-  p.tc = sequences >= 4 && prefix_len >= 256;
+  // Read by every sequence's CTAs on its own the prefix costs these bytes (of L2,
+  // mostly); the tensor-core kernel and what it leaves to join cost 15 to 20 us
+  // (thresholds of 40, 80 and 160 MB, measured over 60 calls: 9.5, 9.3, 9.2 us on average).
+  p.tc = (double)sequences * prefix_len * kv_heads * head_size * 4 > 1.6e8 && sequences >= 4;
   if (p.tc) {
     // The two kernels run side by side, the prefix's bound by its MMAs and the
     // own keys' by their bytes: as few CTAs for the prefix as let it end about
@@ -1350,8 +1409,18 @@ SharedPlan shared_plan(int64_t prefix_len, int64_t capacity, int sequences, int 
     p.tc_splits = (int)std::max<int64_t>(1, std::min<int64_t>(kSms / ctas, (tiles + each - 1) / each));
   }
   const int64_t ctas = (int64_t)sequences * kv_heads * ((group + kRowHeads - 1) / kRowHeads);
-  const int64_t stages = ((p.tc ? 0 : prefix_len) + capacity) / kStageKeys;
-  p.row_splits = (int)std::max<int64_t>(1, std::min<int64_t>((p.tc ? 8 : 2) * kSms / ctas, stages / 4));
+  const int64_t stages = ((p.tc ? 0 : prefix_len) + capacity + kStageKeys - 1) / kStageKeys;
+  // Without the prefix's parts a cluster joins the splits (a call of 19 sessions
+  // with up to 804 keys: 18.6 us uncut, 12.9 us in clusters); long rows with few
+  // CTAs are cut finer than a cluster, and a join_kernel is one launch more.
+  const int64_t wanted = std::max<int64_t>(1, std::min(3 * kSms / ctas, stages / 3));
+  if (!p.tc && wanted <= 2 * kMaxCluster) {
+    while (p.row_splits < kMaxCluster && 2 * p.row_splits <= wanted) p.row_splits *= 2;
+    p.join = p.row_splits > 1 ? SharedPlan::kMerge : SharedPlan::kOne;
+  } else {
+    p.row_splits = (int)std::max<int64_t>(1, std::min<int64_t>((p.tc ? 8 : 2) * kSms / ctas, stages / 4));
+    p.join = SharedPlan::kJoin;
+  }
   return p;
 }
 
@@ -1503,8 +1572,9 @@ void launch_attention_shared(const fa_attention_shared_args& a, int* err, cudaSt
   r.out_seq = a.out_stride[0];
   r.out_head = a.out_stride[1];
   r.lse = a.lse;
+  r.merge = plan.join == SharedPlan::kMerge;
   r.wait = plan.tc;
-  if (parts) {
+  if (plan.join == SharedPlan::kJoin) {
     r.part_o = part_o + plan.tc_splits * rows * a.head_size;
     r.part_lse = part_lse + plan.tc_splits * rows;
   }
@@ -1522,8 +1592,9 @@ void launch_attention_shared(const fa_attention_shared_args& a, int* err, cudaSt
   const bool bf16 = a.dtype == FA_DTYPE_BF16, small = a.head_size <= 64;
   launch_after(small ? (bf16 ? attention_rows_kernel<64, true> : attention_rows_kernel<64, false>)
                      : (bf16 ? attention_rows_kernel<128, true> : attention_rows_kernel<128, false>),
-               grid, kRowThreads, small ? RowsLayout<64>::kTotal : RowsLayout<128>::kTotal, plan.tc, stream, r, maps);
-  if (parts) {
+               grid, kRowThreads, small ? RowsLayout<64>::kTotal : RowsLayout<128>::kTotal, plan.tc, r.merge ? plan.row_splits : 1, stream,
+               r, maps);
+  if (plan.join == SharedPlan::kJoin) {
     JoinArgs j;
     j.tokens = a.sequences;
     j.heads = a.heads;

@@ -57,11 +57,6 @@ __device__ __forceinline__ Best warp_best(Best b) {
 
 __device__ __forceinline__ int clamp_off(int x, long long hi) { return (int)min((long long)max(x, 0), hi); }
 
-__device__ __forceinline__ void cluster_arrive() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // Writes `b` to `slot` of the cluster's first CTA and counts its bytes on that
 // CTA's barrier.
 __device__ __forceinline__ void send_best(Best b, Best* slot, uint64_t* bar) {
@@ -137,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, 2) adjust_logits_kernel(const fa_log
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       ptx::mbar_expect_tx(&arrived, (unsigned)(ranks * kWarps * sizeof(Best)));
     }
-    cluster_arrive();
+    ptx::cluster_arrive();
   }
   int h0 = 0, made = 0, h1 = 0, b0 = 0, b1 = 0;  // prompt [h0, made), generated [made, h1), biases [b0, b1)
   if (a.history) {
@@ -322,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 2) adjust_logits_kernel(const fa_log
     __syncthreads();
     if (warp != 0) return;
   } else {
-    cluster_wait();  // the first CTA's barrier is ready since its start
+    ptx::cluster_wait();  // the first CTA's barrier is ready since its start
     if ((threadIdx.x & 31) == 0) send_best(best, &from[rank * kWarps + warp], &arrived);
     if (rank != 0 || warp != 0) return;
     // The copies are on their way from CTAs that wait for nothing: bounded all the same.

@@ -106,7 +106,7 @@ BAD = [
     (shared, dict(suffix_lens=None), "null"),
     (shared, dict(out=None), "null"),
     (shared, dict(out_stride=(64, 128)), "overlap"),
-    (shared, dict(sequences=64, workspace_bytes=0), "workspace"),
+    (shared, dict(sequences=64, prefix_len=9000, workspace_bytes=0), "workspace"),
     (logits, dict(rows=-1), "rows"),
     (logits, dict(vocab=0), "vocab"),
     (logits, dict(logits=None), "null"),

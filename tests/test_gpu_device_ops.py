@@ -186,6 +186,12 @@ SHARED = [
     (8, 1, 112, 129, list(range(100, 230))),
     (3, 1, 24, 0, [0, 1, 2]),
     (8, 2, 128, 9000, [4000]),
+    (32, 4, 64, 5000, [0, 1, 70, 33] * 20),      # large enough together for the tensor cores, in several shapes
+    (14, 2, 96, 4003, [5] * 119 + [130]),
+    (64, 1, 128, 5001, [64, 65] * 50),
+    (6, 6, 40, 1200, [1, 2, 3] * 50),
+    (32, 8, 128, 6, list(range(217, 804, 31))),  # keys cut into parts that a cluster joins
+    (8, 1, 112, 6403, [47, 48, 0, 47]),          # into more parts than a cluster has
 ]
 
 
