@@ -199,7 +199,7 @@ __device__ __forceinline__ uint4 lds16(unsigned addr) {
 // the rows in `bad`: row r's lane has what it sees, its maximum (times the
 // scale's log2), 1 / sum, its query and its head.  The result goes to the row's
 // place in the stage, 4 channels a lane, from channel `from` on.
-template <typename T, bool kParts>
+template <typename T>
 __device__ __noinline__ void mend_rows(const TcArgs& a, unsigned bad, int first_key, int end_key, int sees, float base,
                                        float inv, long long token, int head, long long k0, int kvh, int from, int width,
                                        unsigned stage, int row_bytes) {
@@ -210,6 +210,7 @@ __device__ __noinline__ void mend_rows(const TcArgs& a, unsigned bad, int first_
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = (float)reinterpret_cast<const T*>(&u)[i];
   };
+#pragma unroll 1
   for (; bad; bad &= bad - 1) {
     const int r = __ffs(bad) - 1;
     const int seen = min(__shfl_sync(0xffffffffu, sees, r), end_key);
@@ -219,6 +220,7 @@ __device__ __noinline__ void mend_rows(const TcArgs& a, unsigned bad, int first_
     const T* k = static_cast<const T*>(a.k) + k0 * a.k_token + kvh * a.k_head;
     const T* v = static_cast<const T*>(a.v) + k0 * a.v_token + kvh * a.v_head;
     bool spoiled = false;
+#pragma unroll 1
     for (int j = max(seen, first_key); j < end_key; ++j) {
       float x[4] = {};
       if (on) load(v + j * a.v_token + c, x);
@@ -229,6 +231,7 @@ __device__ __noinline__ void mend_rows(const TcArgs& a, unsigned bad, int first_
     float o[4] = {}, qx[4] = {};
     const int cq = lane * 4;
     if (cq < a.head_size) load(q + cq, qx);
+#pragma unroll 1
     for (int j = first_key; j < seen; ++j) {
       float kx[4] = {}, vx[4] = {}, dot = 0.0f;
       if (cq < a.head_size) load(k + j * a.k_token + cq, kx);
@@ -245,9 +248,10 @@ __device__ __noinline__ void mend_rows(const TcArgs& a, unsigned bad, int first_
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] *= by;
-    const int chunk = kParts ? lane : lane / 2;
-    const unsigned at = stage + r * row_bytes + ((chunk ^ (r & 7)) << 4) + (kParts ? 0 : (lane & 1) * 8);
-    if (kParts)
+    const bool parts = a.part_o != nullptr;
+    const int chunk = parts ? lane : lane / 2;
+    const unsigned at = stage + r * row_bytes + ((chunk ^ (r & 7)) << 4) + (parts ? 0 : (lane & 1) * 8);
+    if (parts)
       asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(o[0]), "f"(o[1]), "f"(o[2]), "f"(o[3]) : "memory");
     else
       asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(ptx::pack16<kBf16>(o[0], o[1])),
@@ -383,11 +387,13 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
     // ---- the other copies ----
     if (lane == 0) {
       int n = min(ring, 1);
+#pragma unroll 1
       for (; n < ring; ++n) {
         if (n >= L::kStages && !ptx::wait_phase(&kv_empty[n % L::kStages], (n / L::kStages - 1) & 1, abort_flag, a.err, kAttnWaitFree)) break;
         load_kv(n);
       }
       // Copies in flight land before the CTA exits.
+#pragma unroll 1
       for (int s = max(0, n - L::kStages); s < n; ++s)
         ptx::wait_phase(&kv_full[s % L::kStages], (s / L::kStages) & 1, abort_flag, a.err, kAttnWaitLoad, false);
       if (cnt0 > 0) ptx::wait_phase(&q_full[0], 0, abort_flag, a.err, kAttnWaitLoad, false);
@@ -431,6 +437,7 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
             ptx::tc_mma_ss(s_at + b * kUnit, q_low + (((s >> 2) * L::kQHalf + (s & 3) * 32) >> 4),
                            k + (((s >> 2) * L::kHalf + (s & 3) * 32) >> 4), id_s, s > 0);
         } else {
+#pragma unroll 1
           for (int s = 0; s < k_s; ++s)
             ptx::tc_mma_ss(s_at + b * kUnit, q_low + (((s >> 2) * L::kQHalf + (s & 3) * 32) >> 4),
                            k + (((s >> 2) * L::kHalf + (s & 3) * 32) >> 4), id_s, s > 0);
@@ -445,6 +452,7 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
           for (int s = 0; s < kUnit / 16; ++s)
             ptx::tc_mma_ts(o_at, s_at + b * kUnit + s * 8, v + (s * 2048 >> 4), id_o, acc || s > 0);
         } else {
+#pragma unroll 1
           for (int s = 0; s < steps; ++s)
             ptx::tc_mma_ts(o_at, s_at + b * kUnit + s * 8, v + (s * 2048 >> 4), id_o, acc || s > 0);
         }
@@ -452,17 +460,6 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
       };
       auto release = [&](int st) {
         if (ok) ptx::tc_commit(&kv_empty[st]);
-      };
-      // Value rows behind the last key that a row sees are not the sequence's own,
-      // or masked for every row here: 0 x what they hold must stay 0.
-      auto clear_tail = [&](int key) {
-        const int most = min(max(end[0], end[1]) - key0 - key, L::kTileKeys), padded = (most + 15) / 16 * 16;
-        if (most >= padded) return;
-        uint8_t* v = sm + L::kKv + vs.st * L::kTile;
-        for (int c = 0; c < (padded - most) * 8; ++c)
-          for (int h = 0; h < L::kHalves; ++h)
-            *reinterpret_cast<uint4*>(v + h * L::kHalf + (most + c / 8) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       };
       auto steps_of = [&](int n) { return (min(end[w] - key0 - n * kUnit, kUnit) + 15) / 16; };
       if (cnt > 0) wait(&kv_full[0], 0, kAttnWaitLoad);
@@ -476,13 +473,13 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
           release(ks.st);
           ks.next();
         }
+#pragma unroll 1
         for (int n0 = 0; n0 < mine && ok; n0 += 2)
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
             const int n = n0 + b;
             if (!ok || n >= mine) continue;
             wait(&kv_full[vs.st], vs.ph, kAttnWaitLoad);
-            if (ok) clear_tail(n * kUnit);
             wait(&p_full[b], (n0 >> 1) & 1, kAttnWaitSoftmax);
             if (!ok) continue;
             values(b, steps_of(n), n > 0);
@@ -499,12 +496,12 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
         if (ok && mine > 1) scores(1);
         if (cnt > 0) release(0);
         ks.next();
+#pragma unroll 1
         for (int n0 = 0; n0 < cnt && ok; n0 += 2) {  // one V tile, and the K tile after its own
           // Waits, and releases below, also for tiles that only the other issuer uses:
           // one that ran ahead would release a slot's next use.
           wait(&kv_full[vs.st], vs.ph, kAttnWaitLoad);
           if (!ok) break;
-          if (n0 < mine) clear_tail(n0 * kUnit);
           if (n0 + 2 < cnt) wait(&kv_full[ks.st], ks.ph, kAttnWaitLoad);
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
@@ -541,7 +538,8 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
     const float c = a.scale_log2;
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
-    for (int n = 0; n < mine; ++n) {
+#pragma unroll 1
+    for (int n = 0; n < mine && ok; ++n) {
       ok = __all_sync(0xffffffffu,
                       ptx::wait_phase(&s_full[2 * w + (n & 1)], (n >> 1) & 1, abort_flag, a.err, kAttnWaitMma));
       if (!ok) break;
@@ -608,8 +606,7 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
             // O is at rest once the step before is in it.
             ok = __all_sync(0xffffffffu,
                             ptx::wait_phase(&pv_done[2 * w + ((n - 1) & 1)], ((n - 1) >> 1) & 1, abort_flag, a.err,
-                                            kAttnWaitMma));
-            if (!ok) break;
+                                            kAttnWaitMma));  // a failed wait ends the loop at the next one
             ptx::tc_fence_after();
             const float f = rise ? ptx::ex2((m - mx) * c) : 1.0f;
             if (rise) m = mx;
@@ -638,6 +635,22 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
         }
         ptx::tmem_st32(s_addr, p);
         l += sum[0] + sum[1];
+      }
+      // Value rows behind the last key that a row sees are not the sequence's own,
+      // or masked for every row here: 0 x what they hold must stay 0.  The step
+      // that takes some of them in clears them before it hands over.
+      const int most = max(end[0], end[1]) - key0 - n * kUnit;
+      if (most < kUnit && most % 16 != 0) {
+        const int v = 2 * (n * kUnit / L::kTileKeys) + 1, first = most + n * kUnit % L::kTileKeys;  // ring number, row
+        ok = __all_sync(0xffffffffu, ptx::wait_phase(&kv_full[v % L::kStages], (v / L::kStages) & 1, abort_flag, a.err,
+                                                     kAttnWaitLoad));
+        const unsigned at = sbase + L::kKv + v % L::kStages * L::kTile + first * 128;
+        for (int i = r; i < (16 - most % 16) * 8 * L::kHalves; i += kRows)
+          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at + i / 8 / L::kHalves * 128 +
+                                                                      i / 8 % L::kHalves * L::kHalf + (i & 7) * 16),
+                       "r"(0)
+                       : "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       ptx::tc_wait_st();
       ptx::tc_fence_before();
@@ -731,7 +744,7 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
             put(e / 4, __float_as_uint(v[e]), __float_as_uint(v[e + 1]), __float_as_uint(v[e + 2]), __float_as_uint(v[e + 3]));
           if (bad) {
             __syncwarp();
-            mend_rows<T, true>(a, bad, key0, last_key, sees, base, inv, t, h, k0, kvh, from, D / 2, stage, kRowBytes);
+            mend_rows<T>(a, bad, key0, last_key, sees, base, inv, t, h, k0, kvh, from, D / 2, stage, kRowBytes);
           }
           drain(from, 4);
         }
@@ -752,7 +765,7 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
         for (int e = 0; e < D / 2; e += 4) put(e / 4, x[e], x[e + 1], x[e + 2], x[e + 3]);
         if (bad) {
           __syncwarp();
-          mend_rows<T, false>(a, bad, key0, last_key, sees, base, inv, t, h, k0, kvh, 0, D, stage, kRowBytes);
+          mend_rows<T>(a, bad, key0, last_key, sees, base, inv, t, h, k0, kvh, 0, D, stage, kRowBytes);
         }
         drain(0, 2);
       }
