@@ -118,12 +118,22 @@ struct TcLayout {
   static constexpr int kKv = W * kQ;
   static constexpr int kBars = kKv + kStages * kTile;
   static constexpr int kNumBars = 2 * kStages + 2 + 4 + 4 + 4 + 2;
-  static constexpr int kMisc = kBars + 8 * kNumBars;
-  static constexpr int kTotal = kMisc + 16;
+  static constexpr int kMisc = (kBars + 8 * kNumBars + 15) / 16 * 16;
+  static constexpr int kWork = kMisc + 16;  // the CTA's Work
+  static constexpr int kTotal = kWork + 64;
   // TMEM columns: tile w's S buffers at 128 w and 128 w + 64, its O at kO + w D.
   static constexpr int kO = W * 128, kColumns = W * 256;
   static_assert(kO + W * D <= kColumns, "TMEM");
   static_assert(kTotal <= (W == 2 ? 227 : 113) * 1024, "shared memory of one or two CTAs an SM");
+};
+
+// What a CTA does, worked out by its last warp: place (below), then keys.
+struct __align__(16) Work {
+  int q0, q_len, k0, k_len, tok0;  // tok0 < 0: nothing
+  int end[2];                      // keys that some row of the tile sees
+  int key0, key1;                  // this split's keys: first, and behind the last
+  int cnt[2];                      // steps of the tiles
+  int ring;                        // copies of K and V
 };
 
 // Where a CTA works: its sequence's queries and keys, and its first query token.
@@ -316,60 +326,71 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  const int span = W * a.tokens, kvh = blockIdx.x % a.kv_heads;
+  const int kvh = blockIdx.x % a.kv_heads;
   int number = blockIdx.x / a.kv_heads, split = 0;
   if (a.splits > 1) {
     split = number % a.splits;
     number /= a.splits;
   }
   ptx::griddep_launch();
-  Place at;
-  if (a.q_off) {
-    at = a.sequences <= 32 ? place_sorted(a, number, span) : place_searched(a, number, span);
-  } else {
-    at.q_len = (int)a.total_q;
-    at.k_len = (int)a.total_k;
-    at.token = number * span;
-  }
-  if (at.token < 0) return;
-  const int q0 = at.q0, q_len = at.q_len, k0 = at.k0, k_len = at.k_len, tok0 = at.token;
-  int end[2] = {0, 0};  // keys that some row of the tile sees
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    const int t_end = min(tok0 + (w + 1) * a.tokens, q_len);
-    const bool any = tok0 + w * a.tokens < q_len;
-    end[w] = !any ? 0 : a.causal ? max(0, min(k_len, t_end + k_len - q_len)) : k_len;
-  }
-  const int steps_all = (max(end[0], end[1]) + kKeys - 1) / kKeys;
-  int ja = 0, jb = steps_all;
-  if (a.splits > 1) {  // as even as tiles allow: the first `over` splits have one more
-    const int each = steps_all / a.splits, over = steps_all - each * a.splits;
-    ja = split * each + min(split, over);
-    jb = ja + each + (split < over);
-  }
-  const int key0 = ja * kKeys;  // this split's first key
-  const int cnt0 = max(0, (min(jb * kKeys, end[0]) - key0 + kUnit - 1) / kUnit);  // steps of the tiles
-  const int cnt1 = max(0, (min(jb * kKeys, end[1]) - key0 + kUnit - 1) / kUnit);
-  const int cnt = max(cnt0, cnt1), ring = 2 * ((cnt * kUnit + L::kTileKeys - 1) / L::kTileKeys);  // copies of K and V
 
-  // Ring number of K tile i: 2i, of V tile i: 2i + 1.
-  auto load_kv = [&](int n) {
+  // Ring number of K tile i: 2i, of V tile i: 2i + 1, for keys from `first` on.
+  auto load_kv = [&](int n, int first) {
     const int st = n % L::kStages;
     ptx::mbar_expect_tx(&kv_full[st], L::kTile);
     for (int h = 0; h < L::kHalves; ++h)
       ptx::tma_load_3d(sbase + L::kKv + st * L::kTile + h * L::kHalf, n & 1 ? &maps.v : &maps.k, h * 64, kvh,
-                       k0 + key0 + (n >> 1) * L::kTileKeys, &kv_full[st]);
+                       first + (n >> 1) * L::kTileKeys, &kv_full[st]);
   };
-  // The first copies go out before the CTA meets, under the allocation of TMEM.
-  if (warp == 5 * W && lane == 0) {
-    if (ring > 0) load_kv(0);
-    for (int w = 0; w < W; ++w)
-      if ((w == 0 ? cnt0 : cnt1) > 0) {
+  // One warp works out the CTA's place and sends for the first tiles while the
+  // others wait (their copies of that code only fought for the same units).
+  Work* work = reinterpret_cast<Work*>(sm + L::kWork);
+  if (warp == 5 * W) {
+    const int span = W * a.tokens;
+    Place at;
+    if (a.q_off) {
+      at = a.sequences <= 32 ? place_sorted(a, number, span) : place_searched(a, number, span);
+    } else {
+      at.q_len = (int)a.total_q;
+      at.k_len = (int)a.total_k;
+      at.token = number * span;
+    }
+    Work x;
+    x.q0 = at.q0;
+    x.q_len = at.q_len;
+    x.k0 = at.k0;
+    x.k_len = at.k_len;
+    x.tok0 = at.token;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const int t_end = min(at.token + (w + 1) * a.tokens, at.q_len);
+      const bool any = w < W && at.token >= 0 && at.token + w * a.tokens < at.q_len;
+      x.end[w] = !any ? 0 : a.causal ? max(0, min(at.k_len, t_end + at.k_len - at.q_len)) : at.k_len;
+    }
+    const int tiles = (max(x.end[0], x.end[1]) + kKeys - 1) / kKeys;
+    int ja = 0, jb = tiles;
+    if (a.splits > 1) {  // as even as tiles allow: the first `over` splits have one more
+      const int each = tiles / a.splits, over = tiles - each * a.splits;
+      ja = split * each + min(split, over);
+      jb = ja + each + (split < over);
+    }
+    x.key0 = ja * kKeys;
+    x.key1 = jb * kKeys;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) x.cnt[w] = max(0, (min(x.key1, x.end[w]) - x.key0 + kUnit - 1) / kUnit);
+    x.ring = 2 * ((max(x.cnt[0], x.cnt[1]) * kUnit + L::kTileKeys - 1) / L::kTileKeys);
+    if (lane == 0) {
+      *work = x;
+      if (x.ring > 0) load_kv(0, x.k0 + x.key0);
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        if (x.cnt[w] == 0) continue;
         ptx::mbar_expect_tx(&q_full[w], (unsigned)(a.tokens * a.group * 128 * L::kHalves));
         for (int h = 0; h < L::kHalves; ++h)
-          ptx::tma_load_4d(sbase + w * L::kQ + h * L::kQHalf, &maps.q, h * 64, 0, kvh, q0 + tok0 + w * a.tokens,
+          ptx::tma_load_4d(sbase + w * L::kQ + h * L::kQHalf, &maps.q, h * 64, 0, kvh, x.q0 + x.tok0 + w * a.tokens,
                            &q_full[w]);
       }
+    }
   }
   if (warp == 4 * W) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ptx::saddr(tmem_slot)),
@@ -380,6 +401,13 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
+  const int q0 = work->q0, q_len = work->q_len, k0 = work->k0, k_len = work->k_len, tok0 = work->tok0;
+  const int end_all = max(work->end[0], work->end[1]), key0 = work->key0, key1 = work->key1;
+  const int cnt0 = work->cnt[0], cnt1 = work->cnt[1], cnt = max(cnt0, cnt1), ring = work->ring;
+  if (tok0 < 0) {
+    if (warp == 4 * W) ptx::tmem_free<L::kColumns>(*tmem_slot);
+    return;
+  }
   // All 512 columns start at 0; half of them where the SM's other CTA is not.
   const unsigned tm = W == 2 ? 0 : __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
@@ -390,7 +418,7 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
 #pragma unroll 1
       for (; n < ring; ++n) {
         if (n >= L::kStages && !ptx::wait_phase(&kv_empty[n % L::kStages], (n / L::kStages - 1) & 1, abort_flag, a.err, kAttnWaitFree)) break;
-        load_kv(n);
+        load_kv(n, k0 + key0);
       }
       // Copies in flight land before the CTA exits.
 #pragma unroll 1
@@ -461,7 +489,8 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
       auto release = [&](int st) {
         if (ok) ptx::tc_commit(&kv_empty[st]);
       };
-      auto steps_of = [&](int n) { return (min(end[w] - key0 - n * kUnit, kUnit) + 15) / 16; };
+      const int end = work->end[w];
+      auto steps_of = [&](int n) { return (min(end - key0 - n * kUnit, kUnit) + 15) / 16; };
       if (cnt > 0) wait(&kv_full[0], 0, kAttnWaitLoad);
       if (mine > 0) wait(&q_full[w], 0, kAttnWaitLoad);
       if (W == 1) {  // a tile a step
@@ -639,7 +668,7 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
       // Value rows behind the last key that a row sees are not the sequence's own,
       // or masked for every row here: 0 x what they hold must stay 0.  The step
       // that takes some of them in clears them before it hands over.
-      const int most = max(end[0], end[1]) - key0 - n * kUnit;
+      const int most = end_all - key0 - n * kUnit;
       if (most < kUnit && most % 16 != 0) {
         const int v = 2 * (n * kUnit / L::kTileKeys) + 1, first = most + n * kUnit % L::kTileKeys;  // ring number, row
         ok = __all_sync(0xffffffffu, ptx::wait_phase(&kv_full[v % L::kStages], (v / L::kStages) & 1, abort_flag, a.err,
@@ -722,7 +751,7 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
       };
       // Keys that the products took in, masked ones among them: whole steps of 16, cleared behind the last that any row sees.
       const int last_key =
-          min(max(end[0], end[1]), key0 + (min(jb * kKeys, end[w]) - key0 + 15) / 16 * 16);
+          min(end_all, key0 + (min(key1, work->end[w]) - key0 + 15) / 16 * 16);
       const float base = m == -INFINITY ? 0.0f : m * c;
       if (parts) {
 #pragma unroll 1
@@ -778,7 +807,7 @@ __global__ void __launch_bounds__((TcLayout<D, W>::kThreads), W == 2 ? 1 : 2)
   __syncthreads();
   if (warp == 4 * W) {
     ptx::tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "n"(L::kColumns) : "memory");
+    ptx::tmem_free<L::kColumns>(*tmem_slot);
   }
 }
 

@@ -162,6 +162,10 @@ __host__ __device__ constexpr unsigned idesc_f16(bool bf16, bool b_rows, int m, 
          ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24);
 }
 
+template <int N>
+__device__ __forceinline__ void tmem_free(unsigned addr) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "n"(N) : "memory");
+}
 // 32 consecutive 32-bit TMEM columns of this thread's lane.
 __device__ __forceinline__ void tmem_ld32(unsigned addr, unsigned* v) {
   asm volatile(
