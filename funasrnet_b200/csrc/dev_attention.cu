@@ -40,7 +40,7 @@ void need_strides(const int64_t* s, int n) {
   for (int i = 0; i < n; ++i) need(s[i] >= 0 && s[i] < (1ll << 38), "a stride is negative or beyond 2^38 elements");
 }
 
-// Whether no two elements of a strided output share a place.
+// Whether no two elements of a strided output share a place (strides as need_strides leaves them).
 bool apart(const int64_t* strides, const int64_t* extents, int64_t inner) {
   int order[2] = {0, 1};
   if (strides[1] < strides[0]) std::swap(order[0], order[1]);
@@ -48,7 +48,7 @@ bool apart(const int64_t* strides, const int64_t* extents, int64_t inner) {
   for (int d : order) {
     if (extents[d] <= 1) continue;
     if (strides[d] < span) return false;
-    span += strides[d] * (extents[d] - 1);
+    span = (int64_t)std::min((double)span + (double)strides[d] * (double)(extents[d] - 1), 1e12);  // beyond any stride
   }
   return true;
 }
@@ -114,7 +114,7 @@ struct TcLayout {
   static constexpr int kHalves = D / 64, kQHalf = kRows * 128, kQ = kHalves * kQHalf;
   static constexpr int kTileKeys = W == 2 ? 128 : kUnit;
   static constexpr int kHalf = kTileKeys * 128, kTile = kHalves * kHalf;
-  static constexpr int kStages = W == 2 ? (D == 128 ? 5 : 8) : (D == 128 ? 5 : 8);  // K and V tiles in flight
+  static constexpr int kStages = D == 128 ? 5 : 8;  // K and V tiles in flight
   static constexpr int kKv = W * kQ;
   static constexpr int kBars = kKv + kStages * kTile;
   static constexpr int kNumBars = 2 * kStages + 2 + 4 + 4 + 4 + 2;
@@ -1322,76 +1322,10 @@ constexpr double kStepUs = 1.8;  // one key tile against two tiles of rows
 // Bytes of `parts` partial results of `rows` rows.
 int64_t part_bytes(int64_t parts, int64_t rows, int head_size) { return parts * rows * (head_size + 4) * 4; }
 
-// CTAs per KV head of a packed call with w tiles each, an upper bound (tile_sequence).
+// CTAs per KV head of a packed call with w tiles each, an upper bound (place_searched).
 int64_t packed_tiles(int64_t total_q, int sequences, int group, int w) {
   return total_q / (w * (kRows / group)) + sequences;
 }
-
-}  // namespace
-
-int check_attention_packed(const fa_attention_packed_args* a) {
-  need(a != nullptr, "null arguments");
-  check_heads(a->dtype, a->sequences, a->heads, a->kv_heads, a->head_size, a->scale);
-  need(a->total_q >= 0 && a->total_k >= 0 && a->reserved == 0, "negative total or a reserved field that is not 0");
-  need_strides(a->q_stride, 2);
-  need_strides(a->k_stride, 2);
-  need_strides(a->v_stride, 2);
-  need_strides(a->out_stride, 2);
-  if (!heads_supported(a->dtype, a->heads, a->kv_heads, a->head_size)) return kDeclined;
-  if (a->total_q * a->heads >= (1ll << 31) || a->total_k >= (1ll << 30)) return kDeclined;
-  if (a->total_q == 0 || a->sequences == 0) return kHandled;
-  need(a->q && a->out && a->q_offsets && a->k_offsets, "null q, out, q_offsets or k_offsets");
-  need(a->total_k == 0 || (a->k && a->v), "null k or v");
-  const int64_t extents[2] = {a->total_q, a->heads};
-  need(apart(a->out_stride, extents, a->head_size), "rows of out overlap");
-  if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out)) return kDeclined;
-  const auto rows = {a->total_q, (int64_t)a->heads}, keys = {a->total_k, (int64_t)a->kv_heads};
-  if (!strides16(a->q_stride, rows) || !strides16(a->k_stride, keys) || !strides16(a->v_stride, keys) ||
-      !strides16(a->out_stride, rows))
-    return kDeclined;
-  need(a->workspace_bytes >= attention_packed_workspace(a->total_q, a->total_k, a->sequences, a->heads, a->kv_heads,
-                                                        a->head_size) &&
-           (a->workspace_bytes == 0 || (a->workspace && aligned16(a->workspace))),
-       "workspace smaller than fa_dev_attention_packed_workspace, or not on 16 bytes");
-  return kHandled;
-}
-
-int check_attention_shared(const fa_attention_shared_args* a) {
-  need(a != nullptr, "null arguments");
-  check_heads(a->dtype, a->sequences, a->heads, a->kv_heads, a->head_size, a->scale);
-  need(a->prefix_len >= 0 && a->suffix_capacity >= 0, "negative length");
-  need_strides(a->q_stride, 2);
-  need_strides(a->prefix_k_stride, 2);
-  need_strides(a->prefix_v_stride, 2);
-  need_strides(a->suffix_k_stride, 3);
-  need_strides(a->suffix_v_stride, 3);
-  need_strides(a->out_stride, 2);
-  if (!heads_supported(a->dtype, a->heads, a->kv_heads, a->head_size)) return kDeclined;
-  if ((int64_t)a->sequences * a->heads >= (1ll << 31) || a->prefix_len + a->suffix_capacity >= (1ll << 30))
-    return kDeclined;
-  if (a->sequences == 0) return kHandled;
-  need(a->q && a->out, "null q or out");
-  need(a->prefix_len == 0 || (a->prefix_k && a->prefix_v), "null prefix_k or prefix_v");
-  need(a->suffix_capacity == 0 || (a->suffix_k && a->suffix_v && a->suffix_lens),
-       "null suffix_k, suffix_v or suffix_lens");
-  const int64_t extents[2] = {a->sequences, a->heads};
-  need(apart(a->out_stride, extents, a->head_size), "rows of out overlap");
-  if (!aligned16(a->q) || !aligned16(a->prefix_k) || !aligned16(a->prefix_v) || !aligned16(a->suffix_k) ||
-      !aligned16(a->suffix_v) || !aligned16(a->out))
-    return kDeclined;
-  const int64_t n = a->sequences, kv = a->kv_heads;
-  const auto rows = {n, (int64_t)a->heads}, prefix = {a->prefix_len, kv}, suffix = {n, a->suffix_capacity, kv};
-  if (!strides16(a->q_stride, rows) || !strides16(a->prefix_k_stride, prefix) || !strides16(a->prefix_v_stride, prefix) ||
-      !strides16(a->suffix_k_stride, suffix) || !strides16(a->suffix_v_stride, suffix) || !strides16(a->out_stride, rows))
-    return kDeclined;
-  need(a->workspace_bytes >= attention_shared_workspace(a->prefix_len, a->suffix_capacity, a->sequences, a->heads,
-                                                        a->kv_heads, a->head_size) &&
-           (a->workspace_bytes == 0 || (a->workspace && aligned16(a->workspace))),
-       "workspace smaller than fa_dev_attention_shared_workspace, or not on 16 bytes");
-  return kHandled;
-}
-
-namespace {
 
 // How a packed call is cut: tiles per CTA and key ranges.
 struct PackedPlan {
@@ -1420,6 +1354,12 @@ PackedPlan packed_plan(int64_t total_q, int64_t total_k, int sequences, int head
     }
   }
   return p;
+}
+
+// CTAs of a packed call.
+int64_t packed_ctas(const fa_attention_packed_args& a) {
+  const PackedPlan p = packed_plan(a.total_q, a.total_k, a.sequences, a.heads, a.kv_heads, a.head_size);
+  return packed_tiles(a.total_q, a.sequences, a.heads / a.kv_heads, p.w) * a.kv_heads * p.splits;
 }
 
 // How a shared-prefix call is cut.
@@ -1467,6 +1407,70 @@ SharedPlan shared_plan(int64_t prefix_len, int64_t capacity, int sequences, int 
 }
 
 }  // namespace
+
+int check_attention_packed(const fa_attention_packed_args* a) {
+  need(a != nullptr, "null arguments");
+  check_heads(a->dtype, a->sequences, a->heads, a->kv_heads, a->head_size, a->scale);
+  need(a->total_q >= 0 && a->total_k >= 0 && a->reserved == 0, "negative total or a reserved field that is not 0");
+  need_strides(a->q_stride, 2);
+  need_strides(a->k_stride, 2);
+  need_strides(a->v_stride, 2);
+  need_strides(a->out_stride, 2);
+  if (!heads_supported(a->dtype, a->heads, a->kv_heads, a->head_size)) return kDeclined;
+  if (a->total_q >= (1ll << 31) || a->total_q * a->heads >= (1ll << 31) || a->total_k >= (1ll << 30)) return kDeclined;
+  if (a->total_q == 0 || a->sequences == 0) return kHandled;
+  if (packed_ctas(*a) >= (1ll << 30)) return kDeclined;
+  need(a->q && a->out && a->q_offsets && a->k_offsets, "null q, out, q_offsets or k_offsets");
+  need(a->total_k == 0 || (a->k && a->v), "null k or v");
+  const int64_t extents[2] = {a->total_q, a->heads};
+  need(apart(a->out_stride, extents, a->head_size), "rows of out overlap");
+  if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out)) return kDeclined;
+  const auto rows = {a->total_q, (int64_t)a->heads}, keys = {a->total_k, (int64_t)a->kv_heads};
+  if (!strides16(a->q_stride, rows) || !strides16(a->k_stride, keys) || !strides16(a->v_stride, keys) ||
+      !strides16(a->out_stride, rows))
+    return kDeclined;
+  need(a->workspace_bytes >= attention_packed_workspace(a->total_q, a->total_k, a->sequences, a->heads, a->kv_heads,
+                                                        a->head_size) &&
+           (a->workspace_bytes == 0 || (a->workspace && aligned16(a->workspace))),
+       "workspace smaller than fa_dev_attention_packed_workspace, or not on 16 bytes");
+  return kHandled;
+}
+
+int check_attention_shared(const fa_attention_shared_args* a) {
+  need(a != nullptr, "null arguments");
+  check_heads(a->dtype, a->sequences, a->heads, a->kv_heads, a->head_size, a->scale);
+  need(a->prefix_len >= 0 && a->suffix_capacity >= 0, "negative length");
+  need_strides(a->q_stride, 2);
+  need_strides(a->prefix_k_stride, 2);
+  need_strides(a->prefix_v_stride, 2);
+  need_strides(a->suffix_k_stride, 3);
+  need_strides(a->suffix_v_stride, 3);
+  need_strides(a->out_stride, 2);
+  if (!heads_supported(a->dtype, a->heads, a->kv_heads, a->head_size)) return kDeclined;
+  if ((int64_t)a->sequences * a->heads >= (1ll << 31) || std::max(a->prefix_len, a->suffix_capacity) >= (1ll << 30) ||
+      a->prefix_len + a->suffix_capacity >= (1ll << 30))
+    return kDeclined;
+  if (a->sequences == 0) return kHandled;
+  need(a->q && a->out, "null q or out");
+  need(a->prefix_len == 0 || (a->prefix_k && a->prefix_v), "null prefix_k or prefix_v");
+  need(a->suffix_capacity == 0 || (a->suffix_k && a->suffix_v && a->suffix_lens),
+       "null suffix_k, suffix_v or suffix_lens");
+  const int64_t extents[2] = {a->sequences, a->heads};
+  need(apart(a->out_stride, extents, a->head_size), "rows of out overlap");
+  if (!aligned16(a->q) || !aligned16(a->prefix_k) || !aligned16(a->prefix_v) || !aligned16(a->suffix_k) ||
+      !aligned16(a->suffix_v) || !aligned16(a->out))
+    return kDeclined;
+  const int64_t n = a->sequences, kv = a->kv_heads;
+  const auto rows = {n, (int64_t)a->heads}, prefix = {a->prefix_len, kv}, suffix = {n, a->suffix_capacity, kv};
+  if (!strides16(a->q_stride, rows) || !strides16(a->prefix_k_stride, prefix) || !strides16(a->prefix_v_stride, prefix) ||
+      !strides16(a->suffix_k_stride, suffix) || !strides16(a->suffix_v_stride, suffix) || !strides16(a->out_stride, rows))
+    return kDeclined;
+  need(a->workspace_bytes >= attention_shared_workspace(a->prefix_len, a->suffix_capacity, a->sequences, a->heads,
+                                                        a->kv_heads, a->head_size) &&
+           (a->workspace_bytes == 0 || (a->workspace && aligned16(a->workspace))),
+       "workspace smaller than fa_dev_attention_shared_workspace, or not on 16 bytes");
+  return kHandled;
+}
 
 int64_t attention_packed_workspace(int64_t total_q, int64_t total_k, int sequences, int heads, int kv_heads,
                                    int head_size) {

@@ -380,6 +380,9 @@ int check_logits(const fa_logits_args* a) {
   if (a->vocab > FA_LOGITS_MAX_VOCAB || a->rows > (1 << 27)) return kDeclined;
   if (a->rows == 0) return kHandled;
   need(a->logits && a->out, "null logits or out");
+  const int64_t far = 1ll << 34;
+  need(a->logits_stride >= 0 && a->out_stride >= 0 && a->mask_stride >= 0, "negative stride");
+  need(a->rows == 1 || (a->logits_stride < far && a->out_stride < far), "a stride is beyond 2^34 elements");
   need(a->rows == 1 || (a->logits_stride >= a->vocab && a->out_stride >= a->vocab), "rows overlap: stride below vocab");
   // In place, or apart: rows of out on other rows of the logits would be read changed.
   const int64_t size = a->dtype == FA_DTYPE_F32 ? 4 : 2;
@@ -392,7 +395,6 @@ int check_logits(const fa_logits_args* a) {
   }
   need(apart || (x == y && (a->rows == 1 || a->logits_stride == a->out_stride)),
        "out overlaps logits and is not the same rows");
-  need(a->logits_stride >= 0 && a->out_stride >= 0 && a->mask_stride >= 0, "negative stride");
   need(!a->history || a->history_offsets, "history without history_offsets");
   need(!a->bias_tokens || (a->bias_values && a->bias_offsets), "bias_tokens without bias_values or bias_offsets");
   need(!a->mask || a->mask_stride >= (a->vocab + 31) / 32 || a->mask_count <= 1, "mask rows overlap");

@@ -363,8 +363,8 @@ int fa_dev_status(fa_backend* backend);
  * Limits (else FA_DECLINED): FA_DTYPE_F16 or FA_DTYPE_BF16; head_size a multiple
  * of 8 up to 128; heads / kv_heads up to 64; every base address, and every stride
  * of a dimension longer than one, a multiple of 16 bytes;
- * total_q * heads below 2^31, total_k below 2^30; scale above 0 (else
- * FA_ERR_ARGUMENT). */
+ * total_q * heads below 2^31, total_k below 2^30, and not more (sequences +
+ * total_q * heads / 128) * kv_heads than about 2^30; scale above 0 (else FA_ERR_ARGUMENT). */
 typedef struct fa_attention_packed_args {
   const void* q;            /* [total_q x heads x head_size] */
   const void* k;            /* [total_k x kv_heads x head_size] */
@@ -454,7 +454,7 @@ typedef struct fa_logits_args {
   const int32_t* bias_offsets;      /* [rows + 1], not decreasing */
   const uint32_t* mask;             /* [mask_count x mask_stride], or NULL: every token allowed */
   const int32_t* mask_rows;         /* [rows], or NULL: row r has mask row r */
-  int64_t logits_stride, out_stride;/* elements between rows */
+  int64_t logits_stride, out_stride;/* elements between rows, below 2^34 */
   int64_t mask_stride;              /* words between mask rows */
   int64_t history_total, bias_total;
   int32_t dtype, rows, vocab, mask_count;

@@ -107,6 +107,8 @@ BAD = [
     (shared, dict(out=None), "null"),
     (shared, dict(out_stride=(64, 128)), "overlap"),
     (shared, dict(sequences=64, prefix_len=9000, workspace_bytes=0), "workspace"),
+    (packed, dict(out_stride=(1 << 37, (1 << 38) - 8), total_q=(1 << 27) - 1), "overlap"),
+    (logits, dict(rows=1 << 27, logits_stride=1 << 38, out_stride=1 << 38), "stride"),
     (logits, dict(rows=-1), "rows"),
     (logits, dict(vocab=0), "vocab"),
     (logits, dict(logits=None), "null"),
@@ -135,6 +137,8 @@ def test_inconsistent_arguments_are_refused(call, make, change, word):
     (packed, dict(heads=130, kv_heads=1)),
     (packed, dict(total_k=1 << 30)),
     (packed, dict(total_q=1 << 28)),
+    (packed, dict(total_q=1 << 62)),
+    (packed, dict(sequences=1 << 28)),  # more CTAs than a grid has
     (packed, dict(q=(1 << 20) + 8)),
     (packed, dict(k_stride=(1028, 128))),
     (shared, dict(dtype=F32)),
@@ -142,6 +146,7 @@ def test_inconsistent_arguments_are_refused(call, make, change, word):
     (shared, dict(suffix_v=(1 << 22) + 2)),
     (shared, dict(suffix_k_stride=(102401, 1024, 128))),
     (shared, dict(suffix_capacity=1 << 30)),
+    (shared, dict(prefix_len=(1 << 63) - 1)),
     (logits, dict(vocab=(1 << 24) + 1, logits_stride=1 << 25, out_stride=1 << 25)),
 ])
 def test_sizes_outside_the_kernels_are_declined(call, make, change):
