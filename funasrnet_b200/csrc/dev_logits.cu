@@ -6,10 +6,17 @@
 // shared memory and with integer atomics, so that the order of arrival cannot
 // change a result; then it streams its part of the row, copying bits, writing
 // -inf under the mask and keeping the largest unmarked value; then it computes
-// the marked tokens, one thread each.  (Counts per token in shared memory, looked
-// up for every logit, took twice as long: the tables held the stream up.)  The
+// the marked tokens, one thread each, in 32 bits (the result alone is rounded to
+// the type, the pick comes before that).  Counts per token in shared memory, looked
+// up for every logit, took twice as long: the tables held the stream up.  The
 // CTAs of a row form a cluster and send their best (value, index) to the first.
-// One launch, no scratch.  Bound: the logits' bytes, read once and written once.
+// One launch, no scratch.
+//
+// Bound: the logits' bytes, read once and written once.  256 f32 rows of 151936
+// take 72.5 us, 4.3 of the 6.5 TB/s that a copy reaches (the tables' latency at
+// each row's start is not hidden by the SM's other CTA alone, and 256 rows leave 40
+// SMs with half the work of the others); 64 bf16 rows, cut in two, 13.8 us; one row, cut in 16, 6.1 us, a chain of latencies: offsets, lists,
+// atomics, logits, the cluster's best.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -25,11 +32,21 @@ namespace cg = cooperative_groups;
 
 namespace {
 
+// 256 threads make every chain of a thread's work twice as long (256 rows 108 us), 1024 leave one CTA an SM (75).
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMaxCluster = 16;
-constexpr int kSlots = 2048;   // hash table; also the tokens of a pass once it overflows
-constexpr int kUnroll = 4;     // 16-byte groups per thread and iteration
-constexpr int kWanted = 148;   // CTAs from which a row is not cut further
+// Rows that several CTAs share, and rows of one CTA: 16-byte groups per thread and
+// iteration, and slots of the hash table.  A part of a row is over before more loads
+// pay, and every slot is cleared and looked at: one row 6.1 us with 1 group and 512
+// slots, 6.3 with 1024, 7.0 with 2 groups and 2048.  Whole rows need loads in flight:
+// 256 rows 75.8, 72.5 and 75.3 us with 2, 3 and 4 groups (4 spill).
+template <bool kCut>
+struct Tuning {
+  static constexpr int kUnroll = kCut ? 1 : 3, kLogSlots = kCut ? 9 : 11;
+};
+constexpr int kFetch = 2;      // history or bias entries that a thread has in flight
+// CTAs from which a row is not cut further.  64 rows: 24.7 us uncut, 13.8 in halves, 14.2 in quarters.
+constexpr int kWanted = 74;
 constexpr int kMinSpan = 2048, kMaxSpan = 1 << 20;  // tokens of a CTA
 
 void need(bool ok, const char* what) {
@@ -70,15 +87,20 @@ __device__ __forceinline__ void send_best(Best b, Best* slot, uint64_t* bar) {
 
 constexpr int kLogitsWait = 51;  // error-word code of a best value that never came
 
-// f(token, index) for the entries [i0, i1) of a list, by all threads of the CTA.
+// Entries i, i + kThreads, ... of a list that ends before i1; -1 behind it.
+__device__ __forceinline__ void fetch(const int* list, int i, int i1, int* t) {
+#pragma unroll
+  for (int k = 0; k < kFetch; ++k) t[k] = i1 - i > k * kThreads ? list[i + k * kThreads] : -1;
+}
+// f(token, index) for the entries [i0, i1) of a list, by all threads of the CTA; t has the thread's first ones.
 template <typename F>
-__device__ __forceinline__ void for_entries(const int* list, int i0, int i1, F&& f) {
-  for (int i = i0 + (int)threadIdx.x; i < i1; i += 4 * kThreads) {
-    int t[4];
+__device__ __forceinline__ void for_entries(const int* list, int i0, int i1, int* t, F&& f) {
+  for (int i = i0 + (int)threadIdx.x;;) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) t[k] = i1 - i > k * kThreads ? list[i + k * kThreads] : -1;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) f(t[k], i + k * kThreads);
+    for (int k = 0; k < kFetch; ++k) f(t[k], i + k * kThreads);
+    if (i1 - i <= kFetch * kThreads) break;
+    i += kFetch * kThreads;
+    fetch(list, i, i1, t);
   }
 }
 
@@ -87,15 +109,16 @@ __device__ __forceinline__ unsigned bits_of(const unsigned* words, int w0, int e
   return __funnelshift_r(words[(e >> 5) - w0], words[(last >> 5) - w0], e & 31);
 }
 
-template <typename T>
+template <typename T, bool kCut>
 __global__ void __launch_bounds__(kThreads, 2) adjust_logits_kernel(const fa_logits_args a, int span, int* err) {
-  constexpr int VE = 16 / sizeof(T), U = kUnroll, kStep = kThreads * VE;
+  constexpr int VE = 16 / sizeof(T), U = Tuning<kCut>::kUnroll, kSlots = 1 << Tuning<kCut>::kLogSlots, kStep = kThreads * VE;
   constexpr unsigned kFull = (1u << VE) - 1;
   extern __shared__ __align__(16) unsigned marks[];  // one bit per token of the part
   __shared__ int slot_token[kSlots];      // -1: free
   __shared__ unsigned slot_seen[kSlots];  // bit 31: in the prompt; below: times generated.  Then the new logit
   __shared__ int slot_bias[kSlots];       // last bias entry + 1
   __shared__ int overflow;
+  __shared__ int before[kMaxSpan / 1024 + 1];  // marked tokens before each 1024 of the part
   __shared__ __align__(16) Best from[kMaxCluster * kWarps];  // the first CTA: every warp's best
   __shared__ uint64_t arrived;
   const int rank = (int)cg::this_cluster().block_rank(), ranks = (int)cg::this_cluster().num_blocks();
@@ -162,18 +185,27 @@ __global__ void __launch_bounds__(kThreads, 2) adjust_logits_kernel(const fa_log
       slot_bias[s] = 0;
     }
   };
-  // Gathers the entries of tokens [g0, g1) into the slots: by hash, marking the
-  // tokens, or (kDirect) at token - g0.
-  auto gather = [&](auto direct, int g0, int g1) {
-    constexpr bool kDirect = decltype(direct)::value;
-    const unsigned n = g1 - g0;
+  // A marked token's number among the marked ones.
+  auto rank_of = [&](int t) {
+    const int w = (t - lo) >> 5;
+    int n = before[w >> 5] + __popc(marks[w] & ((1u << (t & 31)) - 1));
+    for (int i = w & ~31; i < w; ++i) n += __popc(marks[i]);
+    return n;
+  };
+  // Gathers the entries of this part's tokens into the slots: by hash, marking the
+  // tokens, or (kRanked) those of the marked tokens from number r0 on.
+  auto gather = [&](auto ranked, int r0, int* seen_t, int* bias_t) {
+    constexpr bool kRanked = decltype(ranked)::value;
+    const unsigned n = hi - lo;
     auto slot_of = [&](int t) {
-      if (kDirect) {
-        slot_token[t - g0] = t;
-        return t - g0;
+      if (kRanked) {
+        const int r = rank_of(t) - r0;
+        if ((unsigned)r >= (unsigned)kSlots) return -1;
+        slot_token[r] = t;
+        return r;
       }
       atomicOr(&marks[(t - lo) >> 5], 1u << (t & 31));
-      int s = (int)((unsigned)t * 2654435761u >> 21);  // multiplicative hash to 11 bits
+      int s = (int)((unsigned)t * 2654435761u >> (32 - Tuning<kCut>::kLogSlots));  // multiplicative hash
       for (int probe = 0; probe < 32; ++probe, s = (s + 1) & (kSlots - 1)) {
         const int before = atomicCAS(&slot_token[s], -1, t);
         if (before == -1 || before == t) return s;
@@ -181,15 +213,15 @@ __global__ void __launch_bounds__(kThreads, 2) adjust_logits_kernel(const fa_log
       overflow = 1;
       return -1;
     };
-    for_entries(a.history, h0, h1, [&](int t, int i) {
-      if ((unsigned)(t - g0) >= n) return;
+    for_entries(a.history, h0, h1, seen_t, [&](int t, int i) {
+      if ((unsigned)(t - lo) >= n) return;
       const int s = slot_of(t);
       if (s < 0) return;
       if (i < made) atomicOr(&slot_seen[s], 0x80000000u);
       else atomicAdd(&slot_seen[s], 1u);
     });
-    for_entries(a.bias_tokens, b0, b1, [&](int t, int i) {
-      if ((unsigned)(t - g0) >= n) return;
+    for_entries(a.bias_tokens, b0, b1, bias_t, [&](int t, int i) {
+      if ((unsigned)(t - lo) >= n) return;
       const int s = slot_of(t);
       if (s >= 0) atomicMax(&slot_bias[s], i - b0 + 1);
     });
@@ -217,12 +249,20 @@ __global__ void __launch_bounds__(kThreads, 2) adjust_logits_kernel(const fa_log
       slot_seen[s] = __float_as_uint(allowed[k] & 1u ? y : -INFINITY);
     }
   };
-  if (marked) {
+  if (a.history || a.bias_tokens) {  // under the latency of the offsets
     clear();
     for (int i = threadIdx.x; i < span / 32; i += kThreads) marks[i] = 0;
     if (threadIdx.x == 0) overflow = 0;
+  }
+  int seen_t[kFetch], bias_t[kFetch];
+  auto fetch_first = [&] {
+    fetch(a.history, h0 + (int)threadIdx.x, h1, seen_t);
+    fetch(a.bias_tokens, b0 + (int)threadIdx.x, b1, bias_t);
+  };
+  if (marked) {
+    fetch_first();
     __syncthreads();
-    gather(std::false_type{}, lo, hi);
+    gather(std::false_type{}, 0, seen_t, bias_t);
     __syncthreads();
     if (!overflow) compute(in);  // their logits' latency passes with the stream's first
   }
@@ -297,12 +337,35 @@ __global__ void __launch_bounds__(kThreads, 2) adjust_logits_kernel(const fa_log
     __syncthreads();
     if (!overflow) {
       finish();
-    } else {  // more tokens than slots: a range of kSlots tokens at a time
-      for (int g0 = lo; g0 < hi; g0 += kSlots) {
+    } else {  // more tokens than slots: kSlots of them at a time
+      const int lane = threadIdx.x & 31, blocks = (hi - lo + 1023) / 1024;
+      for (int b = threadIdx.x >> 5; b < blocks; b += kWarps) {
+        const int w = b * 32 + lane, n = __reduce_add_sync(0xffffffffu, w < span / 32 ? __popc(marks[w]) : 0);
+        if (lane == 0) before[b] = n;
+      }
+      __syncthreads();
+      if (threadIdx.x < 32) {
+        int sum = 0;
+        for (int b = lane; b - lane < blocks; b += 32) {
+          const int n = b < blocks ? before[b] : 0;
+          int upto = n;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += x;
+          }
+          if (b < blocks) before[b] = sum + upto - n;
+          sum += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (lane == 0) before[blocks] = sum;
+      }
+      __syncthreads();
+      for (int r0 = 0, all = before[blocks]; r0 < all; r0 += kSlots) {
         __syncthreads();
         clear();
+        fetch_first();
         __syncthreads();
-        gather(std::true_type{}, g0, min(g0 + kSlots, hi));
+        gather(std::true_type{}, r0, seen_t, bias_t);
         __syncthreads();
         compute(out);
         finish();
@@ -353,22 +416,25 @@ void launch(const fa_logits_args& a, int* err, cudaStream_t stream) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  FA_CUDA(cudaLaunchKernelEx(&cfg, adjust_logits_kernel<T>, a, span, err));
+  FA_CUDA(cudaLaunchKernelEx(&cfg, ranks > 1 ? adjust_logits_kernel<T, true> : adjust_logits_kernel<T, false>, a, span, err));
 }
 
-template <typename T>
+template <typename T, bool kCut>
 void prepare() {
-  FA_CUDA(cudaFuncSetAttribute(adjust_logits_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  FA_CUDA(cudaFuncSetAttribute(adjust_logits_kernel<T, kCut>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                FA_LOGITS_MAX_VOCAB / kMaxCluster / 8));
-  FA_CUDA(cudaFuncSetAttribute(adjust_logits_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  FA_CUDA(cudaFuncSetAttribute(adjust_logits_kernel<T, kCut>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
 }
 
 }  // namespace
 
 void prepare_dev_logits() {
-  prepare<float>();
-  prepare<__half>();
-  prepare<__nv_bfloat16>();
+  prepare<float, true>();
+  prepare<float, false>();
+  prepare<__half, true>();
+  prepare<__half, false>();
+  prepare<__nv_bfloat16, true>();
+  prepare<__nv_bfloat16, false>();
 }
 
 int check_logits(const fa_logits_args* a) {
