@@ -1397,15 +1397,29 @@ SharedPlan shared_plan(int64_t prefix_len, int64_t capacity, int sequences, int 
   // (thresholds of 40, 80 and 160 MB, measured over 60 calls: 9.5, 9.3, 9.2 us on average).
   p.tc = (double)sequences * prefix_len * kv_heads * head_size * 4 > 1.6e8 && sequences >= 4;
   if (p.tc) {
-    // The two kernels run side by side, the prefix's bound by its MMAs and the
-    // own keys' by their bytes: as few CTAs for the prefix as let it end about
-    // when those (half of the capacity, at 6.2 TB/s) are through; a key tile
-    // takes about 1.4 us there.
-    const int64_t ctas = ((int64_t)sequences * group + 2 * kRows - 1) / (2 * kRows) * kv_heads;
+    // The two kernels run side by side, the prefix's bound by its MMAs and the own
+    // keys' by their bytes: more key ranges end the prefix sooner, leave fewer SMs
+    // to the own keys meanwhile (a CTA of the prefix fills an SM) and more parts to
+    // join.  Microseconds: 1.7 a key tile of two tiles of rows (one: 0.7 of it, head
+    // sizes up to 64: 0.6), own keys for 0.6 of the capacity at 6.2 TB/s, less what
+    // the free SMs read by then, and the parts.  Fitted to 24 calls, each measured with
+    // seven cuts: on average 2 % behind the best of them (filling the SMs with the
+    // prefix: 10 %; 237 sessions on 11045 keys take 72 us so and 64 as chosen here).
+    const int64_t rows = (int64_t)sequences * group, ctas = (rows + 2 * kRows - 1) / (2 * kRows) * kv_heads;
     const int64_t tiles = (prefix_len + kKeys - 1) / kKeys;
-    const double own_us = 2.0 * sequences * capacity * kv_heads * head_size / 6.2e6;
-    const int64_t each = std::max<int64_t>(2, (int64_t)(own_us * 0.6));
-    p.tc_splits = (int)std::max<int64_t>(1, std::min<int64_t>(kSms / ctas, (tiles + each - 1) / each));
+    const double tile_us = 1.7 * (rows > kRows ? 1.0 : 0.7) * (head_size <= 64 ? 0.6 : 1.0);
+    const double own_us = 2.0 + 0.6 * 4.0 * sequences * capacity * kv_heads * head_size / 6.2e6;
+    const double part_us = 0.7 * 8.0 * sequences * heads * head_size / 6e6;
+    double best = 1e30;
+    for (int64_t n = 1; n == 1 || (n <= kSms / ctas && 2 * n <= tiles + 1); ++n) {
+      const double prefix_us = 2.5 + (double)((tiles + n - 1) / n) * tile_us;
+      const double meanwhile = prefix_us * std::min(1.0, 1.2 * std::max<int64_t>(0, kSms - n * ctas) / kSms);
+      const double us = prefix_us + std::max(0.0, own_us - meanwhile) + n * part_us;
+      if (us < best) {
+        best = us;
+        p.tc_splits = (int)n;
+      }
+    }
   }
   const int64_t ctas = (int64_t)sequences * kv_heads * ((group + kRowHeads - 1) / kRowHeads);
   const int64_t stages = ((p.tc ? 0 : prefix_len) + capacity + kStageKeys - 1) / kStageKeys;
