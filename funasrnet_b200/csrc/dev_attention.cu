@@ -855,11 +855,15 @@ struct RowsMaps {
   CUtensorMap sk, sv;  // suffix: (channel, KV head, key, sequence), 16 keys a copy: none behind the length but in the last
 };
 
-template <int D>
+// S stages.  D = 64: four, or two where more CTAs wait than SMs hold of those, five of
+// which fit an SM instead of three (179 sessions of 18 keys, 16 KV heads: 21 us, then
+// 16; two sessions of 7000 keys: 11.0 us, with two stages 12.1).  D = 128: two, three CTAs.
+template <int D, int S>
 struct RowsLayout {
   static constexpr int kHalf = kStageKeys * 128;  // 64 keys x 64 channels, 128-byte swizzle
   static constexpr int kTile = D / 64 * kHalf;
-  static constexpr int kStages = D == 128 ? 2 : 4;
+  static constexpr int kStages = S;
+  static constexpr int kCtas = D == 64 && S == 2 ? 5 : 3;  // of an SM
   static constexpr int kBars = kStages * 2 * kTile;
   static constexpr int kMisc = kBars + 8 * 3 * kStages;
   static constexpr int kTotal = kMisc + 16 + 1024;
@@ -903,10 +907,10 @@ __device__ __forceinline__ unsigned transpose8(unsigned x) {
 // own keys of 256 sessions alone 83 us, 6.1 TB/s.  (Loads from global memory into
 // registers needed the L1 for what was in flight: they ran at half the rate on an
 // SM whose memory the tensor-core kernel had claimed.)
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kRowThreads, 3) attention_rows_kernel(const RowsArgs a,
-                                                                        const __grid_constant__ RowsMaps maps) {
-  using L = RowsLayout<D>;
+template <int D, int S, bool BF16>
+__global__ void __launch_bounds__(kRowThreads, (RowsLayout<D, S>::kCtas))
+    attention_rows_kernel(const RowsArgs a, const __grid_constant__ RowsMaps maps) {
+  using L = RowsLayout<D, S>;
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   constexpr int KB = D / 32, VB = D / 64, NO = D / 16;
   extern __shared__ uint8_t sm_raw[];
@@ -1309,6 +1313,13 @@ void launch_tc(const TcArgs& t, const TcMaps& maps, int w, int dtype, cudaStream
     w == 2 ? launch_tc_of<128, 2>(t, maps, dtype, stream) : launch_tc_of<128, 1>(t, maps, dtype, stream);
 }
 
+template <int D, int S>
+void launch_rows(const RowsArgs& r, const RowsMaps& maps, unsigned grid, bool after, int cluster, int dtype,
+                 cudaStream_t stream) {
+  launch_after(dtype == FA_DTYPE_BF16 ? attention_rows_kernel<D, S, true> : attention_rows_kernel<D, S, false>, grid,
+               kRowThreads, RowsLayout<D, S>::kTotal, after, cluster, stream, r, maps);
+}
+
 void launch_join(const JoinArgs& j, int dtype, cudaStream_t stream) {
   const int w = j.parts > 8 ? kJoinWarps : 1;
   const unsigned grid = (unsigned)((j.tokens * j.heads * w + kJoinWarps - 1) / kJoinWarps);
@@ -1520,10 +1531,12 @@ void prepare_dev_attention() {
   auto set = [](auto kernel, int bytes) {
     FA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
   };
-  set(attention_rows_kernel<64, false>, RowsLayout<64>::kTotal);
-  set(attention_rows_kernel<64, true>, RowsLayout<64>::kTotal);
-  set(attention_rows_kernel<128, false>, RowsLayout<128>::kTotal);
-  set(attention_rows_kernel<128, true>, RowsLayout<128>::kTotal);
+  set(attention_rows_kernel<64, 4, false>, RowsLayout<64, 4>::kTotal);
+  set(attention_rows_kernel<64, 4, true>, RowsLayout<64, 4>::kTotal);
+  set(attention_rows_kernel<64, 2, false>, RowsLayout<64, 2>::kTotal);
+  set(attention_rows_kernel<64, 2, true>, RowsLayout<64, 2>::kTotal);
+  set(attention_rows_kernel<128, 2, false>, RowsLayout<128, 2>::kTotal);
+  set(attention_rows_kernel<128, 2, true>, RowsLayout<128, 2>::kTotal);
   set(attention_tc_kernel<64, 1, false>, TcLayout<64, 1>::kTotal);
   set(attention_tc_kernel<64, 1, true>, TcLayout<64, 1>::kTotal);
   set(attention_tc_kernel<64, 2, false>, TcLayout<64, 2>::kTotal);
@@ -1666,11 +1679,13 @@ void launch_attention_shared(const fa_attention_shared_args& a, int* err, cudaSt
     encode_suffix(&maps.sv, a.dtype, a.suffix_v, a.head_size, a.kv_heads, a.suffix_capacity, a.sequences, a.suffix_v_stride);
   }
   const unsigned grid = (unsigned)((int64_t)a.sequences * a.kv_heads * r.blocks * r.splits);
-  const bool bf16 = a.dtype == FA_DTYPE_BF16, small = a.head_size <= 64;
-  launch_after(small ? (bf16 ? attention_rows_kernel<64, true> : attention_rows_kernel<64, false>)
-                     : (bf16 ? attention_rows_kernel<128, true> : attention_rows_kernel<128, false>),
-               grid, kRowThreads, small ? RowsLayout<64>::kTotal : RowsLayout<128>::kTotal, plan.tc, r.merge ? plan.row_splits : 1, stream,
-               r, maps);
+  const int cluster = r.merge ? plan.row_splits : 1;
+  if (a.head_size > 64)
+    launch_rows<128, 2>(r, maps, grid, plan.tc, cluster, a.dtype, stream);
+  else if (grid > (unsigned)(RowsLayout<64, 4>::kCtas * kSms))
+    launch_rows<64, 2>(r, maps, grid, plan.tc, cluster, a.dtype, stream);
+  else
+    launch_rows<64, 4>(r, maps, grid, plan.tc, cluster, a.dtype, stream);
   if (plan.join == SharedPlan::kJoin) {
     JoinArgs j;
     j.tokens = a.sequences;

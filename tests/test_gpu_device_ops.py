@@ -192,6 +192,8 @@ SHARED = [
     (6, 6, 40, 1200, [1, 2, 3] * 50),
     (32, 8, 128, 6, list(range(217, 804, 31))),  # keys cut into parts that a cluster joins
     (8, 1, 112, 6403, [47, 48, 0, 47]),          # into more parts than a cluster has
+    (16, 16, 64, 130, list(range(0, 240, 4))),   # more rows than the SMs hold at a time
+    (12, 6, 48, 3, [1, 0, 77] * 40),
 ]
 
 
