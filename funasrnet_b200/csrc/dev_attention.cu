@@ -1366,15 +1366,18 @@ PackedPlan packed_plan(int64_t total_q, int64_t total_k, int sequences, int head
   const double ctas = (double)packed_tiles(total_q, sequences, heads / kv_heads, p.w) * kv_heads;
   // The longest sequence is taken for 2.5 times the average: its CTAs' steps, or
   // all steps spread over the SMs, at kStepUs each; cutting the keys costs a
-  // second kernel and the parts' bytes, written and read.
+  // second kernel and the parts' bytes, written and read.  Chunks on histories of
+  // 3001 to 20000 keys take 299 us uncut and 91 as cut here (in 4; 115 in 3, 105 in
+  // 8); two tokens on 1749 keys 13.0 us with ranges of two tiles
+  // allowed and 20.3 with no fewer than four.
   auto cost = [&](int s) {
     const double longest = std::max(1.0, (sequences > 1 ? 2.5 : 1.0) * steps / s);
-    const double each = p.w == 2 ? kStepUs : 0.7 * kStepUs, sms = p.w == 2 ? kSms : 2 * kSms;
+    const double each = (p.w == 2 ? kStepUs : 0.7 * kStepUs) * (head_size <= 64 ? 0.6 : 1.0), sms = p.w == 2 ? kSms : 2 * kSms;
     const double parts = s > 1 ? 4.0 + 2.0 * s * total_q * heads * (head_size + 1) * 4 / 4e6 : 0.0;
     return std::max(longest, ctas * steps / sms) * each + ctas * s / sms * 1.5 + parts;
   };
   double best = cost(1);
-  for (int s = 2; s <= 64 && s * 4 <= steps; s += s < 8 ? 1 : s / 4) {
+  for (int s = 2; s <= 64 && s * 2 <= steps; s += s < 8 ? 1 : s / 4) {
     const double c = cost(s);
     if (c < best) {
       best = c;

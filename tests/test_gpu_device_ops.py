@@ -362,6 +362,9 @@ def test_packed_many_sequences(dev, dtype, sequences):
     ("f16", 6, 2, 96, [40], [40 + 6000], True),
     ("bf16", 2, 1, 128, [260], [3000], False),
     ("f16", 2, 1, 40, [100, 1], [2100, 6000], True),
+    ("f16", 12, 4, 112, [2, 0, 37], [901, 333, 1020], True),  # short ones, with one tile of rows a CTA
+    ("bf16", 16, 16, 32, [1, 2], [1023, 777], False),
+    ("bf16", 8, 8, 128, [130], [1000], True),
 ])
 def test_packed_keys_cut_into_parts(dev, dtype, heads, kv_heads, size, new, keys, causal):
     """Few rows and many keys: the call is cut over the keys and joined; rows of no sequence stay as they were."""
@@ -382,7 +385,7 @@ def test_packed_keys_cut_into_parts(dev, dtype, heads, kv_heads, size, new, keys
     dev.status()
 
 
-@pytest.mark.parametrize("size,keys", [(128, 300), (64, 300), (128, 6000)])
+@pytest.mark.parametrize("size,keys", [(128, 300), (64, 300), (128, 6000), (128, 900)])
 def test_packed_masked_keys_that_are_not_finite(dev, size, keys):
     """Keys and values behind the causal border are infinite or NaN: the queries before them do not see them, and those
     at and after them do."""
