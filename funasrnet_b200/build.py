@@ -1,11 +1,13 @@
 """Builds libfunasr_cuda.so in-tree for sm_100a with nvcc.
 
-    python -m funasrnet_b200.build            # library only
+    python -m funasrnet_b200.build            # the library, and the torch binding where torch is installed
     python -m funasrnet_b200.build --oracle   # also the CPU oracle (test infrastructure)
 """
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -18,7 +20,6 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libfunasr_cuda.so"
-BINDING = PKG / "_torch_ops.so"  # CPython module of device_ops.py
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # -fmad=false: every a*b+c stays two roundings unless a kernel asks for an FMA
@@ -63,7 +64,7 @@ def build_library(verbose: bool = False) -> Path:
     deps = [p for p in sorted(CSRC.glob("*")) if p.name != "torch_binding.cpp"] + [ROOT / "include" / "funasr_cuda.h"]
     newest = max(p.stat().st_mtime for p in deps)
     if LIB.exists() and LIB.stat().st_mtime >= newest and os.environ.get("FA_FORCE_BUILD") != "1":
-        build_binding()
+        _binding_if_possible()
         return LIB
     objs = []
     with cf.ThreadPoolExecutor(max_workers=len(SOURCES)) as ex:
@@ -83,25 +84,52 @@ def build_library(verbose: bool = False) -> Path:
     if r.returncode != 0:
         raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
     tmp.replace(LIB)
-    build_binding()
+    _binding_if_possible()
     return LIB
+
+
+def torch_version() -> str | None:
+    """The installed torch's version, None without torch.  Does not import it (seconds) where its metadata tell."""
+    if importlib.util.find_spec("torch") is None:
+        return None
+    try:
+        return importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        import torch
+
+        return str(torch.__version__)
+
+
+def binding_path() -> Path:
+    """CPython module of device_ops.py, for this Python and this torch: another of either has another file."""
+    return PKG / f"_torch_ops.{sysconfig.get_config_var('SOABI')}.torch-{torch_version()}.so"
+
+
+def _binding_if_possible() -> None:
+    """The C library stands by itself: no torch, or no compiler or headers for the binding, only leave that out."""
+    if torch_version() is None:
+        print("torch is not installed: the binding of device_ops.py is left out", file=sys.stderr)
+        return
+    try:
+        build_binding()
+    except (OSError, RuntimeError) as e:
+        print(f"the binding of device_ops.py is left out: {e}", file=sys.stderr)
 
 
 def build_binding() -> Path:
     """_torch_ops: the CPython binding of the device-pointer operators for torch tensors.  It calls the library
-    next to it and the installed torch's C++ interface, so it is rebuilt when torch's version changes."""
+    next to it and the installed torch's C++ interface."""
+    src, binding = CSRC / "torch_binding.cpp", binding_path()
+    newest = max(src.stat().st_mtime, (ROOT / "include" / "funasr_cuda.h").stat().st_mtime)
+    if binding.exists() and binding.stat().st_mtime >= newest and os.environ.get("FA_FORCE_BUILD") != "1":
+        return binding
+    gxx = "/usr/bin/g++" if Path("/usr/bin/g++").exists() else shutil.which("g++")
+    if gxx is None:
+        raise RuntimeError("g++ not found")
     import torch
 
-    src = CSRC / "torch_binding.cpp"
-    stamp = BUILD / "torch_version"
-    newest = max(src.stat().st_mtime, (ROOT / "include" / "funasr_cuda.h").stat().st_mtime)
-    if (BINDING.exists() and BINDING.stat().st_mtime >= newest and stamp.exists()
-            and stamp.read_text() == torch.__version__):
-        return BINDING
-    BUILD.mkdir(exist_ok=True)
     home = Path(torch.__file__).parent
-    gxx = "/usr/bin/g++" if Path("/usr/bin/g++").exists() else shutil.which("g++")
-    tmp = BINDING.with_suffix(".so.tmp")
+    tmp = binding.with_suffix(".so.tmp")
     cmd = [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-isystem", str(home / "include"), "-isystem", str(home / "include" / "torch" / "csrc" / "api" / "include"),
            "-isystem", sysconfig.get_path("include"), str(src), "-o", str(tmp), "-L", str(PKG), f"-l:{LIB.name}",
@@ -109,9 +137,8 @@ def build_binding() -> Path:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"binding build failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
-    tmp.replace(BINDING)
-    stamp.write_text(torch.__version__)
-    return BINDING
+    tmp.replace(binding)
+    return binding
 
 
 def build_oracle() -> Path:

@@ -27,7 +27,7 @@ import torch  # noqa: F401  (the binding uses its C++ interface)
 
 from ._lib import FaError, check, lib
 from .backend import CudaFloatBackend
-from .build import BINDING
+from .build import binding_path
 
 _lock = threading.Lock()
 _binding = None
@@ -38,10 +38,12 @@ def _native():
     global _binding
     with _lock:
         if _binding is None:
-            if not BINDING.exists():
-                raise RuntimeError(f"{BINDING} is missing: build it with `python -m funasrnet_b200.build`")
+            path = binding_path()
+            if not path.exists():
+                raise RuntimeError(f"{path} is missing: build it for this Python and torch with "
+                                   "`python -m funasrnet_b200.build`")
             lib()  # the binding calls the same library
-            spec = importlib.util.spec_from_file_location("funasrnet_b200._torch_ops", BINDING)
+            spec = importlib.util.spec_from_file_location("funasrnet_b200._torch_ops", path)
             module = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(module)
             _binding = module
