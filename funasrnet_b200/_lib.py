@@ -88,6 +88,7 @@ SIGNATURES = {
     "fa_batch_generate": (i32, [vp, i32, vp]),
     "fa_batch_generate_until": (i32, [vp, i32, vp, i32, vp, vp]),
     "fa_batch_last_ms": (i32, [vp, P(f32)]),
+    "fa_backend_stream": (i32, [vp, vp]),
     "fa_dev_status": (i32, [vp]),
     "fa_dev_attention_packed": (i32, [vp, vp, vp]),
     "fa_dev_attention_packed_workspace": (i64, [i64, i64, i32, i32, i32, i32]),

@@ -739,6 +739,15 @@ static int enqueue_dev(fa_backend* b, const Args* args, void* stream, int (*chec
 
 extern "C" {
 
+int fa_backend_stream(fa_backend* b, void** stream) {
+  return guarded([&] {
+    check_backend(b);
+    if (!stream) throw Error(kErrArgument, "null output");
+    *stream = b->stream;
+    return (int)kHandled;
+  });
+}
+
 int fa_dev_status(fa_backend* b) {
   return guarded([&] {
     check_backend(b);

@@ -12,18 +12,23 @@ contexts on one GPU calls them around its decode step:
 Arguments are torch tensors on the backend's device.  A call returns True, or
 False when the library declines the shape or alignment (outputs untouched);
 tensors that do not fit together raise ``ValueError``, what the library refuses
-``FaError``.  ``stream`` is a CUDA stream handle such as
-``torch.cuda.current_stream().cuda_stream`` (0 is the default stream); None
-selects the backend's own stream.  ``workspace`` is any contiguous tensor of at
-least the bytes that the ``*_workspace`` method gives; calls that may overlap in
-time need one each.
+``FaError``.
+
+``stream`` is a CUDA stream handle such as
+``torch.cuda.current_stream().cuda_stream`` (0 is the default stream); tensors of
+another stream have to outlive the call's work (``Tensor.record_stream``).  Without
+it a call runs on the backend's own stream, after what torch's current stream
+holds and before what is enqueued there next; giving the stream saves the two
+events of that.  ``workspace`` is any contiguous tensor of at least the bytes that
+the ``*_workspace`` method gives; calls that may overlap in time need one each.
 """
 from __future__ import annotations
 
+import ctypes as C
 import importlib.util
 import threading
 
-import torch  # noqa: F401  (the binding uses its C++ interface)
+import torch
 
 from ._lib import FaError, check, lib
 from .backend import CudaFloatBackend
@@ -57,6 +62,19 @@ class DeviceOps:
         self.b = backend
         self._device = backend.device
         self._native = _native()
+        h = C.c_void_p()
+        check(lib().fa_backend_stream(backend.handle, C.byref(h)))
+        self._own = torch.cuda.ExternalStream(h.value, device=self._device)
+
+    def _in_order(self, method, *args, **kw) -> bool:
+        """The call on the backend's own stream, between the work of torch's current stream and what follows there."""
+        self.b.handle  # raises when the backend is disposed, and its stream with it
+        now = torch.cuda.current_stream(self._device)
+        self._own.wait_stream(now)
+        try:
+            return method(*args, stream=self._own.cuda_stream, **kw)
+        finally:
+            now.wait_stream(self._own)
 
     # --------------------------------------------------------------- attention ----
 
@@ -74,6 +92,9 @@ class DeviceOps:
         positions of their sequence.  ``lse`` [tokens, heads] float32 receives
         the log of the sum of exponentials; ``scale`` defaults to size ** -0.5.
         """
+        if stream is None:
+            return self._in_order(self.attention_packed, q, k, v, q_offsets, k_offsets, out, causal=causal, scale=scale,
+                                  lse=lse, workspace=workspace)
         rc = self._native.attention_packed(self.b.handle.value, self._device, q, k, v, q_offsets, k_offsets, out, causal,
                                            scale, lse, workspace, stream)
         return rc == 0 or check(rc) == 0
@@ -91,6 +112,9 @@ class DeviceOps:
         size]; suffix_k, suffix_v [sequences, capacity, kv_heads, size], of
         which sequence b uses the first ``suffix_lens[b]`` (int32) positions.
         """
+        if stream is None:
+            return self._in_order(self.attention_shared, q, prefix_k, prefix_v, suffix_k, suffix_v, suffix_lens, out,
+                                  scale=scale, lse=lse, workspace=workspace)
         rc = self._native.attention_shared(self.b.handle.value, self._device, q, prefix_k, prefix_v, suffix_k, suffix_v,
                                            suffix_lens, out, scale, lse, workspace, stream)
         return rc == 0 or check(rc) == 0
@@ -109,6 +133,11 @@ class DeviceOps:
         ceil(vocab / 32)] holds one bit per allowed token (32-bit words), and
         ``mask_rows[r]`` picks the row's mask (negative: none).  All optional.
         """
+        if stream is None:
+            return self._in_order(self.adjust_logits, logits, out, tokens, history=history, history_offsets=history_offsets,
+                                  prompt_lens=prompt_lens, repetition=repetition, presence=presence, frequency=frequency,
+                                  bias_tokens=bias_tokens, bias_values=bias_values, bias_offsets=bias_offsets, mask=mask,
+                                  mask_rows=mask_rows)
         rc = self._native.adjust_logits(self.b.handle.value, self._device, logits, out, tokens, history, history_offsets,
                                         prompt_lens, repetition, presence, frequency, bias_tokens, bias_values,
                                         bias_offsets, mask, mask_rows, stream)

@@ -325,7 +325,9 @@ int fa_lm_head_argmax_noalloc(fa_backend* backend, const fa_weight* weight, cons
  *    backend's device; the struct itself is host memory, read during the call.
  *  - A call enqueues its kernels on `stream` (a cudaStream_t; NULL selects the
  *    backend's own stream, as fa_lm_head_argmax_noalloc does; cudaStreamLegacy
- *    names the default stream) and returns; the caller synchronises.
+ *    names the default stream) and returns; the caller synchronises.  The
+ *    backend's stream waits for no other: fa_backend_stream gives it to hosts that
+ *    order it with theirs.
  *  - Nothing is allocated, so calls can be captured into a CUDA graph.  A call
  *    that needs scratch memory takes it from `workspace`, whose contents need no
  *    preparation and mean nothing afterwards; calls that may overlap in time
@@ -342,6 +344,9 @@ int fa_lm_head_argmax_noalloc(fa_backend* backend, const fa_weight* weight, cons
 #define FA_DTYPE_F32 0
 #define FA_DTYPE_F16 1
 #define FA_DTYPE_BF16 2
+
+/* The backend's own stream (a cudaStream_t), valid as long as the backend. */
+int fa_backend_stream(fa_backend* backend, void** stream);
 
 /* Waits for the device, then FA_OK, or FA_ERR_TIMEOUT when a bounded wait of one
  * of the operators below gave up since the last call (its outputs are invalid). */

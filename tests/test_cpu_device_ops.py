@@ -217,3 +217,10 @@ def test_binding_refuses_tensors_that_do_not_fit(built_lib):
         native.adjust_logits(0, 0, x[0], x, *none)
     with pytest.raises(ValueError, match="expected a torch tensor"):
         native.attention_shared(0, 0, q, k, k, None, k, off, q, None, None, None, None)
+
+
+def test_the_backends_stream_needs_a_backend(built_lib):
+    from funasrnet_b200._lib import lib
+
+    out = C.c_void_p()
+    assert lib().fa_backend_stream(None, C.byref(out)) == ARGUMENT

@@ -1,0 +1,97 @@
+"""The device-pointer operators among torch's own work: streams and captured graphs."""
+import pytest
+from test_gpu_device_ops import dev, dtype_of, here, i32, packed_space, randn, shared_space, torch_  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def calls(dev):
+    """(name, inputs to fill, outputs, call) of each operator on small buffers."""
+    torch = torch_()
+    dt = dtype_of("bf16")
+    q, k, v = randn(1, 30, 8, 128, dtype=dt), randn(2, 900, 1, 128, dtype=dt), randn(3, 900, 1, 128, dtype=dt)
+    off, ko = i32([0, 30]), i32([0, 900])
+    out, lse = torch.zeros_like(q), torch.zeros(30, 8, device="cuda")
+    space = packed_space(dev, q, k, off)
+    sq, sk, lens = q[:5], k.view(5, 180, 1, 128), i32([1, 0, 180, 33, 70])
+    sout, slse = torch.zeros_like(sq), torch.zeros(5, 8, device="cuda")
+    sspace = shared_space(dev, sq, k, sk)
+    x = randn(4, 6, 20000, dtype=torch.float32)
+    y, tokens = torch.zeros_like(x), i32([0] * 6)
+    hist, hoff, pen = i32(list(range(60))), i32([10 * i for i in range(7)]), torch.full((6,), 1.5, device="cuda")
+    return [
+        ("packed", q, (out, lse), lambda **kw: dev.attention_packed(q, k, v, off, ko, out, lse=lse, workspace=space, **kw)),
+        ("shared", q, (sout, slse),
+         lambda **kw: dev.attention_shared(sq, k, v, sk, sk, lens, sout, lse=slse, workspace=sspace, **kw)),
+        ("logits", x, (y, tokens), lambda **kw: dev.adjust_logits(x, y, tokens, history=hist, history_offsets=hoff,
+                                                                  repetition=pen, **kw)),
+    ]
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_without_a_stream_a_call_follows_torchs_work_and_precedes_it(dev, which):
+    """The input's producer is late, the output's consumer follows at once; both on torch's current stream."""
+    torch = torch_()
+    _, fill, outs, call = calls(dev)[which]
+    fresh = (randn(9, *fill.shape, dtype=torch.float32) * 2).to(fill.dtype)
+    fill.copy_(fresh)
+    assert call(stream=here())
+    torch.cuda.synchronize()
+    want = [o.clone() for o in outs]
+    fill.zero_()
+    for o in outs:
+        o.zero_()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)  # some 50 ms
+        fill.copy_(fresh)
+        assert call()
+        got = [o.clone() for o in outs]
+        for o in outs:
+            o.zero_()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    dev.status()
+    assert all(not o.any() for o in outs)  # nothing wrote them afterwards
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_without_a_stream_a_call_is_part_of_a_captured_graph(dev, which):
+    torch = torch_()
+    _, fill, outs, call = calls(dev)[which]
+    assert call(stream=here())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert call()
+    fresh = (randn(9, *fill.shape, dtype=torch.float32) * 2).to(fill.dtype)
+    fill.copy_(fresh)
+    assert call(stream=here())
+    torch.cuda.synchronize()
+    want = [o.clone() for o in outs]
+    for o in outs:
+        o.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    dev.status()
+
+
+def test_a_disposed_backend_is_refused_with_and_without_a_stream(built_lib):
+    from funasrnet_b200.backend import CudaFloatBackend
+    from funasrnet_b200.device_ops import DeviceOps
+
+    backend = CudaFloatBackend(0)
+    ops = DeviceOps(backend)
+    _, _, outs, call = calls(ops)[2]
+    assert call()
+    torch_().cuda.synchronize()
+    backend.dispose()
+    for o in outs:
+        o.fill_(7)
+    for kw in ({}, {"stream": here()}):
+        with pytest.raises(RuntimeError, match="disposed"):
+            call(**kw)
+    torch_().cuda.synchronize()
+    assert all((o == 7).all() for o in outs)
