@@ -90,6 +90,7 @@ SIGNATURES = {
     "fa_batch_last_ms": (i32, [vp, P(f32)]),
     "fa_backend_stream": (i32, [vp, vp]),
     "fa_dev_status": (i32, [vp]),
+    "fa_dev_fault_test": (i32, [vp, vp]),
     "fa_dev_attention_packed": (i32, [vp, vp, vp]),
     "fa_dev_attention_packed_workspace": (i64, [i64, i64, i32, i32, i32, i32]),
     "fa_dev_attention_shared": (i32, [vp, vp, vp]),

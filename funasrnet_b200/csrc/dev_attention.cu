@@ -9,6 +9,9 @@
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
+#include <map>
+#include <mutex>
+#include <vector>
 
 #include "dev_ops.h"
 #include "dev_ptx.cuh"
@@ -18,7 +21,12 @@ namespace fa {
 
 namespace {
 
-__device__ int g_dev_error;
+// A word per backend.  Module memory, so that a captured graph may outlive the
+// backend whose word it would set; backends beyond kErrorWords share words.
+constexpr int kErrorWords = 4096;
+__device__ int g_dev_errors[kErrorWords];
+std::mutex g_words_mu;
+std::map<int, std::vector<int>> g_word_users;  // by device
 
 // ------------------------------------------------------------- checks ----
 
@@ -76,7 +84,13 @@ constexpr int kKeys = 128;     // keys of a K or V tile in shared memory
 constexpr int kUnit = 64;      // keys per softmax step: half a tile
 constexpr float kSlack = 8.0f; // powers of two by which a row's maximum may rise before its sums are rescaled
 
-enum AttnError : int { kAttnWaitLoad = 41, kAttnWaitMma = 42, kAttnWaitSoftmax = 43, kAttnWaitFree = 44 };
+enum AttnError : int {
+  kAttnWaitLoad = 41,
+  kAttnWaitMma = 42,
+  kAttnWaitSoftmax = 43,
+  kAttnWaitFree = 44,
+  kAttnWaitTest = 45
+};
 
 struct TcArgs {
   const int* q_off = nullptr;  // null: one sequence of all rows
@@ -1705,19 +1719,57 @@ void launch_attention_shared(const fa_attention_shared_args& a, int* err, cudaSt
   }
 }
 
-int* device_error_word() {
+ErrorWord take_error_word(int device, cudaStream_t stream) {
+  std::lock_guard<std::mutex> lk(g_words_mu);
+  std::vector<int>& users = g_word_users[device];
+  users.resize(kErrorWords);
+  ErrorWord w;
+  w.device = device;
+  w.slot = (int)(std::min_element(users.begin(), users.end()) - users.begin());
   void* p = nullptr;
-  FA_CUDA(cudaGetSymbolAddress(&p, g_dev_error));
-  return static_cast<int*>(p);
+  FA_CUDA(cudaGetSymbolAddress(&p, g_dev_errors));
+  w.word = static_cast<int*>(p) + w.slot;
+  if (users[w.slot] == 0) {
+    FA_CUDA(cudaMemsetAsync(w.word, 0, sizeof(int), stream));
+    FA_CUDA(cudaStreamSynchronize(stream));
+  }
+  ++users[w.slot];
+  return w;
 }
 
-int take_device_error() {
+void give_error_word(const ErrorWord& w) {
+  if (w.word == nullptr) return;
+  std::lock_guard<std::mutex> lk(g_words_mu);
+  --g_word_users[w.device][w.slot];
+}
+
+int read_error_word(const ErrorWord& w, cudaStream_t stream) {
   FA_CUDA(cudaDeviceSynchronize());
   int code = 0;
-  FA_CUDA(cudaMemcpyFromSymbol(&code, g_dev_error, sizeof(code)));
-  const int zero = 0;
-  if (code != 0) FA_CUDA(cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(zero)));
+  FA_CUDA(cudaMemcpyAsync(&code, w.word, sizeof(code), cudaMemcpyDeviceToHost, stream));
+  FA_CUDA(cudaStreamSynchronize(stream));
+  if (code != 0) {
+    FA_CUDA(cudaMemsetAsync(w.word, 0, sizeof(int), stream));
+    FA_CUDA(cudaStreamSynchronize(stream));
+  }
   return code;
+}
+
+namespace {
+// A wait that nothing ends.
+__global__ void fault_test_kernel(int* err) {
+  __shared__ uint64_t bar;
+  __shared__ int abort_flag;
+  ptx::mbar_init(&bar, 1);
+  abort_flag = 0;
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  ptx::wait_phase(&bar, 0, &abort_flag, err, kAttnWaitTest);
+}
+}  // namespace
+
+void launch_fault_test(int* err, cudaStream_t stream) {
+  fault_test_kernel<<<1, 1, 0, stream>>>(err);
+  FA_CUDA(cudaGetLastError());
 }
 
 }  // namespace fa

@@ -25,7 +25,7 @@ int64_t attention_packed_workspace(int64_t total_q, int64_t total_k, int sequenc
 int64_t attention_shared_workspace(int64_t prefix_len, int64_t suffix_capacity, int sequences, int heads, int kv_heads,
                                    int head_size);
 
-// `err`: device_error_word() of the current device.
+// `err`: the backend's error word.
 void launch_attention_packed(const fa_attention_packed_args& a, int* err, cudaStream_t stream);
 void launch_attention_shared(const fa_attention_shared_args& a, int* err, cudaStream_t stream);
 void launch_adjust_logits(const fa_logits_args& a, int* err, cudaStream_t stream);
@@ -33,10 +33,18 @@ void launch_adjust_logits(const fa_logits_args& a, int* err, cudaStream_t stream
 // Function attributes of these kernels on the current device; before any launch.
 void prepare_dev_attention();
 void prepare_dev_logits();
-// The current context's error word, which a bounded wait that gives up sets.
-int* device_error_word();
-// Waits for the device, then the error word of its current context's kernels
-// (0: no bounded wait gave up), cleared by the read.
-int take_device_error();
+
+// A backend's error word, which a bounded wait of its kernels that gives up
+// sets; `stream` is the backend's, the device the current one.
+struct ErrorWord {
+  int device = 0, slot = 0;
+  int* word = nullptr;
+};
+ErrorWord take_error_word(int device, cudaStream_t stream);
+void give_error_word(const ErrorWord& w);
+// Waits for the device, then the word (0: no bounded wait gave up), cleared by the read.
+int read_error_word(const ErrorWord& w, cudaStream_t stream);
+// Enqueues a bounded wait that nothing ends.
+void launch_fault_test(int* err, cudaStream_t stream);
 
 }  // namespace fa

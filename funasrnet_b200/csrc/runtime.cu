@@ -113,7 +113,7 @@ struct fa_backend {
   int models = 0;
   DevBuf in, out, aux, aux2;
   DevBuf bxq, bxs, berr;  // frame-tile operands of multi-frame projections
-  int* dev_error = nullptr;  // error word of the device-pointer operators
+  ErrorWord dev_error;  // of the device-pointer operators
   std::vector<float> staging;
 };
 
@@ -243,8 +243,8 @@ int fa_backend_create(int device, fa_backend** out) {
     prepare_kernels();
     prepare_dev_attention();
     prepare_dev_logits();
-    b->dev_error = device_error_word();
     b->name = std::string("CUDA ") + prop.name + " (sm_" + std::to_string(prop.major) + std::to_string(prop.minor) + ")";
+    b->dev_error = take_error_word(device, b->stream);
     *out = b.release();
     return (int)kHandled;
   });
@@ -266,6 +266,7 @@ int fa_backend_destroy(fa_backend* b) {
       b->aux.release();
       b->aux2.release();
       cudaStreamDestroy(b->stream);
+      give_error_word(b->dev_error);
       b->disposed = true;
     }
     delete b;
@@ -732,7 +733,7 @@ static int enqueue_dev(fa_backend* b, const Args* args, void* stream, int (*chec
     if (b->disposed) throw Error(kErrDisposed, "backend disposed");
     DeviceGuard g(b->device);
     FA_CUDA(cudaSetDevice(b->device));  // a thread's first call: tensor maps need the context to be current
-    launch(*args, b->dev_error, stream != nullptr ? static_cast<cudaStream_t>(stream) : b->stream);
+    launch(*args, b->dev_error.word, stream != nullptr ? static_cast<cudaStream_t>(stream) : b->stream);
     return (int)kHandled;
   });
 }
@@ -752,8 +753,17 @@ int fa_dev_status(fa_backend* b) {
   return guarded([&] {
     check_backend(b);
     DeviceGuard g(b->device);
-    const int code = take_device_error();
+    const int code = read_error_word(b->dev_error, b->stream);
     if (code != 0) throw Error(kErrTimeout, "a bounded device wait gave up (code " + std::to_string(code) + ")");
+    return (int)kHandled;
+  });
+}
+
+int fa_dev_fault_test(fa_backend* b, void* stream) {
+  return guarded([&] {
+    check_backend(b);
+    DeviceGuard g(b->device);
+    launch_fault_test(b->dev_error.word, stream != nullptr ? static_cast<cudaStream_t>(stream) : b->stream);
     return (int)kHandled;
   });
 }

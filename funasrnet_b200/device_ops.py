@@ -144,7 +144,7 @@ class DeviceOps:
         return rc == 0 or check(rc) == 0
 
     def status(self) -> None:
-        """Waits for the device; raises ``FaError`` (timeout) when a bounded device wait of these operators gave up."""
+        """Waits for the device; raises ``FaError`` (timeout) when a bounded wait of a call on this backend gave up."""
         check(lib().fa_dev_status(self.b.handle))
 
 

@@ -349,8 +349,11 @@ int fa_lm_head_argmax_noalloc(fa_backend* backend, const fa_weight* weight, cons
 int fa_backend_stream(fa_backend* backend, void** stream);
 
 /* Waits for the device, then FA_OK, or FA_ERR_TIMEOUT when a bounded wait of one
- * of the operators below gave up since the last call (its outputs are invalid). */
+ * of the operators below, called on this backend, gave up since the last call
+ * (its outputs are invalid).  Calls on other backends of the device have their own status. */
 int fa_dev_status(fa_backend* backend);
+/* Test hook: enqueues a bounded wait that nothing ends; it gives up after two seconds. */
+int fa_dev_fault_test(fa_backend* backend, void* stream);
 
 /* Attention of several packed sequences.  Sequence b has the queries
  * q_offsets[b] .. q_offsets[b+1] and the keys k_offsets[b] .. k_offsets[b+1];
