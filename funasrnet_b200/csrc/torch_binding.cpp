@@ -8,9 +8,11 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/core/grad_mode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <initializer_list>
 #include <stdexcept>
 #include <string>
 
@@ -27,6 +29,13 @@ struct Refused : std::runtime_error {
 const at::Tensor& tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) refuse(name, "expected a torch tensor");
   return THPVariable_Unpack(o);
+}
+
+// Tells autograd that a call has overwritten an output, as torch's own in-place operations do.
+void written(PyObject* o) {
+  if (o == Py_None) return;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 int dtype_of(const at::Tensor& t, const char* name) {
@@ -106,6 +115,12 @@ struct Call {  // the arguments that every function starts with, and the stream 
     stream = s == Py_None ? nullptr : PyLong_AsVoidPtr(s);
     if (s != Py_None && stream == nullptr) stream = reinterpret_cast<void*>(1);
     if (PyErr_Occurred()) throw Refused("");
+    // Autograd would take the outputs for constants.
+    if (!at::GradMode::is_enabled()) return;
+    for (Py_ssize_t i = 2; i < n; ++i)
+      if (THPVariable_Check(args[i]) && THPVariable_Unpack(args[i]).requires_grad())
+        throw Refused("a tensor requires grad, but this operator has no backward pass: call it under torch.no_grad() or "
+                      "detach the tensor");
   }
 };
 
@@ -133,11 +148,14 @@ PyObject* guarded(Py_ssize_t n, Py_ssize_t expected, F&& f) {
 }
 
 template <typename Args>
-int enqueue(int (*fn)(fa_backend*, const Args*, void*), const Call& c, const Args& a) {
+int enqueue(int (*fn)(fa_backend*, const Args*, void*), const Call& c, const Args& a,
+            std::initializer_list<PyObject*> outputs) {
   int rc;
   Py_BEGIN_ALLOW_THREADS
   rc = fn(c.backend, &a, c.stream);
   Py_END_ALLOW_THREADS
+  if (rc == FA_OK)
+    for (PyObject* o : outputs) written(o);
   return rc;
 }
 
@@ -170,7 +188,7 @@ PyObject* attention_packed(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (causal < 0) throw Refused("");
     a.causal = causal;
     a.scale = scale_of(args[9], size);
-    return enqueue(fa_dev_attention_packed, c, a);
+    return enqueue(fa_dev_attention_packed, c, a, {args[7], args[10]});
   });
 }
 
@@ -203,7 +221,7 @@ PyObject* attention_shared(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.kv_heads = small(kv_heads, "prefix_k");
     a.head_size = small(size, "q");
     a.scale = scale_of(args[9], size);
-    return enqueue(fa_dev_attention_shared, c, a);
+    return enqueue(fa_dev_attention_shared, c, a, {args[8], args[10]});
   });
 }
 
@@ -245,7 +263,7 @@ PyObject* adjust_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.mask_rows = flat<int32_t>(args[15], at::kInt, count, c.device, "mask_rows");
     a.rows = small(count, "logits");
     a.vocab = small(vocab, "logits");
-    return enqueue(fa_dev_adjust_logits, c, a);
+    return enqueue(fa_dev_adjust_logits, c, a, {args[3], args[4]});
   });
 }
 

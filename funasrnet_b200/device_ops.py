@@ -12,7 +12,8 @@ contexts on one GPU calls them around its decode step:
 Arguments are torch tensors on the backend's device.  A call returns True, or
 False when the library declines the shape or alignment (outputs untouched);
 tensors that do not fit together raise ``ValueError``, what the library refuses
-``FaError``.
+``FaError``.  There is no backward pass: tensors that require grad are refused where
+grad mode is on, and a call raises the version of the tensors that it writes.
 
 ``stream`` is a CUDA stream handle such as
 ``torch.cuda.current_stream().cuda_stream`` (0 is the default stream); tensors of

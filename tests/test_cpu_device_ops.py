@@ -224,3 +224,28 @@ def test_the_backends_stream_needs_a_backend(built_lib):
 
     out = C.c_void_p()
     assert lib().fa_backend_stream(None, C.byref(out)) == ARGUMENT
+
+
+def test_binding_refuses_tensors_that_require_grad(built_lib):
+    """Wherever such a tensor stands, before anything else is looked at; under no_grad it is taken."""
+    import torch
+
+    from funasrnet_b200 import device_ops
+
+    native = device_ops._native()
+    half, off = torch.zeros(7, 4, 64, dtype=torch.half), torch.zeros(2, dtype=torch.int32)
+    cache = torch.zeros(7, 9, 4, 64, dtype=torch.half)
+    packed = [0, 0, half, half, half, off, off, half, True, None, None, None, None]
+    shared = [0, 0, half, half, half, cache, cache, torch.zeros(7, dtype=torch.int32), half, None, None, None, None]
+    x, f = torch.zeros(3, 100), torch.zeros(3)
+    logits = [0, 0, x, x, None, None, None, None, f, f, f, None, None, None, None, None, None]
+    for fn, args, places in ((native.attention_packed, packed, (2, 3, 4, 7)), (native.attention_shared, shared, (2, 3, 4, 5, 6, 8)),
+                             (native.adjust_logits, logits, (2, 3, 8, 9, 10))):
+        with pytest.raises(ValueError, match="not on the backend's device"):
+            fn(*args)
+        for i in places:
+            with_grad = args[:i] + [args[i].clone().requires_grad_()] + args[i + 1:]
+            with pytest.raises(ValueError, match="requires grad"):
+                fn(*with_grad)
+            with torch.no_grad(), pytest.raises(ValueError, match="not on the backend's device"):
+                fn(*with_grad)

@@ -1,4 +1,4 @@
-"""The device-pointer operators among torch's own work: streams and captured graphs."""
+"""The device-pointer operators among torch's own work: streams, captured graphs, autograd's view of their outputs."""
 import pytest
 from test_gpu_device_ops import dev, dtype_of, here, i32, packed_space, randn, shared_space, torch_  # noqa: F401
 
@@ -95,3 +95,44 @@ def test_a_disposed_backend_is_refused_with_and_without_a_stream(built_lib):
             call(**kw)
     torch_().cuda.synchronize()
     assert all((o == 7).all() for o in outs)
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_a_call_raises_the_version_of_its_outputs(dev, which):
+    """Autograd refuses a backward pass through a tensor that a call has overwritten since it was saved."""
+    torch = torch_()
+    _, _, outs, call = calls(dev)[which]
+    before = [o._version for o in outs]
+    assert call(stream=here())
+    assert all(o._version > b for o, b in zip(outs, before))
+    if which < 2:
+        w = torch.ones_like(outs[0], requires_grad=True)
+        loss = (w * outs[0]).sum()
+        assert call(stream=here())
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    torch.cuda.synchronize()
+
+
+def test_tensors_that_require_grad_are_refused_and_inference_tensors_taken(dev):
+    torch = torch_()
+    dt = dtype_of("f16")
+    q, k = randn(1, 4, 2, 64, dtype=dt), randn(2, 9, 2, 64, dtype=dt)
+    off, ko = i32([0, 4]), i32([0, 9])
+    out = torch.full_like(q, 7.0)
+    leaf = q.clone().requires_grad_()
+    for args in ((leaf, k, k), (q, k.clone().requires_grad_(), k), (q, k, k.clone().requires_grad_())):
+        with pytest.raises(ValueError, match="requires grad"):
+            dev.attention_packed(*args, off, ko, out, stream=here())
+    torch.cuda.synchronize()
+    assert (out == 7.0).all()
+    with torch.no_grad():
+        assert dev.attention_packed(leaf, k, k, off, ko, out, stream=here())
+    with torch.inference_mode():
+        out2 = torch.zeros_like(q)
+        assert dev.attention_packed(q, k, k, off, ko, out2, stream=here())
+    torch.cuda.synchronize()
+    assert torch.equal(out, out2)
+    assert dev.attention_packed(q, k, k, off, ko, out2, stream=here())  # an inference tensor outside that mode
+    torch.cuda.synchronize()
+    assert torch.equal(out, out2)
