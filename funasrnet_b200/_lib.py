@@ -95,6 +95,8 @@ SIGNATURES = {
     "fa_dev_attention_packed_workspace": (i64, [i64, i64, i32, i32, i32, i32]),
     "fa_dev_attention_shared": (i32, [vp, vp, vp]),
     "fa_dev_attention_shared_workspace": (i64, [i64, i64, i32, i32, i32, i32]),
+    "fa_dev_attention_packed_workspace_bound": (i64, [i64, i64, i32, i32, i32]),
+    "fa_dev_attention_shared_workspace_bound": (i64, [i64, i64, i32, i32, i32, i32]),
     "fa_dev_adjust_logits": (i32, [vp, vp, vp]),
 }
 

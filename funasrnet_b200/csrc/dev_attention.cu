@@ -1364,6 +1364,12 @@ constexpr double kStepUs = 1.8;  // one key tile against two tiles of rows, meas
 // Bytes of `parts` partial results of `rows` rows.
 int64_t part_bytes(int64_t parts, int64_t rows, int head_size) { return parts * rows * (head_size + 4) * 4; }
 
+// Rows of all partial results of a packed call together, at most: what bounds a
+// workspace for any batch up to given sizes.  Ranges that fill the SMs two or
+// three times over need fewer (188288 in 3 million random calls).
+constexpr int64_t kMostPartRows = 192 * 1024;
+constexpr int kMostSplits = 64;
+
 // CTAs per KV head of a packed call with w tiles each, an upper bound (place_searched).
 int64_t packed_tiles(int64_t total_q, int sequences, int group, int w) {
   return total_q / (w * (kRows / group)) + sequences;
@@ -1391,7 +1397,8 @@ PackedPlan packed_plan(int64_t total_q, int64_t total_k, int sequences, int head
     return std::max(longest, ctas * steps / sms) * each + ctas * s / sms * 1.5 + parts;
   };
   double best = cost(1);
-  for (int s = 2; s <= 64 && s * 2 <= steps; s += s < 8 ? 1 : s / 4) {
+  for (int s = 2; s <= kMostSplits && s * 2 <= steps && (double)s * total_q * heads <= kMostPartRows;
+       s += s < 8 ? 1 : s / 4) {
     const double c = cost(s);
     if (c < best) {
       best = c;
@@ -1407,6 +1414,14 @@ int64_t packed_ctas(const fa_attention_packed_args& a) {
   return packed_tiles(a.total_q, a.sequences, a.heads / a.kv_heads, p.w) * a.kv_heads * p.splits;
 }
 
+// Bytes that serve every packed call of up to total_q queries and total_k keys.
+int64_t packed_bound(int64_t total_q, int64_t total_k, int heads, int head_size) {
+  const int64_t splits = std::min<int64_t>(kMostSplits, total_k / (2 * kKeys));
+  if (splits < 2) return 0;
+  const double rows = std::min((double)kMostPartRows, (double)splits * total_q * heads);
+  return part_bytes(1, (int64_t)rows, head_size);
+}
+
 // How a shared-prefix call is cut.
 struct SharedPlan {
   bool tc = false;      // the prefix on the tensor cores, for all sequences at once
@@ -1417,13 +1432,21 @@ struct SharedPlan {
   enum { kOne, kMerge, kJoin } join = kOne;
   int parts() const { return tc_splits + (join == kJoin ? row_splits : 0); }  // partial results in the workspace
 };
+// CTAs of the rows kernel per SM that key ranges are cut for where a join_kernel
+// follows: without the prefix's kernel beside it, and with it.
+constexpr int kRowJoin = 2, kRowJoinTc = 8;
+
+// Read by every sequence's CTAs on its own the prefix costs these bytes (of L2,
+// mostly); the tensor-core kernel and what it leaves to join cost 15 to 20 us
+// (thresholds of 40, 80 and 160 MB, measured over 60 calls: 9.5, 9.3, 9.2 us on average).
+bool prefix_on_tc(int64_t prefix_len, int sequences, int kv_heads, int head_size) {
+  return (double)sequences * prefix_len * kv_heads * head_size * 4 > 1.6e8 && sequences >= 4;
+}
+
 SharedPlan shared_plan(int64_t prefix_len, int64_t capacity, int sequences, int heads, int kv_heads, int head_size) {
   SharedPlan p;
   const int group = heads / kv_heads;
-  // Read by every sequence's CTAs on its own the prefix costs these bytes (of L2,
-  // mostly); the tensor-core kernel and what it leaves to join cost 15 to 20 us
-  // (thresholds of 40, 80 and 160 MB, measured over 60 calls: 9.5, 9.3, 9.2 us on average).
-  p.tc = (double)sequences * prefix_len * kv_heads * head_size * 4 > 1.6e8 && sequences >= 4;
+  p.tc = prefix_on_tc(prefix_len, sequences, kv_heads, head_size);
   if (p.tc) {
     // The two kernels run side by side, the prefix's bound by its MMAs and the own
     // keys' by their bytes: more key ranges end the prefix sooner, leave fewer SMs
@@ -1459,10 +1482,30 @@ SharedPlan shared_plan(int64_t prefix_len, int64_t capacity, int sequences, int 
     while (p.row_splits < kMaxCluster && 2 * p.row_splits <= wanted) p.row_splits *= 2;
     p.join = p.row_splits > 1 ? SharedPlan::kMerge : SharedPlan::kOne;
   } else {
-    p.row_splits = (int)std::max<int64_t>(1, std::min<int64_t>((p.tc ? 8 : 2) * kSms / ctas, stages / 4));
+    p.row_splits = (int)std::max<int64_t>(1, std::min<int64_t>((p.tc ? kRowJoinTc : kRowJoin) * kSms / ctas, stages / 4));
     p.join = SharedPlan::kJoin;
   }
   return p;
+}
+
+// Bytes that serve every shared-prefix call up to these sizes: the parts of
+// shared_plan, each at the most that its conditions leave, which grow with the
+// sizes.  `rows` is the batch's query rows; a CTA of the prefix has 2 kRows of
+// them, one of the rows kernel kRowHeads.
+int64_t shared_bound(int64_t prefix_len, int64_t capacity, int sequences, int heads, int kv_heads, int head_size) {
+  prefix_len = std::min<int64_t>(prefix_len, 1 << 30);
+  capacity = std::min<int64_t>(capacity, 1 << 30);
+  const double rows = std::min((double)sequences * heads, 2147483647.0);  // larger calls, and prefixes, are declined
+  const auto parts = [&](double splits, double most) { return std::min(splits * rows, most); };
+  double need = 0.0;
+  const int64_t stages = (prefix_len + capacity + kStageKeys - 1) / kStageKeys;
+  if (stages / 3 > 2 * kMaxCluster) need = parts(stages / 4, kRowJoin * kSms * kRowHeads);
+  if (prefix_on_tc(prefix_len, sequences, kv_heads, head_size)) {
+    const int64_t tiles = (prefix_len + kKeys - 1) / kKeys, own = (capacity + kStageKeys - 1) / kStageKeys;
+    need = std::max(need, std::max(rows, parts((tiles + 1) / 2, kSms * 2 * kRows)) +
+                              std::max(rows, parts(own / 4, kRowJoinTc * kSms * kRowHeads)));
+  }
+  return part_bytes(1, (int64_t)need, head_size);
 }
 
 }  // namespace
@@ -1542,6 +1585,18 @@ int64_t attention_shared_workspace(int64_t prefix_len, int64_t suffix_capacity, 
   if (sequences <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > 64) return 0;
   const SharedPlan p = shared_plan(prefix_len, suffix_capacity, sequences, heads, kv_heads, head_size);
   return part_bytes(p.parts(), (int64_t)sequences * heads, head_size);
+}
+
+int64_t attention_packed_workspace_bound(int64_t total_q, int64_t total_k, int heads, int kv_heads, int head_size) {
+  if (total_q <= 0 || total_k <= 0 || heads <= 0 || kv_heads <= 0 || head_size <= 0 || heads % kv_heads) return 0;
+  return packed_bound(total_q, total_k, heads, head_size);
+}
+int64_t attention_shared_workspace_bound(int64_t prefix_len, int64_t suffix_capacity, int sequences, int heads,
+                                         int kv_heads, int head_size) {
+  if (prefix_len < 0 || suffix_capacity < 0 || sequences <= 0 || heads <= 0 || kv_heads <= 0 || head_size <= 0 ||
+      heads % kv_heads)
+    return 0;
+  return shared_bound(prefix_len, suffix_capacity, sequences, heads, kv_heads, head_size);
 }
 
 void prepare_dev_attention() {

@@ -25,6 +25,10 @@ int64_t attention_packed_workspace(int64_t total_q, int64_t total_k, int sequenc
 int64_t attention_shared_workspace(int64_t prefix_len, int64_t suffix_capacity, int sequences, int heads, int kv_heads,
                                    int head_size);
 
+int64_t attention_packed_workspace_bound(int64_t total_q, int64_t total_k, int heads, int kv_heads, int head_size);
+int64_t attention_shared_workspace_bound(int64_t prefix_len, int64_t suffix_capacity, int sequences, int heads,
+                                         int kv_heads, int head_size);
+
 // `err`: the backend's error word.
 void launch_attention_packed(const fa_attention_packed_args& a, int* err, cudaStream_t stream);
 void launch_attention_shared(const fa_attention_shared_args& a, int* err, cudaStream_t stream);

@@ -786,6 +786,16 @@ int64_t fa_dev_attention_shared_workspace(int64_t prefix_len, int64_t suffix_cap
   return attention_shared_workspace(prefix_len, suffix_capacity, sequences, heads, kv_heads, head_size);
 }
 
+int64_t fa_dev_attention_packed_workspace_bound(int64_t total_q, int64_t total_k, int heads, int kv_heads,
+                                                int head_size) {
+  return attention_packed_workspace_bound(total_q, total_k, heads, kv_heads, head_size);
+}
+
+int64_t fa_dev_attention_shared_workspace_bound(int64_t prefix_len, int64_t suffix_capacity, int sequences, int heads,
+                                                int kv_heads, int head_size) {
+  return attention_shared_workspace_bound(prefix_len, suffix_capacity, sequences, heads, kv_heads, head_size);
+}
+
 int fa_dev_adjust_logits(fa_backend* b, const fa_logits_args* args, void* stream) {
   return enqueue_dev(b, args, stream, check_logits, launch_adjust_logits);
 }

@@ -21,7 +21,9 @@ another stream have to outlive the call's work (``Tensor.record_stream``).  With
 it a call runs on the backend's own stream, after what torch's current stream
 holds and before what is enqueued there next; giving the stream saves the two
 events of that.  ``workspace`` is any contiguous tensor of at least the bytes that
-the ``*_workspace`` method gives; calls that may overlap in time need one each.
+the ``*_workspace`` method gives for the call's tensors, or the
+``*_workspace_bound`` method for every call up to given sizes (a smaller batch can
+need more than a larger one); calls that may overlap in time need one each.
 """
 from __future__ import annotations
 
@@ -84,6 +86,11 @@ class DeviceOps:
         return int(lib().fa_dev_attention_packed_workspace(q.shape[0], k.shape[0], q_offsets.shape[0] - 1, q.shape[1],
                                                            k.shape[1], q.shape[2]))
 
+    @staticmethod
+    def attention_packed_workspace_bound(tokens: int, keys: int, heads: int, kv_heads: int, size: int) -> int:
+        """Bytes that are enough for every :meth:`attention_packed` of up to so many tokens and keys."""
+        return int(lib().fa_dev_attention_packed_workspace_bound(tokens, keys, heads, kv_heads, size))
+
     def attention_packed(self, q, k, v, q_offsets, k_offsets, out, *, causal: bool = True, scale: float | None = None,
                          lse=None, workspace=None, stream: int | None = None) -> bool:
         """Attention of packed sequences: q, out [tokens, heads, size]; k, v [keys, kv_heads, size].
@@ -104,6 +111,12 @@ class DeviceOps:
         """Bytes of workspace for :meth:`attention_shared` on tensors of these shapes."""
         return int(lib().fa_dev_attention_shared_workspace(prefix_k.shape[0], suffix_k.shape[1], q.shape[0], q.shape[1],
                                                            prefix_k.shape[1], q.shape[2]))
+
+    @staticmethod
+    def attention_shared_workspace_bound(prefix: int, capacity: int, sequences: int, heads: int, kv_heads: int,
+                                         size: int) -> int:
+        """Bytes that are enough for every :meth:`attention_shared` of up to this prefix, capacity and batch."""
+        return int(lib().fa_dev_attention_shared_workspace_bound(prefix, capacity, sequences, heads, kv_heads, size))
 
     def attention_shared(self, q, prefix_k, prefix_v, suffix_k, suffix_v, suffix_lens, out, *,
                          scale: float | None = None, lse=None, workspace=None, stream: int | None = None) -> bool:

@@ -393,11 +393,14 @@ typedef struct fa_attention_packed_args {
   int32_t reserved;         /* 0 */
 } fa_attention_packed_args;
 int fa_dev_attention_packed(fa_backend* backend, const fa_attention_packed_args* args, void* stream);
-/* Bytes of workspace a call of these sizes needs (0: none).  Smaller calls can need
- * more than larger ones, which leave no SM idle: the maximum over a program's
- * sizes serves them all. */
+/* Bytes of workspace a call of exactly these sizes needs (0: none).  Smaller calls
+ * can need more than larger ones, which leave no SM idle. */
 int64_t fa_dev_attention_packed_workspace(int64_t total_q, int64_t total_k, int sequences, int heads, int kv_heads,
                                           int head_size);
+/* Bytes that are enough for every call of up to total_q queries and total_k keys in any
+ * number of sequences: what a program with changing batches allocates once. */
+int64_t fa_dev_attention_packed_workspace_bound(int64_t total_q, int64_t total_k, int heads, int kv_heads,
+                                                int head_size);
 
 /* Attention of one query token per sequence over a prefix that all sequences
  * share followed by the sequence's own keys: what decoding sessions of one
@@ -427,8 +430,13 @@ typedef struct fa_attention_shared_args {
   float scale;
 } fa_attention_shared_args;
 int fa_dev_attention_shared(fa_backend* backend, const fa_attention_shared_args* args, void* stream);
+/* As for fa_dev_attention_packed: the bytes of a call of exactly these sizes (a batch
+ * that lost a session can need more), and bytes that are enough for every call of up
+ * to this prefix, capacity and number of sequences. */
 int64_t fa_dev_attention_shared_workspace(int64_t prefix_len, int64_t suffix_capacity, int sequences, int heads,
                                           int kv_heads, int head_size);
+int64_t fa_dev_attention_shared_workspace_bound(int64_t prefix_len, int64_t suffix_capacity, int sequences, int heads,
+                                                int kv_heads, int head_size);
 
 /* What changes the logits between the lm_head and the greedy pick
  * (QwenDecoder.cs:262-268, 278-326), and that pick.  For every row, in 32 bits

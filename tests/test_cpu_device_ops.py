@@ -249,3 +249,44 @@ def test_binding_refuses_tensors_that_require_grad(built_lib):
                 fn(*with_grad)
             with torch.no_grad(), pytest.raises(ValueError, match="not on the backend's device"):
                 fn(*with_grad)
+
+
+def test_workspace_bounds_hold_for_every_smaller_call(built_lib):
+    """Sizes that grow when a batch shrinks, then random ones: no call up to the given sizes needs more than their bound,
+    and bounds grow with the sizes."""
+    import random
+
+    from funasrnet_b200._lib import lib
+
+    packed_size, packed_bound = lib().fa_dev_attention_packed_workspace, lib().fa_dev_attention_packed_workspace_bound
+    shared_size, shared_bound = lib().fa_dev_attention_shared_workspace, lib().fa_dev_attention_shared_workspace_bound
+    assert packed_size(300, 1000, 1, 16, 8, 128) < packed_size(100, 1000, 1, 16, 8, 128) <= packed_bound(300, 1000, 16, 8, 128)
+    assert shared_size(2048, 4000, 4, 16, 8, 128) < shared_size(2048, 4000, 3, 16, 8, 128)
+    assert shared_size(2048, 4000, 3, 16, 8, 128) <= shared_bound(2048, 4000, 4, 16, 8, 128)
+    assert shared_size(2048, 100, 85, 16, 8, 128) <= shared_bound(2048, 100, 86, 16, 8, 128)
+    rng = random.Random(17)
+
+    def size(lo, hi):
+        return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+    for _ in range(4000):
+        kv_heads, group, head = rng.choice([1, 2, 8, 16]), rng.choice([1, 2, 3, 7, 8, 64]), rng.choice([8, 64, 72, 128])
+        heads = kv_heads * group
+        q, k = size(1, 60000), size(1, 1 << 22)
+        bound = packed_bound(q, k, heads, kv_heads, head)
+        assert bound <= packed_bound(2 * q, k, heads, kv_heads, head) and bound <= packed_bound(q, 3 * k, heads, kv_heads, head)
+        for _ in range(25):
+            assert packed_size(size(1, q), size(1, k), size(1, 200), heads, kv_heads, head) <= bound
+        prefix, cap, n = size(1, 300000) - 1, size(1, 20000) - 1, size(1, 600)
+        bound = shared_bound(prefix, cap, n, heads, kv_heads, head)
+        for bigger in ((2 * prefix, cap, n), (prefix, 2 * cap, n), (prefix, cap, 2 * n)):
+            assert bound <= shared_bound(*bigger, heads, kv_heads, head)
+        for _ in range(25):
+            assert shared_size(size(1, prefix + 1) - 1, size(1, cap + 1) - 1, size(1, n), heads, kv_heads, head) <= bound
+        assert shared_size(prefix, cap, n, heads, kv_heads, head) <= bound
+    # Nothing to cut, sizes out of range, and the largest.
+    assert packed_bound(100, 511, 16, 8, 128) == 0 and shared_bound(0, 300, 500, 16, 8, 128) == 0
+    assert packed_bound(-1, 5, 8, 8, 128) == packed_bound(5, 5, 15, 8, 128) == shared_bound(5, 5, 0, 8, 8, 128) == 0
+    assert 0 < packed_bound(1 << 62, 1 << 62, 16, 8, 128) < 1 << 30
+    assert 0 < shared_bound((1 << 63) - 1, (1 << 63) - 1, 100, 16, 8, 128) < 1 << 30
+    assert shared_bound(1 << 40, 1 << 40, (1 << 31) - 1, (1 << 31) - 1, (1 << 31) - 1, 128) > 0

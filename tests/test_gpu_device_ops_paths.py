@@ -166,3 +166,39 @@ def test_logits_ties_between_touched_and_untouched_tokens(dev, rows, vocab):
         assert tokens.tolist() == [min(p) for p in mine]
         for r, p in enumerate(mine):
             assert (out[r, list(p)] == 2.0).all()
+
+
+# ------------------------------------------------------ one workspace for all batches ----
+
+
+def test_one_workspace_serves_a_batch_that_shrinks(dev):
+    """Sessions end and prompts arrive in other numbers: a workspace of the bound's size, and not a byte more, is enough."""
+    torch = torch_()
+    heads, kv_heads, size, dt = 16, 8, 128, dtype_of("bf16")
+
+    def guarded(n):
+        store = torch.full((n + 256,), 77, dtype=torch.uint8, device="cuda")
+        return store[:n], store[n:]
+
+    prefix, cap, most = 2048, 4000, 6
+    space, guard = guarded(dev.attention_shared_workspace_bound(prefix, cap, most, heads, kv_heads, size))
+    q, pk, pv = randn(1, most, heads, size, dtype=dt), *(randn(i, prefix, kv_heads, size, dtype=dt) for i in (2, 3))
+    sk, sv = (randn(i, most, cap, kv_heads, size, dtype=dt) for i in (4, 5))
+    lens = [70, 4000, 0, 999, 1, 333]
+    for n in range(most, 0, -1):
+        out, lse = torch.zeros_like(q[:n]), torch.zeros(n, heads, device="cuda")
+        assert dev.attention_shared(q[:n], pk, pv, sk[:n], sv[:n], i32(lens[:n]), out, lse=lse, workspace=space, stream=here())
+        torch.cuda.synchronize()
+        check_shared(q[:n], pk, pv, sk[:n], sv[:n], lens[:n], size ** -0.5, out, lse)
+        assert (guard == 77).all()
+    total_q, total_k = 400, 9000
+    space, guard = guarded(dev.attention_packed_workspace_bound(total_q, total_k, heads, kv_heads, size))
+    q, k, v = randn(1, total_q, heads, size, dtype=dt), *(randn(i, total_k, kv_heads, size, dtype=dt) for i in (2, 3))
+    for new, keys in (([400], [9000]), ([300], [1000]), ([100], [1000]), ([1], [9000]), ([64, 1, 7], [64, 6000, 77])):
+        a, b = sum(new), sum(keys)
+        out, lse = torch.zeros_like(q[:a]), torch.zeros(a, heads, device="cuda")
+        assert dev.attention_packed(q[:a], k[:b], v[:b], i32(sums(new)), i32(sums(keys)), out, lse=lse, workspace=space,
+                                    stream=here())
+        torch.cuda.synchronize()
+        check_packed(q[:a], k[:b], v[:b], new, keys, True, size ** -0.5, out, lse)
+        assert (guard == 77).all()
