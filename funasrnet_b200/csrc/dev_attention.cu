@@ -8,7 +8,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <vector>
@@ -1524,6 +1523,7 @@ int check_attention_packed(const fa_attention_packed_args* a) {
   if (packed_ctas(*a) >= (1ll << 30)) return kDeclined;
   need(a->q && a->out && a->q_offsets && a->k_offsets, "null q, out, q_offsets or k_offsets");
   need(a->total_k == 0 || (a->k && a->v), "null k or v");
+  need(aligned_to(4, {a->lse, a->q_offsets, a->k_offsets}), "lse or offsets not aligned to 4 bytes");
   const int64_t extents[2] = {a->total_q, a->heads};
   need(apart(a->out_stride, extents, a->head_size), "rows of out overlap");
   if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out)) return kDeclined;
@@ -1557,6 +1557,7 @@ int check_attention_shared(const fa_attention_shared_args* a) {
   need(a->prefix_len == 0 || (a->prefix_k && a->prefix_v), "null prefix_k or prefix_v");
   need(a->suffix_capacity == 0 || (a->suffix_k && a->suffix_v && a->suffix_lens),
        "null suffix_k, suffix_v or suffix_lens");
+  need(aligned_to(4, {a->lse, a->suffix_lens}), "lse or suffix_lens not aligned to 4 bytes");
   const int64_t extents[2] = {a->sequences, a->heads};
   need(apart(a->out_stride, extents, a->head_size), "rows of out overlap");
   if (!aligned16(a->q) || !aligned16(a->prefix_k) || !aligned16(a->prefix_v) || !aligned16(a->suffix_k) ||

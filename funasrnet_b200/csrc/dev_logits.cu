@@ -446,6 +446,10 @@ int check_logits(const fa_logits_args* a) {
   if (a->vocab > FA_LOGITS_MAX_VOCAB || a->rows > (1 << 27)) return kDeclined;
   if (a->rows == 0) return kHandled;
   need(a->logits && a->out, "null logits or out");
+  need(aligned_to(a->dtype == FA_DTYPE_F32 ? 4 : 2, {a->logits, a->out}), "logits or out not aligned to their type");
+  need(aligned_to(4, {a->tokens, a->history, a->history_offsets, a->prompt_lens, a->repetition, a->presence, a->frequency,
+                      a->bias_tokens, a->bias_values, a->bias_offsets, a->mask, a->mask_rows}),
+       "an array not aligned to 4 bytes");
   const int64_t far = 1ll << 34;
   need(a->logits_stride >= 0 && a->out_stride >= 0 && a->mask_stride >= 0, "negative stride");
   need(a->rows == 1 || (a->logits_stride < far && a->out_stride < far), "a stride is beyond 2^34 elements");

@@ -4,6 +4,9 @@
 
 #include <cuda_runtime.h>
 
+#include <cstdint>
+#include <initializer_list>
+
 #include "../../include/funasr_cuda.h"
 #include "fa_common.h"
 
@@ -13,6 +16,13 @@ namespace fa {
 static_assert(sizeof(fa_attention_packed_args) == 184 && sizeof(fa_attention_shared_args) == 232 &&
                   sizeof(fa_logits_args) == 168,
               "argument struct layout");
+
+// Whether all addresses are multiples of `size`, which the device faults without.
+inline bool aligned_to(uintptr_t size, std::initializer_list<const void*> addresses) {
+  for (const void* p : addresses)
+    if (reinterpret_cast<uintptr_t>(p) % size != 0) return false;
+  return true;
+}
 
 // kHandled, or kDeclined for sizes and alignments outside the kernels; throws
 // on inconsistent arguments.  Host checks only: no device is needed.

@@ -334,7 +334,8 @@ int fa_lm_head_argmax_noalloc(fa_backend* backend, const fa_weight* weight, cons
  *    (on two streams, in two graphs) need a workspace each.
  *  - Strides count elements.  The innermost dimension is contiguous.
  *  - FA_DECLINED, with the outputs untouched, for shapes and alignments outside
- *    the limits given at each call; FA_ERR_ARGUMENT for inconsistent arguments.
+ *    the limits given at each call; FA_ERR_ARGUMENT for inconsistent arguments,
+ *    and for addresses that are no multiple of their element's size.
  *  - Offsets and lengths are read on the device and clamped to the extents that
  *    the struct gives: wrong ones give unspecified results, never an access
  *    outside the arrays.

@@ -290,3 +290,35 @@ def test_workspace_bounds_hold_for_every_smaller_call(built_lib):
     assert 0 < packed_bound(1 << 62, 1 << 62, 16, 8, 128) < 1 << 30
     assert 0 < shared_bound((1 << 63) - 1, (1 << 63) - 1, 100, 16, 8, 128) < 1 << 30
     assert shared_bound(1 << 40, 1 << 40, (1 << 31) - 1, (1 << 31) - 1, (1 << 31) - 1, 128) > 0
+
+
+@pytest.mark.parametrize("make,change", [
+    (packed, dict(lse=66)),
+    (packed, dict(q_offsets=65)),
+    (packed, dict(k_offsets=62)),
+    (shared, dict(lse=2)),
+    (shared, dict(suffix_lens=67)),
+    (logits, dict(logits=(1 << 20) + 2)),
+    (logits, dict(out=(1 << 22) + 1)),
+    (logits, dict(dtype=BF16, logits=(1 << 20) + 1)),
+    (logits, dict(tokens=65)),
+    (logits, dict(history=66, history_offsets=64)),
+    (logits, dict(history=64, history_offsets=66)),
+    (logits, dict(prompt_lens=66)),
+    (logits, dict(repetition=66)),
+    (logits, dict(presence=66)),
+    (logits, dict(frequency=66)),
+    (logits, dict(bias_tokens=66, bias_values=64, bias_offsets=64)),
+    (logits, dict(bias_tokens=64, bias_values=66, bias_offsets=64)),
+    (logits, dict(bias_tokens=64, bias_values=64, bias_offsets=66)),
+    (logits, dict(mask=66, mask_count=4, mask_stride=32)),
+    (logits, dict(mask_rows=66)),
+])
+def test_addresses_off_their_types_are_refused(call, make, change):
+    """The device would fault on them."""
+    rc, message = call(make(**change))
+    assert rc == ARGUMENT and "aligned" in message, message
+
+
+def test_half_rows_on_two_bytes_are_taken(call):
+    assert call(logits(dtype=F16, logits=(1 << 20) + 2, out=(1 << 22) + 6)) == (ARGUMENT, "null backend")
