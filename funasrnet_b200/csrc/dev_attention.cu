@@ -1353,6 +1353,9 @@ void encode_q(CUtensorMap* m, int dtype, const void* base, int head_size, int gr
 }
 
 constexpr int kSms = 148;
+// The kernel adds keys and the rows of a CTA's tiles to a token's number in 32 bits.
+constexpr int64_t kMostSum = (1ll << 31) - 1024;
+static_assert(2 * kRows <= 1024 && 2 * kKeys <= 1024, "sums of a token and a tile");
 constexpr int kMaxCluster = 8;   // splits of attention_rows_kernel that a cluster joins
 // Key tiles of a sequence up to which a CTA takes one tile of rows (W = 1): nine
 // sequences of 100 to 1500 frames take 69 us so and 81 with W = 2, two prompts of
@@ -1518,7 +1521,9 @@ int check_attention_packed(const fa_attention_packed_args* a) {
   need_strides(a->v_stride, 2);
   need_strides(a->out_stride, 2);
   if (!heads_supported(a->dtype, a->heads, a->kv_heads, a->head_size)) return kDeclined;
-  if (a->total_q >= (1ll << 31) || a->total_q * a->heads >= (1ll << 31) || a->total_k >= (1ll << 30)) return kDeclined;
+  if (a->total_q >= (1ll << 31) || a->total_q * a->heads >= (1ll << 31) || a->total_k >= (1ll << 30) ||
+      a->total_q + a->total_k > kMostSum)
+    return kDeclined;
   if (a->total_q == 0 || a->sequences == 0) return kHandled;
   if (packed_ctas(*a) >= (1ll << 30)) return kDeclined;
   need(a->q && a->out && a->q_offsets && a->k_offsets, "null q, out, q_offsets or k_offsets");
@@ -1549,7 +1554,7 @@ int check_attention_shared(const fa_attention_shared_args* a) {
   need_strides(a->suffix_v_stride, 3);
   need_strides(a->out_stride, 2);
   if (!heads_supported(a->dtype, a->heads, a->kv_heads, a->head_size)) return kDeclined;
-  if ((int64_t)a->sequences * a->heads >= (1ll << 31) || std::max(a->prefix_len, a->suffix_capacity) >= (1ll << 30) ||
+  if ((int64_t)a->sequences * a->heads >= (1ll << 31) || a->sequences > kMostSum || std::max(a->prefix_len, a->suffix_capacity) >= (1ll << 30) ||
       a->prefix_len + a->suffix_capacity >= (1ll << 30))
     return kDeclined;
   if (a->sequences == 0) return kHandled;

@@ -372,7 +372,8 @@ int fa_dev_fault_test(fa_backend* backend, void* stream);
  * Limits (else FA_DECLINED): FA_DTYPE_F16 or FA_DTYPE_BF16; head_size a multiple
  * of 8 up to 128; heads / kv_heads up to 64; every base address, and every stride
  * of a dimension longer than one, a multiple of 16 bytes;
- * total_q * heads below 2^31, total_k below 2^30, and not more (sequences +
+ * total_q * heads below 2^31, total_k below 2^30, total_q + total_k (and a shared
+ * call's sequences) up to 2^31 - 1024, and not more (sequences +
  * total_q * heads / 128) * kv_heads than about 2^30; scale above 0 (else FA_ERR_ARGUMENT). */
 typedef struct fa_attention_packed_args {
   const void* q;            /* [total_q x heads x head_size] */

@@ -322,3 +322,18 @@ def test_addresses_off_their_types_are_refused(call, make, change):
 
 def test_half_rows_on_two_bytes_are_taken(call):
     assert call(logits(dtype=F16, logits=(1 << 20) + 2, out=(1 << 22) + 6)) == (ARGUMENT, "null backend")
+
+
+@pytest.mark.parametrize("make,change", [
+    (packed, dict(total_q=(1 << 31) - 100, total_k=50, heads=1, kv_heads=1)),
+    (packed, dict(total_q=(1 << 31) - (1 << 20), total_k=1 << 20, heads=1, kv_heads=1)),
+    (shared, dict(sequences=(1 << 31) - 100, heads=1, kv_heads=1)),
+])
+def test_sizes_whose_sums_pass_32_bits_are_declined(call, make, change):
+    """The kernels add a tile's rows to a token, and keys to tokens, in 32 bits."""
+    assert call(make(**change))[0] == DECLINED
+
+
+def test_the_largest_sums_are_taken(call):
+    change = dict(total_q=(1 << 31) - (1 << 20), total_k=(1 << 20) - 1024, heads=1, kv_heads=1)
+    assert call(packed(**change)) == (ARGUMENT, "null backend")
