@@ -136,3 +136,57 @@ def test_tensors_that_require_grad_are_refused_and_inference_tensors_taken(dev):
     assert dev.attention_packed(q, k, k, off, ko, out2, stream=here())  # an inference tensor outside that mode
     torch.cuda.synchronize()
     assert torch.equal(out, out2)
+
+
+def test_graphs_of_every_chain_of_kernels_replayed_at_once(dev):
+    """Two captured graphs with a workspace each, of the calls that launch several kernels (packed keys cut and joined; the
+    prefix on the tensor cores, own keys beside it, join), replayed on two streams at once with other inputs."""
+    torch = torch_()
+    dt = dtype_of("f16")
+
+    class Chain:
+        def __init__(self, seed):
+            self.q, self.k, self.v = (randn(seed + i, n, h, 128, dtype=dt) for i, (n, h) in enumerate(((64, 16), (2600, 8), (2600, 8))))
+            self.sk, self.sv = (randn(seed + i, 64, 90, 8, 128, dtype=dt) for i in (3, 4))
+            self.qo, self.ko = i32([0, 1, 64]), i32([0, 2000, 2600])
+            self.lens = i32([(seed + 7 * i) % 91 for i in range(64)])
+            self.outs = [torch.zeros_like(self.q), torch.zeros(64, 16, device="cuda"), torch.zeros_like(self.q),
+                         torch.zeros(64, 16, device="cuda")]
+            self.spaces = [packed_space(dev, self.q, self.k, self.qo), shared_space(dev, self.q, self.k, self.sk)]
+            assert all(s.numel() > 16 for s in self.spaces)
+
+        def __call__(self):
+            for _ in range(3):  # the second call's kernels follow the first one's in the same workspace
+                assert dev.attention_packed(self.q, self.k, self.v, self.qo, self.ko, self.outs[0], lse=self.outs[1],
+                                            workspace=self.spaces[0], stream=here())
+                assert dev.attention_shared(self.q, self.k, self.v, self.sk, self.sv, self.lens, self.outs[2], lse=self.outs[3],
+                                            workspace=self.spaces[1], stream=here())
+
+    chains = [Chain(1), Chain(50)]
+    for c in chains:
+        c()
+    torch.cuda.synchronize()
+    graphs = []
+    for c in chains:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            c()
+    streams = [torch.cuda.Stream() for _ in chains]
+    for turn in range(4):
+        want = []
+        for c in chains:
+            c.q.copy_(randn(100 + turn, *c.q.shape, dtype=dt))
+            c()
+            torch.cuda.synchronize()
+            want.append([o.clone() for o in c.outs])
+            for o in c.outs:
+                o.zero_()
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                for _ in range(3):
+                    g.replay()
+        torch.cuda.synchronize()
+        for c, w in zip(chains, want):
+            assert all(torch.equal(a, b) for a, b in zip(c.outs, w)), f"turn {turn}"
+    dev.status()
