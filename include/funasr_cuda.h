@@ -405,11 +405,13 @@ int64_t fa_dev_attention_packed_workspace_bound(int64_t total_q, int64_t total_k
                                                 int head_size);
 
 /* Attention of one query token per sequence over a prefix that all sequences
- * share followed by the sequence's own keys: what decoding sessions of one
- * prompt computes (fa_session_share_prefix), with the prefix stored and read once
- * for the whole batch.  Sequence b sees the prefix_len prefix keys and the first
- * suffix_lens[b] of its suffix_capacity own ones (what lies behind is not used).
- * Formula, precision, empty rows and limits as fa_dev_attention_packed. */
+ * share followed by the sequence's own keys, with the prefix stored and read once
+ * for the whole batch (fa_session_share_prefix copies it into every session; the
+ * sessions' own caches have another layout and are not given out).  Sequence b
+ * sees the prefix_len prefix keys and the first suffix_lens[b] of its
+ * suffix_capacity own ones (what lies behind is not used).
+ * Formula, precision, empty rows and limits as fa_dev_attention_packed;
+ * sequences * heads below 2^31, prefix_len + suffix_capacity below 2^30. */
 typedef struct fa_attention_shared_args {
   const void* q;               /* [sequences x heads x head_size] */
   const void* prefix_k;        /* [prefix_len x kv_heads x head_size] */
@@ -455,7 +457,7 @@ int64_t fa_dev_attention_shared_workspace_bound(int64_t prefix_len, int64_t suff
  * was generated.  Ids outside the vocabulary are ignored.  Bit t % 32 of word
  * t / 32 of mask row mask_rows[r] allows token t; a negative or too large
  * mask_rows[r] allows every token.
- * Limits (else FA_DECLINED): vocab up to FA_LOGITS_MAX_VOCAB. */
+ * Limits (else FA_DECLINED): vocab up to FA_LOGITS_MAX_VOCAB, rows up to 2^27. */
 #define FA_LOGITS_MAX_VOCAB 16777216
 typedef struct fa_logits_args {
   const void* logits;               /* [rows x vocab] */
