@@ -20,7 +20,8 @@ grad mode is on, and a call raises the version of the tensors that it writes.
 another stream have to outlive the call's work (``Tensor.record_stream``).  Without
 it a call runs on the backend's own stream, after what torch's current stream
 holds and before what is enqueued there next; giving the stream saves the two
-events of that.  ``workspace`` is any contiguous tensor of at least the bytes that
+events of that, and keeps the backend's stream out of a capture while other threads
+use it.  ``workspace`` is any contiguous tensor of at least the bytes that
 the ``*_workspace`` method gives for the call's tensors, or the
 ``*_workspace_bound`` method for every call up to given sizes (a smaller batch can
 need more than a larger one); calls that may overlap in time need one each.
